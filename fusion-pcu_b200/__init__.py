@@ -21,7 +21,9 @@ __all__ = [
     "matmul_host_scratch", "strict_matmul_host_left", "strict_matmul_epilogue", "EpilogueStage", "strict_sgd",
     "strict_mse", "mse_workspace", "strict_mse_segment_prepare", "strict_mse_segment_walk", "strict_mse_sgd",
     "strict_mse_sgd_segment_prepare", "strict_mse_sgd_segment", "checked_binary", "checked_relu", "checked_relu_backward", "matmul_fault", "sgd_fault",
-    "mse_fault", "element_fault", "GuardedChain", "CHAIN_OUTCOMES", "chain_validate", "wait",
+    "mse_fault", "element_fault", "GuardedChain", "CHAIN_OUTCOMES", "chain_validate", "wait", "group_norm",
+    "group_norm_backward", "distill_loss", "distill_loss_backward", "distill_loss_step", "block_quantize",
+    "block_matmul",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -145,6 +147,22 @@ def _declare(L):
     L.pcu_b200_guarded_checked_relu_backward.argtypes = [i32, i32, vp, vp, vp, u64, vp, u32, vp]
     L.pcu_b200_chain_validate.argtypes = [vp, u32, vp, ctypes.POINTER(i32), ctypes.POINTER(u32)]
     L.pcu_b200_wait.argtypes = [vp, u32]
+    L.pcu_b200_group_norm_workspace_size.argtypes = [i32, u64, u64, u64, u64]
+    L.pcu_b200_group_norm_workspace_size.restype = sz
+    L.pcu_b200_group_norm_backward_workspace_size.argtypes = [i32, u64, u64, u64, u64]
+    L.pcu_b200_group_norm_backward_workspace_size.restype = sz
+    learn = {  # arguments in front of (status, stream)
+        "group_norm": [i32, i32, vp, vp, vp, vp, vp, u64, u64, u64, u64, u64, u64, u64, u64, u32, vp, sz],
+        "group_norm_backward": [i32, i32] + [vp] * 8 + [u64] * 10 + [vp, sz],
+        "distill_loss": [i32, vp, u64, u64, u64, vp, vp, u64, vp, u32, vp, vp],
+        "distill_loss_backward": [i32, vp, u64, u64, u64, vp, vp, u64, vp, u32, vp, vp, i32, vp, u64],
+        "distill_loss_step": [i32, vp, u64, u64, u64, vp, vp, u64, vp, u32, vp, vp, vp, i32, vp, u64],
+        "block_quantize": [i32, vp, u64, u64, u64, i32, vp, u64, vp],
+        "block_matmul": [i32, vp, vp, vp, vp, vp, u64, u64, u64, u64, u64, u64],
+    }
+    for name, args in learn.items():
+        getattr(L, "pcu_b200_" + name).argtypes = args + [vp, vp]
+        getattr(L, "pcu_b200_guarded_" + name).argtypes = args + [vp, u32, vp]
     L.pcu_b200_last_comm_error.restype = i32
     L.pcu_b200_comm_unique_id.argtypes = [vp]
     L.pcu_b200_comm_init.argtypes = [vp, i32, i32, ctypes.POINTER(vp)]
@@ -626,3 +644,7 @@ def wait(stream=None, timeout_ms=1000):
         return False
     _check(rc)
     return True
+
+
+from .learn import (block_matmul, block_quantize, distill_loss, distill_loss_backward, distill_loss_step,  # noqa: E402
+                    group_norm, group_norm_backward)

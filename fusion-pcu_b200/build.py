@@ -1,7 +1,8 @@
 """Build the provider's shared library, fusion-pcu_b200/libpcu_b200.so, for sm_100a.
 
 Every kernel is compiled ahead of time (no NVRTC) with the strict arithmetic flags the
-contract needs: no FMA contraction, no flush-to-zero, IEEE division and square root.
+contract needs: no FMA contraction, no flush-to-zero, IEEE division and square root.  The
+learning operators (include/pcu_b200_learn.h), which have no strict contract, allow contraction.
 Objects go to _build/ (git-ignored); the .so stays in-tree so it travels with the repo.
 """
 import concurrent.futures
@@ -16,12 +17,16 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(ROOT, "_build", "provider")
 LIBRARY = os.path.join(HERE, "libpcu_b200.so")
 SOURCES = ["abi.cu", "streaming.cu", "strict_matmul.cu", "strict_mse.cu", "tensor_graph.cu", "host_staging.cu",
-           "comm.cu", "calibrate.cu"]
-HEADERS = ["checked_law.cuh", "common.cuh", "mse_walk_plan.h", "provider.h"]
+           "comm.cu", "calibrate.cu", "group_norm.cu", "distill.cu", "block_matmul.cu"]
+HEADERS = ["checked_law.cuh", "common.cuh", "learn.cuh", "mse_walk_plan.h", "provider.h"]
+PUBLIC = ["pcu_b200.h", "pcu_b200_graph.h", "pcu_b200_learn.h"]
+# the learning operators are not bound to the strict law's separate roundings
+CONTRACTED = {"group_norm.cu", "distill.cu", "block_matmul.cu"}
 
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 STRICT = ["--fmad=false", "--ftz=false", "--prec-div=true", "--prec-sqrt=true"]
+FLOAT = ["--fmad=true", "--ftz=false", "--prec-div=true", "--prec-sqrt=true"]
 COMMON = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC,-O2,-ffp-contract=off", "-I", os.path.join(ROOT, "include"),
           "-I", CSRC]
 
@@ -35,12 +40,11 @@ def _stale(target, deps):
 
 def _compile(src, verbose):
     obj = os.path.join(BUILD, src.replace(".cu", ".o"))
-    deps = [os.path.join(CSRC, src), os.path.join(ROOT, "include", "pcu_b200.h"),
-            os.path.join(ROOT, "include", "pcu_b200_graph.h"), __file__] + \
+    deps = [os.path.join(CSRC, src), __file__] + [os.path.join(ROOT, "include", h) for h in PUBLIC] + \
         [os.path.join(CSRC, h) for h in HEADERS]
     if not _stale(obj, deps):
         return obj, ""
-    cmd = [NVCC, "-c", os.path.join(CSRC, src), "-o", obj] + ARCH + STRICT + COMMON
+    cmd = [NVCC, "-c", os.path.join(CSRC, src), "-o", obj] + ARCH + (FLOAT if src in CONTRACTED else STRICT) + COMMON
     if verbose:
         cmd += ["-Xptxas", "-v"]
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -29,20 +29,6 @@ __global__ void chain_reset_kernel(unsigned long long *records, uint32_t stages)
     }
 }
 
-// The guard of stage `stage` of a record slab: admitted by record stage-1, deciding record
-// stage's disposition in its first kernel.
-pcu::ChainGuard slab_guard(uint64_t *records, uint32_t stage) {
-    auto *r = reinterpret_cast<unsigned long long *>(records);
-    pcu::ChainGuard g{};
-    g.disp = r + 2ull * stage + 1;
-    g.decide = 1;
-    if (stage > 0) {
-        g.prev_status = r + 2ull * (stage - 1);
-        g.prev_disp = r + 2ull * (stage - 1) + 1;
-    }
-    return g;
-}
-
 }  // namespace
 
 namespace pcu {
@@ -56,6 +42,20 @@ int chain_decide_only(const ChainGuard &guard, cudaStream_t stream) {
 }  // namespace pcu
 
 namespace pcu_host {
+
+// The guard of stage `stage` of a record slab: admitted by record stage-1, deciding record
+// stage's disposition in its first kernel.
+pcu::ChainGuard slab_guard(uint64_t *records, uint32_t stage) {
+    auto *r = reinterpret_cast<unsigned long long *>(records);
+    pcu::ChainGuard g{};
+    g.disp = r + 2ull * stage + 1;
+    g.decide = 1;
+    if (stage > 0) {
+        g.prev_status = r + 2ull * (stage - 1);
+        g.prev_disp = r + 2ull * (stage - 1) + 1;
+    }
+    return g;
+}
 
 int set_cuda_error(cudaError_t err) {
     g_last_cuda_error = (int)err;
@@ -131,7 +131,7 @@ extern "C" int pcu_b200_guarded_strict_matmul(int dtype, int policy, const void 
     if (!chain_records) return PCU_B200_ERROR_INVALID_ARGUMENT;
     return pcu::strict_matmul(dtype, policy, left, right, out, rows, inner, columns, left_stride, right_stride,
                               transpose_left, transpose_right, workspace, workspace_bytes,
-                              chain_records + 2ull * chain_stage, stream, slab_guard(chain_records, chain_stage));
+                              chain_records + 2ull * chain_stage, stream, pcu_host::slab_guard(chain_records, chain_stage));
 }
 
 extern "C" int pcu_b200_guarded_strict_sgd(int dtype, int policy, const void *weights, const void *gradient, void *out,
@@ -139,7 +139,7 @@ extern "C" int pcu_b200_guarded_strict_sgd(int dtype, int policy, const void *we
                                            uint32_t chain_stage, void *stream) {
     if (!chain_records) return PCU_B200_ERROR_INVALID_ARGUMENT;
     return pcu::strict_sgd(dtype, policy, weights, gradient, out, count, rate_bits_f32,
-                           chain_records + 2ull * chain_stage, stream, slab_guard(chain_records, chain_stage));
+                           chain_records + 2ull * chain_stage, stream, pcu_host::slab_guard(chain_records, chain_stage));
 }
 
 extern "C" int pcu_b200_guarded_strict_mse(int dtype, int policy, const void *prediction, const void *target,
@@ -147,7 +147,7 @@ extern "C" int pcu_b200_guarded_strict_mse(int dtype, int policy, const void *pr
                                            uint64_t *chain_records, uint32_t chain_stage, void *stream) {
     if (!chain_records) return PCU_B200_ERROR_INVALID_ARGUMENT;
     return pcu::strict_mse(dtype, policy, prediction, target, out, count, workspace, workspace_bytes,
-                           chain_records + 2ull * chain_stage, stream, slab_guard(chain_records, chain_stage));
+                           chain_records + 2ull * chain_stage, stream, pcu_host::slab_guard(chain_records, chain_stage));
 }
 
 extern "C" int pcu_b200_guarded_checked_binary(int dtype, int policy, int op, const void *left, const void *right,
@@ -155,14 +155,14 @@ extern "C" int pcu_b200_guarded_checked_binary(int dtype, int policy, int op, co
                                                uint64_t *chain_records, uint32_t chain_stage, void *stream) {
     if (!chain_records) return PCU_B200_ERROR_INVALID_ARGUMENT;
     return pcu::checked_binary(dtype, policy, op, left, right, out, count, left_uniform, right_uniform,
-                               chain_records + 2ull * chain_stage, stream, slab_guard(chain_records, chain_stage));
+                               chain_records + 2ull * chain_stage, stream, pcu_host::slab_guard(chain_records, chain_stage));
 }
 
 extern "C" int pcu_b200_guarded_checked_relu(int dtype, int policy, const void *input, void *out, uint64_t count,
                                              uint64_t *chain_records, uint32_t chain_stage, void *stream) {
     if (!chain_records) return PCU_B200_ERROR_INVALID_ARGUMENT;
     return pcu::checked_relu(dtype, policy, input, out, count, chain_records + 2ull * chain_stage, stream,
-                             slab_guard(chain_records, chain_stage));
+                             pcu_host::slab_guard(chain_records, chain_stage));
 }
 
 extern "C" int pcu_b200_guarded_checked_relu_backward(int dtype, int policy, const void *input, const void *upstream,
@@ -170,7 +170,7 @@ extern "C" int pcu_b200_guarded_checked_relu_backward(int dtype, int policy, con
                                                       uint32_t chain_stage, void *stream) {
     if (!chain_records) return PCU_B200_ERROR_INVALID_ARGUMENT;
     return pcu::checked_relu_backward(dtype, policy, input, upstream, out, count, chain_records + 2ull * chain_stage,
-                                      stream, slab_guard(chain_records, chain_stage));
+                                      stream, pcu_host::slab_guard(chain_records, chain_stage));
 }
 
 namespace {

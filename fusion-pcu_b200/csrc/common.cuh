@@ -85,6 +85,7 @@ namespace pcu_host {
 int set_cuda_error(cudaError_t err);  // records err for pcu_b200_last_cuda_error; returns PCU_B200_ERROR_CUDA
 int launch_status(void);              // checks cudaGetLastError after a launch
 int sm_count(void);                   // SMs of the current device (cached per device)
+pcu::ChainGuard slab_guard(uint64_t *records, uint32_t stage);  // stage `stage` of a chain's record slab
 
 inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
