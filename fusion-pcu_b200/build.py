@@ -18,7 +18,7 @@ BUILD = os.path.join(ROOT, "_build", "provider")
 LIBRARY = os.path.join(HERE, "libpcu_b200.so")
 SOURCES = ["abi.cu", "streaming.cu", "strict_matmul.cu", "strict_mse.cu", "tensor_graph.cu", "host_staging.cu",
            "comm.cu", "calibrate.cu", "group_norm.cu", "distill.cu", "block_matmul.cu"]
-HEADERS = ["checked_law.cuh", "common.cuh", "learn.cuh", "mse_walk_plan.h", "provider.h"]
+HEADERS = ["checked_law.cuh", "common.cuh", "learn.cuh", "mse_walk_plan.h", "provider.h", "tma.cuh"]
 PUBLIC = ["pcu_b200.h", "pcu_b200_graph.h", "pcu_b200_learn.h"]
 # the learning operators are not bound to the strict law's separate roundings
 CONTRACTED = {"group_norm.cu", "distill.cu", "block_matmul.cu"}

@@ -25,9 +25,6 @@
 //     cells are bit-identical to the law because no step faulted.
 //   * Shapes whose strides or base addresses TMA cannot describe use a plain tiled kernel
 //     with the same epilogue.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -35,6 +32,7 @@
 #include "common.cuh"
 #include "pcu_b200.h"
 #include "provider.h"
+#include "tma.cuh"
 
 // Tuning knobs (defaults are the measured best; override with -D for sweeps).
 #ifndef PCU_MM_UNROLL_F32
@@ -254,54 +252,6 @@ __device__ __noinline__ void exact_cell(const MatmulParams<T> &p, int np, uint64
 template <typename T>
 __device__ __forceinline__ bool needs_exact(const MatmulParams<T> &p, T acc, int rmin, int cmin) {
     return nonfinite_bits<T>(Fmt<T>::bits(acc)) || (p.row_minexp && rmin + cmin < p.threshold);
-}
-
-// ------------------------------------------------------------------ TMA / mbarrier helpers
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// Bounded wait: false after kWaitLimitNs (the caller reports kWatchdog).
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = global_ns();
-    for (;;) {
-#pragma unroll 1
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (global_ns() - t0 > kWaitLimitNs) return false;
-    }
-}
-
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
-            "r"(smem_addr(dst)),
-        "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y)
-        : "memory");
 }
 
 template <typename T> struct Tile;
@@ -614,25 +564,12 @@ namespace {
 
 using namespace pcu;
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static std::once_flag once;
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    std::call_once(once, [] {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-    });
-    return fn;
-}
-
 // 2-D tile map over a row-major matrix of `outer` rows x `inner_dim` elements with row
 // stride `ld` elements; box = box_inner x box_outer elements.
 template <typename T>
 bool make_map(CUtensorMap *map, const T *base, uint64_t inner_dim, uint64_t outer, uint64_t ld, uint32_t box_inner,
               uint32_t box_outer, bool swizzle128) {
-    auto encode = tensor_map_encoder();
+    auto encode = pcu_host::tensor_map_encoder();
     if (!encode) return false;
     if (!pcu_host::aligned(base, 16) || (ld * sizeof(T)) % 16 != 0) return false;
     if (inner_dim == 0 || outer == 0 || inner_dim >= (1ull << 31) || outer >= (1ull << 31)) return false;
