@@ -25,15 +25,67 @@ __device__ __forceinline__ float from_e4m3(unsigned code) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3)));
 }
 
-// value * (1 / scale), exact: the reciprocal of a power of two >= 2^-126 is one <= 2^126
-__device__ __forceinline__ unsigned to_e4m3(float v, float inverse) {
-    return isfinite(v) ? (unsigned)__nv_cvt_float_to_fp8(v * inverse, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
+// 16 elements from `from` on, `count` of them there, the others 0.  Whole 16-byte loads where the
+// address allows it.
+template <typename T> __device__ __forceinline__ void load_codes_input(const T *from, int count, float (&v)[16]) {
+    if (count == 16 && (reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 16; i += V) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(from + i));
+            const T *t = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i + j] = Elem<T>::load(t[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = i < count ? Elem<T>::load(from[i]) : 0.0f;
+    }
+}
+
+// The largest magnitude's bits, which order as the magnitudes do; 0x7f800000 and above: an infinity
+// or a NaN is among them.
+__device__ __forceinline__ unsigned largest_bits(const float (&v)[16]) {
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+    return most;
+}
+
+// Values that are not finite: recorded, and made NaN.  Returns the largest bits of the others.
+__device__ __forceinline__ unsigned settle(float (&v)[16], uint64_t event, unsigned long long *status) {
+    unsigned most = 0;
+    for (int i = 0; i < 16; ++i) {
+        const unsigned bits = __float_as_uint(v[i]) & 0x7fffffffu;
+        if (bits < 0x7f800000u) {
+            most = max(most, bits);
+        } else {
+            record_fault(status, event + i, PCU_B200_KIND_INVALID);
+            v[i] = NAN;
+        }
+    }
+    return most;
+}
+
+// v * inverse as codes; exact up to the rounding to a code: the inverse of a power of two >= 2^-126
+// is one <= 2^126.
+__device__ __forceinline__ void store_codes(unsigned char *to, int count, const float (&v)[16], float inverse) {
+    alignas(16) unsigned short pair[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        pair[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * inverse, v[2 * i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
+    if (count == 16 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+        *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(pair);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < count) to[i] = (unsigned char)(pair[i / 2] >> 8 * (i % 2));
+    }
 }
 
 template <typename T> struct QuantizeParams {
     const T *input;
     uint64_t rows, columns, stride;
-    int high;
     unsigned char *codes;
     uint64_t codes_stride;
     float *scales;
@@ -41,28 +93,48 @@ template <typename T> struct QuantizeParams {
     ChainGuard guard;
 };
 
-// One CTA per block.
-template <typename T> __global__ void __launch_bounds__(kBlock) quantize_kernel(const QuantizeParams<T> p) {
+// Eight threads take a row's 128 elements of a block, 16 each, and keep them in registers between
+// the maximum and the codes, so the input is read once.  HIGH 1: a block is such a row, 32 blocks per
+// CTA.  HIGH 128: a CTA takes a block, 4 rows per thread.
+constexpr int kQuantizeThreads = 256;
+
+template <typename T, int HIGH>
+__global__ void __launch_bounds__(kQuantizeThreads) quantize_kernel(const QuantizeParams<T> p) {
     if (!chain_admits(p.guard)) return;
-    __shared__ float scratch[kBlock / 32];
-    const uint64_t kb = blockIdx.x % ((p.columns + kBlock - 1) / kBlock), rb = blockIdx.x / ((p.columns + kBlock - 1) / kBlock);
-    const uint64_t c = kb * kBlock + threadIdx.x, r0 = rb * p.high, r1 = min(r0 + p.high, p.rows);
-    float amax = 0;
-    if (c < p.columns)
-        for (uint64_t r = r0; r < r1; ++r) {
-            const float v = fabsf(Elem<T>::load(p.input[r * p.stride + c]));
-            if (isfinite(v)) amax = fmaxf(amax, v);
-            else record_fault(p.status, r * p.columns + c, PCU_B200_KIND_INVALID);
-        }
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-    if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = amax;
-    __syncthreads();
-    const float scale = block_scale(fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3])));
-    if (threadIdx.x == 0) p.scales[blockIdx.x] = scale;
-    if (c < p.columns)
-        for (uint64_t r = r0; r < r1; ++r)
-            p.codes[r * p.codes_stride + c] =
-                (unsigned char)to_e4m3(Elem<T>::load(p.input[r * p.stride + c]), 1.0f / scale);
+    constexpr int kRows = kQuantizeThreads / 8, PASSES = HIGH == 1 ? 1 : HIGH / kRows;
+    const unsigned across = (unsigned)((p.columns + kBlock - 1) / kBlock);
+    const unsigned block = HIGH == 1 ? blockIdx.x * kRows + threadIdx.x / 8 : blockIdx.x;
+    const uint64_t column = (uint64_t)(block % across) * kBlock + threadIdx.x % 8 * 16;
+    const uint64_t first = HIGH == 1 ? block / across : (uint64_t)(block / across) * HIGH + threadIdx.x / 8;
+    const int count = column < p.columns ? (int)min((uint64_t)16, p.columns - column) : 0;
+    float v[PASSES][16];
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const uint64_t row = first + i * kRows;
+        load_codes_input(p.input + row * p.stride + column, row < p.rows ? count : 0, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        unsigned here = largest_bits(v[i]);
+        if (here >= 0x7f800000u) here = settle(v[i], (first + i * kRows) * p.columns + column, p.status);
+        most = max(most, here);
+    }
+    for (int o = 4; o; o >>= 1) most = max(most, __shfl_xor_sync(~0u, most, o));
+    if (HIGH > 1) {
+        __shared__ unsigned scratch[kRows];
+        if (threadIdx.x % 8 == 0) scratch[threadIdx.x / 8] = most;
+        __syncthreads();
+        most = scratch[threadIdx.x % 32];
+        for (int o = 16; o; o >>= 1) most = max(most, __shfl_xor_sync(~0u, most, o));
+    }
+    const float scale = block_scale(__uint_as_float(most)), inverse = 1.0f / scale;
+    if (first < p.rows && threadIdx.x % (HIGH == 1 ? 8 : kQuantizeThreads) == 0) p.scales[block] = scale;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const uint64_t row = first + i * kRows;
+        if (row < p.rows && count) store_codes(p.codes + row * p.codes_stride + column, count, v[i], inverse);
+    }
 }
 
 template <typename T> struct ProductParams {
@@ -407,10 +479,14 @@ template <typename T>
 static int quantize_typed(const void *input, uint64_t rows, uint64_t columns, uint64_t stride, int high, void *codes,
                           uint64_t codes_stride, float *scales, uint64_t *status, cudaStream_t stream,
                           const ChainGuard &guard) {
-    QuantizeParams<T> p{(const T *)input, rows, columns, stride, high, (unsigned char *)codes, codes_stride, scales,
+    QuantizeParams<T> p{(const T *)input, rows, columns, stride, (unsigned char *)codes, codes_stride, scales,
                         reinterpret_cast<unsigned long long *>(status), guard};
     const uint64_t blocks = (rows + high - 1) / high * ((columns + kBlock - 1) / kBlock);
-    quantize_kernel<T><<<(unsigned)blocks, kBlock, 0, stream>>>(p);
+    constexpr int kRows = kQuantizeThreads / 8;
+    if (high == 1)
+        quantize_kernel<T, 1><<<(unsigned)((blocks + kRows - 1) / kRows), kQuantizeThreads, 0, stream>>>(p);
+    else
+        quantize_kernel<T, kBlock><<<(unsigned)blocks, kQuantizeThreads, 0, stream>>>(p);
     return pcu_host::launch_status();
 }
 
