@@ -212,15 +212,14 @@ template <typename T> __global__ void __launch_bounds__(256) product_plain_kerne
 
 // ------------------------------------------------------------------ tensor core product
 //
-// D = P . Q^T over blocks of 128 of the inner dimension, P's 128 rows and Q's BN rows per tile.  The
-// tensor core cannot apply a scale that changes from block to block of its accumulator, so each
-// block's product goes to a TMEM buffer of its own and the epilogue warps add it, scaled, to
-// binary32 sums in registers while the next block's product runs.
-//   * batch form: P = left, Q = right: a tile of 128 rows x 256 columns.
-//   * row form (few rows): P = right, Q = left: 128 columns x BN rows, so that the weights, which
-//     are all the traffic there is, fill the instruction's 128 rows.  The blocks of one tile are
-//     split over a cluster's CTAs; the first CTA adds their sums, in rank order.
-// Warp 0 issues the TMA loads, warp 1 the tcgen05.mma instructions, the others drain TMEM.
+// D = P . Q^T over blocks of 128 of the inner dimension.  The tensor core cannot apply a scale that
+// changes from block to block of its accumulator, so each block's product goes to a TMEM buffer of
+// its own and the epilogue warps add it, scaled, to binary32 sums in registers while the next
+// blocks' products run.
+//   * batch form (product_kernel): P = left, Q = right.  A pair of CTAs works on 256 x 256 cells.
+//   * row form (product_rows_kernel), few rows: P = right, Q = left, 128 columns x BN rows, so that
+//     the weights, which are all the traffic there is, fill the instruction's 128 rows.  The blocks
+//     of one tile are split over a cluster's CTAs; the first CTA adds their sums, in rank order.
 // All waits are bounded (mbar_wait); one that runs out records the watchdog kind, and the CTA still
 // waits for its own copies and products before it frees TMEM and returns.
 
@@ -239,18 +238,44 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
+// True in one lane, always the same.  The warp that issues tensor core work runs its loop as a whole,
+// so that descriptors stay in uniform registers, and elects a lane for the instructions themselves;
+// a loop of one lane alone took 600 cycles to issue a block's eight products, which take 512.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t elected;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(elected));
+    return elected != 0;
+}
+
 // The barrier completes when all tensor core work issued before by this thread has.
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
                  : "memory");
 }
 
-__device__ __forceinline__ void tmem_load16(uint32_t (&v)[16], uint32_t address) {
+// This thread's lane and the columns from `address` on.
+__device__ __forceinline__ void tmem_load(uint32_t (&v)[16], uint32_t address) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        "{%0, %1, %2, %3, %4, %5, %6, %7, "
+        "%8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(address));
+}
+__device__ __forceinline__ void tmem_load(uint32_t (&v)[32], uint32_t address) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(address));
 }
 
@@ -262,23 +287,32 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                   "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
 
-template <int BN_, bool ROWS_> struct ProductShape {
-    static constexpr int BM = 128, BN = BN_;
-    static constexpr bool ROWS = ROWS_;               // the row form
-    static constexpr int EPILOGUE = BN == 256 ? 8 : 4;  // warps; warp w drains TMEM lanes 32 (w % 4)...
-    static constexpr int COLUMNS = BN / (EPILOGUE / 4);  // accumulator columns per thread
-    static constexpr int THREADS = (2 + EPILOGUE) * 32;
-    static constexpr int BUFFERS = BN == 256 ? 2 : 4;
-    static constexpr int TMEM_COLUMNS = BUFFERS * BN;
-    static constexpr int P_BYTES = BM * kBlock, Q_BYTES = BN * kBlock, STAGE_BYTES = P_BYTES + Q_BYTES;
-    static constexpr int STAGES = ROWS ? 5 : 4;
-    static constexpr int PARTIAL_BYTES = BM * BN * 4;  // one CTA's sums, handed to the cluster's first
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
-    static_assert(!ROWS || BN <= 32, "the row form keeps a column's factor in a lane");
-    static_assert(PARTIAL_BYTES <= STAGES * STAGE_BYTES || !ROWS, "the sums take the stages' place");
-};
+// Two binary32 multiply-adds in one instruction: sum += (a0 f0, a1 f1).
+__device__ __forceinline__ void fma_two(uint64_t &sum, uint32_t a0, uint32_t a1, float f0, float f1) {
+    asm("{\n\t.reg .b64 a, f;\n\t"
+        "mov.b64 a, {%1, %2};\n\tmov.b64 f, {%3, %4};\n\t"
+        "fma.rn.f32x2 %0, a, f, %0;\n\t}"
+        : "+l"(sum)
+        : "r"(a0), "r"(a1), "f"(f0), "f"(f1));
+}
 
+// A whole warp waits, with one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
+    return __all_sync(~0u, mbar_wait(bar, parity));
+}
+
+// What both forms take.  Tiles come in groups of 8 tile rows, column by column inside a group, so
+// that the tiles worked on at once share a few panels of both operands in L2.
 template <typename T> struct TileParams {
     ProductParams<T> out;
     uint64_t p_rows, q_rows;  // extents along the tile's rows and columns
@@ -287,26 +321,306 @@ template <typename T> struct TileParams {
     int blocks;  // of 128 along the inner dimension
 };
 
-template <typename T, typename S>
-__global__ void __launch_bounds__(S::THREADS, 1)
+template <typename T>
+__device__ __forceinline__ void tile_place(const TileParams<T> &t, unsigned id, unsigned &p, unsigned &q) {
+    const unsigned group = id / (8 * t.tiles_q) * 8, rows = min(8u, t.tiles_p - group), in = id - group * t.tiles_q;
+    p = group + in % rows;
+    q = in / rows;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t cluster_address(uint32_t address, uint32_t rank) {
+    uint32_t remote;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(rank));
+    return remote;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// ---- batch form
+//
+// A pair of CTAs (a cluster of 2) owns 256 x 256 cells: each holds 128 rows of P and half of Q's rows,
+// and one tcgen05.mma of the pair reads both, so each SM brings 32 KB per block of 128 from L2 where a
+// CTA by itself, with 128 x 256 cells, brings 48 KB (and was bound by that, at 10 TB/s of L2 reads).  A
+// block's product is two units of 128 columns, each with one of four TMEM buffers: a unit is drained
+// while others are computed or wait.
+// Warps: 0 TMA loads, 1 tcgen05.mma (first CTA only), 2 and 3 the rows' scales into shared memory (read
+// by each epilogue thread for itself they were 32 cache lines a load), 4 to 19 drain TMEM: warp w the
+// lanes from 32 (w % 4), every other unit and 64 of its columns.  A TMEM load takes some 200 cycles and a
+// wait waits for all of a warp's, so the drain is a chain of loads in each warp: about 550 cycles a block
+// with sixteen warps that take a unit in turn, 1,400 with eight that take half of every unit.
+struct Batch {
+    static constexpr int HALF = 128, BM = 2 * HALF, BN = 256, UNIT = 128, UNITS = BN / UNIT, BUFFERS = 4;
+    static constexpr int EPILOGUE = 16, COLUMNS = UNIT / (EPILOGUE / 4 / UNITS), PIECE = 32, THREADS = (4 + EPILOGUE) * 32;
+    // Registers a thread: of the first four warps, and of the others (64 sums, 32 on their way).  The
+    // launch gives every thread what the bounds allow, LAUNCHED, and the warps share it anew.
+    static constexpr int LAUNCHED = 96, SERVING = 32, DRAINING = 112;
+    static_assert(4 * SERVING + EPILOGUE * DRAINING <= (4 + EPILOGUE) * LAUNCHED, "a larger share would wait forever");
+    static constexpr int TMEM_COLUMNS = BUFFERS * UNIT;
+    static constexpr int P_BYTES = HALF * kBlock, Q_BYTES = BN / 2 * kBlock, STAGE_BYTES = P_BYTES + Q_BYTES;
+    static constexpr int STAGES = 6, CHUNK = 16;  // blocks of scales per chunk
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+};
+
+// A load by either CTA of a pair that signals the first CTA's barrier.
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(shape), "r"(add)
+        : "memory");
+}
+
+// The barrier at this place in both CTAs completes when the pair's products issued before have.
+__device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+// An arrival at a barrier of any CTA of the cluster, for a TMEM buffer that has been read: nothing in
+// memory is handed over (the loads have ended and tcgen05.fence orders them), so it is relaxed.  A
+// release at cluster scope waits for all of the thread's memory accesses, 1,000 cycles here.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ TileParams<T> t) {
+    using S = Batch;
     const ProductParams<T> &p = t.out;
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ unsigned char smem_raw[];
-    unsigned char *const tiles = smem_raw + (1024 - (smem_addr(smem_raw) & 1023) & 1023);
+    unsigned char *const tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], ready[S::BUFFERS], drained[S::BUFFERS], scaled[2], spent[2];
+    __shared__ uint64_t finished;
+    __shared__ uint32_t tmem_base;
+    __shared__ float row_scale[2][S::CHUNK][S::HALF + 1], column_scale[2][S::CHUNK][S::UNITS];
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // uniform, for the compiler too
+    const uint32_t rank = cluster_rank();
+    const unsigned first = blockIdx.x / 2, step = gridDim.x / 2;
+    const int KB = t.blocks;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < S::BUFFERS; ++i) mbar_init(&ready[i], 1), mbar_init(&drained[i], 2 * S::EPILOGUE / S::UNITS);
+        for (int i = 0; i < 2; ++i) mbar_init(&scaled[i], 2), mbar_init(&spent[i], S::EPILOGUE);
+        mbar_init(&finished, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(S::TMEM_COLUMNS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();  // the other CTA's barriers are initialised and its TMEM is allocated
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = __shfl_sync(~0u, tmem_base, 0);
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::SERVING));
+        if (warp == 0) {
+            if (lane == 0) {
+                int it = 0;
+                bool ok = true;
+                for (unsigned id = first; ok && id < t.tiles; id += step) {
+                    unsigned tp, tq;
+                    tile_place(t, id, tp, tq);
+                    const int p0 = (int)(tp * S::BM + rank * S::HALF), q0 = (int)(tq * S::BN + rank * (S::UNIT / 2));
+                    for (int kb = 0; kb < KB; ++kb, ++it) {
+                        const int s = it % S::STAGES;
+                        if (!(ok = mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1))) break;
+                        unsigned char *to = tiles + s * S::STAGE_BYTES;
+                        const uint32_t bar = cluster_address(smem_addr(&full[s]), 0);
+                        if (rank == 0) mbar_expect_tx(&full[s], 2 * S::STAGE_BYTES);  // both CTAs' loads
+                        tma_load_pair(to, &map_p, bar, kb * kBlock, p0);
+#pragma unroll
+                        for (int u = 0; u < S::UNITS; ++u)  // this CTA's half of each unit's columns
+                            tma_load_pair(to + S::P_BYTES + u * (S::UNIT / 2) * kBlock, &map_q, bar, kb * kBlock, q0 + u * S::UNIT);
+                    }
+                }
+                if (!ok) record_fault(p.status, 0, kWatchdog);
+                // Nothing is left in flight towards either CTA's shared memory when the pair ends.
+                if (rank == 0)
+                    for (int i = it > S::STAGES ? it - S::STAGES : 0; i < it; ++i)
+                        mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
+            }
+        } else if (warp == 1) {
+            if (rank == 0) {
+                constexpr uint32_t shape = 1u << 4 | (uint32_t)(S::UNIT / 8) << 17 | (uint32_t)(S::BM / 16) << 24;
+                const uint32_t stage0 = smem_addr(tiles);
+                int it = 0, unit = 0;
+                bool ok = true;
+                for (unsigned id = first; ok && id < t.tiles; id += step)
+                    for (int kb = 0; ok && kb < KB; ++kb, ++it) {
+                        const int s = it % S::STAGES;
+                        if (!(ok = warp_wait(&full[s], (it / S::STAGES) & 1))) break;
+                        const uint64_t pd = k_major_descriptor(stage0 + s * S::STAGE_BYTES);
+#pragma unroll
+                        for (int u = 0; u < S::UNITS; ++u, ++unit) {
+                            const int b = unit % S::BUFFERS;
+                            if (!(ok = __all_sync(~0u, mbar_wait_cluster(&drained[b], ((unit / S::BUFFERS) & 1) ^ 1)))) break;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            const uint64_t qd = pd + ((S::P_BYTES + u * (S::UNIT / 2) * kBlock) >> 4);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further along the swizzled rows
+                                    mma_pair(tmem + b * S::UNIT, pd + 2 * k, qd + 2 * k, shape, k != 0);
+                                mma_commit_pair(&ready[b]);
+                                if (u + 1 == S::UNITS) mma_commit_pair(&empty[s]);
+                            }
+                            __syncwarp();
+                        }
+                    }
+                if (elect_one()) mma_commit_pair(&finished);
+                __syncwarp();
+                ok = warp_wait(&finished, 0) && ok;
+                if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
+            }
+        } else {
+            int chunk = 0;
+            bool ok = true;
+            for (unsigned id = first; ok && id < t.tiles; id += step) {
+                unsigned tp, tq;
+                tile_place(t, id, tp, tq);
+                const uint64_t row0 = (uint64_t)tp * S::BM + rank * S::HALF + (warp - 2) * (S::HALF / 2);
+                for (int k0 = 0; k0 < KB; k0 += S::CHUNK, ++chunk) {
+                    const int c = chunk & 1, kb = k0 + lane % S::CHUNK;
+                    if (!(ok = warp_wait(&spent[c], ((chunk / 2) & 1) ^ 1))) break;
+#pragma unroll 8
+                    for (int r = lane / S::CHUNK; r < S::HALF / 2; r += 32 / S::CHUNK)
+                        row_scale[c][lane % S::CHUNK][(warp - 2) * (S::HALF / 2) + r] =
+                            kb < KB && row0 + r < t.p_rows ? t.p_scales[(row0 + r) * KB + kb] : 0.0f;
+                    if (warp == 2) {
+                        const uint64_t block = (uint64_t)tq * S::UNITS + lane / S::CHUNK;
+                        static_assert(32 / S::CHUNK == S::UNITS, "a lane for each unit's scale of each block");
+                        column_scale[c][lane % S::CHUNK][lane / S::CHUNK] =
+                            kb < KB && block * kBlock < t.q_rows ? t.q_scales[block * KB + kb] : 0.0f;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&scaled[c]);
+                }
+            }
+            if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::DRAINING));
+        const int quarter = warp % 4, local = quarter * 32 + lane;  // this thread's row of the CTA's half
+        const int u = (warp - 4) / (S::EPILOGUE / S::UNITS);        // the unit of each block that this warp takes
+        const int from = (warp - 4) / 4 % (S::EPILOGUE / 4 / S::UNITS) * S::COLUMNS;  // its first column in it
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + from;
+        const uint32_t drained0 = cluster_address(smem_addr(&drained[0]), 0);
+        int unit = u, chunk = 0;
+        bool ok = true;  // after a wait that ran out nothing more is waited for, and nothing stored
+        for (unsigned id = first; ok && id < t.tiles; id += step) {
+            uint64_t pair[S::COLUMNS / 2];  // two binary32 sums each, for two-lane multiply-adds
+#pragma unroll
+            for (int i = 0; i < S::COLUMNS / 2; ++i) pair[i] = 0;
+#pragma unroll 1
+            for (int kb = 0; kb < KB; ++kb, unit += S::UNITS) {
+                const int c = chunk & 1, in = kb % S::CHUNK, b = unit % S::BUFFERS;
+                if (in == 0) ok = ok && warp_wait(&scaled[c], (chunk / 2) & 1);
+                const float factor = row_scale[c][in][local] * column_scale[c][in][u];
+                ok = ok && warp_wait(&ready[b], (unit / S::BUFFERS) & 1);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int h = 0; h < S::COLUMNS; h += S::PIECE) {
+                    uint32_t v[S::PIECE];
+                    tmem_load(v, lanes + b * S::UNIT + h);
+                    tmem_wait(v);
+                    if (h + S::PIECE == S::COLUMNS) {  // the unit has been read
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(drained0 + 8 * b);
+                    }
+#pragma unroll
+                    for (int i = 0; i < S::PIECE; i += 2) fma_two(pair[(h + i) / 2], v[i], v[i + 1], factor, factor);
+                }
+                if (in == S::CHUNK - 1 || kb == KB - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&spent[c]);
+                    ++chunk;
+                }
+            }
+            if (!ok) break;
+            unsigned tp, tq;
+            tile_place(t, id, tp, tq);
+            const uint64_t row = (uint64_t)tp * S::BM + rank * S::HALF + local;
+            if (row < t.p_rows) {
+#pragma unroll
+                for (int h = 0; h < S::COLUMNS; h += 16) {
+                    float sum[16];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        asm("mov.b64 {%0, %1}, %2;" : "=f"(sum[2 * i]), "=f"(sum[2 * i + 1]) : "l"(pair[h / 2 + i]));
+                    store_row<T, 16>(p, row, (uint64_t)tq * S::BN + u * S::UNIT + from + h, sum);
+                }
+            }
+        }
+        if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
+    }
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();  // the pair's products and arrivals are done in both CTAs
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLUMNS) : "memory");
+}
+
+// ---- row form
+template <int BN_> struct Rows {
+    static constexpr int BM = 128, BN = BN_, BUFFERS = 4, EPILOGUE = 4, THREADS = (2 + EPILOGUE) * 32;
+    static constexpr int TMEM_COLUMNS = BUFFERS * BN;
+    static constexpr int P_BYTES = BM * kBlock, Q_BYTES = BN * kBlock, STAGE_BYTES = P_BYTES + Q_BYTES;
+    static constexpr int STAGES = 5;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+    static_assert(BN <= 32, "a column's factor is kept in a lane");
+    static_assert(BM * BN * 4 <= STAGES * STAGE_BYTES, "the sums take the stages' place");
+};
+
+template <typename T, typename S>
+__global__ void __launch_bounds__(S::THREADS)
+    product_rows_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                        const __grid_constant__ TileParams<T> t) {
+    const ProductParams<T> &p = t.out;
+    if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *const tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     __shared__ uint64_t full[S::STAGES], empty[S::STAGES], ready[S::BUFFERS], drained[S::BUFFERS], finished;
     __shared__ uint32_t tmem_base;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-
-    // blocks [kb0, kb1) of the inner dimension: a cluster's share, all of them in the batch form
-    uint32_t rank = 0, ranks = 1;
-    if (S::ROWS) {
-        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-    }
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // uniform, for the compiler too
+    // blocks [kb0, kb1) of the inner dimension: this CTA's share
+    uint32_t ranks;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    const uint32_t rank = cluster_rank();
     const int kb0 = (int)((int64_t)t.blocks * rank / ranks), kb1 = (int)((int64_t)t.blocks * (rank + 1) / ranks);
-    const unsigned first = S::ROWS ? blockIdx.x / ranks : blockIdx.x, step = S::ROWS ? gridDim.x / ranks : gridDim.x;
+    unsigned tp, tq;
+    tile_place(t, blockIdx.x / ranks, tp, tq);
+    const int p0 = (int)(tp * S::BM), q0 = (int)(tq * S::BN);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
@@ -323,31 +637,19 @@ __global__ void __launch_bounds__(S::THREADS, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = tmem_base;
-
-    // Tiles in groups of 8 tile rows, column by column inside a group, so that the tiles worked on at
-    // once share a few panels of both operands in L2.
-    auto place = [&](unsigned id, int &p0, int &q0) {
-        const unsigned group = id / (8 * t.tiles_q) * 8, rows = min(8u, t.tiles_p - group), in = id - group * t.tiles_q;
-        p0 = (int)((group + in % rows) * S::BM);
-        q0 = (int)(in / rows * S::BN);
-    };
+    const uint32_t tmem = __shfl_sync(~0u, tmem_base, 0);
 
     if (warp == 0) {
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            for (unsigned id = first; ok && id < t.tiles; id += step) {
-                int p0, q0;
-                place(id, p0, q0);
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % S::STAGES;
-                    if (!(ok = mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1))) break;
-                    unsigned char *to = tiles + s * S::STAGE_BYTES;
-                    mbar_expect_tx(&full[s], S::STAGE_BYTES);
-                    tma_load_2d(to, &map_p, &full[s], kb * kBlock, p0);
-                    tma_load_2d(to + S::P_BYTES, &map_q, &full[s], kb * kBlock, q0);
-                }
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % S::STAGES;
+                if (!(ok = mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1))) break;
+                unsigned char *to = tiles + s * S::STAGE_BYTES;
+                mbar_expect_tx(&full[s], S::STAGE_BYTES);
+                tma_load_2d(to, &map_p, &full[s], kb * kBlock, p0);
+                tma_load_2d(to + S::P_BYTES, &map_q, &full[s], kb * kBlock, q0);
             }
             if (!ok) record_fault(p.status, 0, kWatchdog);
             // nothing is left in flight towards this CTA's shared memory when it ends
@@ -355,94 +657,68 @@ __global__ void __launch_bounds__(S::THREADS, 1)
                 mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t shape = 1u << 4 | (uint32_t)(S::BN / 8) << 17 | (uint32_t)(S::BM / 16) << 24;
-            int it = 0;
-            bool ok = true;
-            for (unsigned id = first; ok && id < t.tiles; id += step)
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % S::STAGES, b = it % S::BUFFERS;
-                    if (!(ok = mbar_wait(&drained[b], ((it / S::BUFFERS) & 1) ^ 1) &&
-                               mbar_wait(&full[s], (it / S::STAGES) & 1)))
-                        break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = smem_addr(tiles + s * S::STAGE_BYTES);
-                    const uint64_t pd = k_major_descriptor(at), qd = k_major_descriptor(at + S::P_BYTES);
-#pragma unroll
-                    for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further along the swizzled rows
-                        mma_e4m3(tmem + b * S::BN, pd + 2 * k, qd + 2 * k, shape, k != 0);
-                    mma_commit(&empty[s]);
-                    mma_commit(&ready[b]);
-                }
-            if (!ok) record_fault(p.status, 0, kWatchdog);
-            mma_commit(&finished);
-            if (!mbar_wait(&finished, 0)) record_fault(p.status, 0, kWatchdog);
-        }
-    } else {
-        const int quarter = warp % 4, half = (warp - 2) / 4;
-        const int local = quarter * 32 + lane, from = half * S::COLUMNS;  // this thread's row and first column
-        float sum[S::COLUMNS];
+        constexpr uint32_t shape = 1u << 4 | (uint32_t)(S::BN / 8) << 17 | (uint32_t)(S::BM / 16) << 24;
+        const uint32_t stage0 = smem_addr(tiles);
         int it = 0;
         bool ok = true;
-        for (unsigned id = first; ok && id < t.tiles; id += step) {
-            int p0, q0;
-            place(id, p0, q0);
-            const uint64_t row = (uint64_t)p0 + local, column = (uint64_t)q0 + from;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % S::STAGES, b = it % S::BUFFERS;
+            if (!(ok = warp_wait(&drained[b], ((it / S::BUFFERS) & 1) ^ 1) && warp_wait(&full[s], (it / S::STAGES) & 1)))
+                break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint64_t pd = k_major_descriptor(stage0 + s * S::STAGE_BYTES), qd = pd + (S::P_BYTES >> 4);
+            if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < S::COLUMNS; ++i) sum[i] = 0;
-            // Batch form: one factor per thread and block, its columns being one block of 128 of the right
-            // operand's.  Row form: lane c holds column c's.  Read one block ahead of its use.
-            auto factor_of = [&](int kb) -> float {
-                if (kb >= kb1) return 0.0f;
-                if (!S::ROWS)
-                    return row < t.p_rows && column < t.q_rows
-                               ? t.p_scales[row * t.blocks + kb] * t.q_scales[column / kBlock * t.blocks + kb]
-                               : 0.0f;
-                return lane < S::BN && (uint64_t)q0 + lane < t.q_rows
-                           ? t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb] * t.p_scales[(uint64_t)p0 / kBlock * t.blocks + kb]
-                           : 0.0f;
-            };
-            float next = factor_of(kb0);
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int b = it % S::BUFFERS;
-                const float factor = next;
-                next = factor_of(kb + 1);
-                if (!(ok = __all_sync(~0u, mbar_wait(&ready[b], (it / S::BUFFERS) & 1)))) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + b * S::BN + from;
-                uint32_t v[2][16];
-                tmem_load16(v[0], at);
-#pragma unroll
-                for (int c = 0; c < S::COLUMNS / 16; ++c) {
-                    tmem_wait(v[c & 1]);
-                    if (c + 1 < S::COLUMNS / 16) {
-                        tmem_load16(v[(c + 1) & 1], at + (c + 1) * 16);
-                    } else {  // the buffer has been read
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&drained[b]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float f = S::ROWS ? __shfl_sync(~0u, factor, c * 16 + i) : factor;
-                        sum[c * 16 + i] = fmaf(__uint_as_float(v[c & 1][i]), f, sum[c * 16 + i]);
-                    }
-                }
+                for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further along the swizzled rows
+                    mma_e4m3(tmem + b * S::BN, pd + 2 * k, qd + 2 * k, shape, k != 0);
+                mma_commit(&empty[s]);
+                mma_commit(&ready[b]);
             }
-            if (!ok) break;
-            if (!S::ROWS) {
-                if (row < t.p_rows) store_row<T, S::COLUMNS>(p, row, column, sum);
-            } else if (ranks == 1) {
-#pragma unroll
-                for (int i = 0; i < S::COLUMNS; ++i)
-                    if (row < t.p_rows && column + i < t.q_rows) store_cell(p, column + i, row, sum[i]);
-            } else {
-                // to the cluster's first CTA, behind every CTA's last use of its stages (see below)
-#pragma unroll
-                for (int i = 0; i < S::COLUMNS; ++i) reinterpret_cast<float *>(tiles)[i * S::BM + local] = sum[i];
-            }
+            __syncwarp();
         }
+        if (elect_one()) mma_commit(&finished);
+        __syncwarp();
+        ok = warp_wait(&finished, 0) && ok;
         if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
+    } else {
+        const int quarter = warp % 4, local = quarter * 32 + lane;  // this thread's row of the tile
+        const uint64_t row = (uint64_t)p0 + local;
+        // Lane c holds the product of both operands' scales for the tile's column c, read one block ahead.
+        auto scale_of = [&](int kb) -> float {
+            return kb < kb1 && lane < S::BN && (uint64_t)q0 + lane < t.q_rows
+                       ? t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb] * t.p_scales[(uint64_t)tp * t.blocks + kb]
+                       : 0.0f;
+        };
+        float sum[S::BN], next = scale_of(kb0);
+#pragma unroll
+        for (int i = 0; i < S::BN; ++i) sum[i] = 0;
+        int it = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int b = it % S::BUFFERS;
+            const float factor = next;
+            next = scale_of(kb + 1);
+            if (!(ok = warp_wait(&ready[b], (it / S::BUFFERS) & 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t v[S::BN];
+            tmem_load(v, tmem + ((uint32_t)(quarter * 32) << 16) + b * S::BN);
+            tmem_wait(v);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&drained[b]);
+#pragma unroll
+            for (int i = 0; i < S::BN; ++i) sum[i] = fmaf(__uint_as_float(v[i]), __shfl_sync(~0u, factor, i), sum[i]);
+        }
+        if (!ok) {
+            if (lane == 0) record_fault(p.status, 0, kWatchdog);
+        } else if (ranks == 1) {
+#pragma unroll
+            for (int i = 0; i < S::BN; ++i)
+                if (row < t.p_rows && (uint64_t)q0 + i < t.q_rows) store_cell(p, (uint64_t)q0 + i, row, sum[i]);
+        } else {  // for the cluster's first CTA; every load and product of this CTA is done
+#pragma unroll
+            for (int i = 0; i < S::BN; ++i) reinterpret_cast<float *>(tiles)[i * S::BM + local] = sum[i];
+        }
     }
 
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -450,28 +726,26 @@ __global__ void __launch_bounds__(S::THREADS, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLUMNS) : "memory");
-    if (S::ROWS && ranks > 1) {
-        // each CTA's sums are in its own shared memory: the first CTA reads them all
-        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    if (ranks > 1) {
+        cluster_sync();  // each CTA's sums are in its own shared memory
         if (rank == 0) {
-            int p0, q0;
-            place(first, p0, q0);
             for (int i = threadIdx.x; i < S::BM * S::BN; i += S::THREADS) {
                 const uint64_t column = (uint64_t)p0 + i % S::BM, row = (uint64_t)q0 + i / S::BM;
                 if (column >= t.p_rows || row >= t.q_rows) continue;
                 float total = 0;
                 for (uint32_t r = 0; r < ranks; ++r) {
-                    uint32_t remote;
                     float v;
-                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(tiles) + 4 * i), "r"(r));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                 : "=f"(v)
+                                 : "r"(cluster_address(smem_addr(tiles) + 4 * i, r))
+                                 : "memory");
                     total += v;
                 }
                 store_cell(p, row, column, total);
             }
         }
         __syncwarp();
-        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+        cluster_sync();  // and stay until they have been read
     }
 }
 
@@ -502,35 +776,60 @@ static bool code_map(CUtensorMap *map, const unsigned char *base, uint64_t rows,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, typename S>
-static int launch_product(const ProductParams<T> &p, const CUtensorMap &map_p, const CUtensorMap &map_q, unsigned ranks,
-                          cudaStream_t stream) {
+// Once per device: the dynamic shared memory that a kernel may ask for, and whether it is launched
+// with the registers a thread that its warps share out.
+template <auto kernel> static int allow_shared(int bytes, int registers = 0) {
     static std::mutex lock;
     static bool configured[64] = {false};
     int device = 0;
     if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return pcu_host::set_cuda_error(e);
-    {
-        std::lock_guard<std::mutex> guard(lock);
-        if (device >= 64 || !configured[device]) {
-            if (cudaError_t e = cudaFuncSetAttribute(product_kernel<T, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                     S::SMEM_BYTES);
-                e != cudaSuccess)
-                return pcu_host::set_cuda_error(e);
-            if (device < 64) configured[device] = true;
-        }
+    std::lock_guard<std::mutex> guard(lock);
+    if (device < 64 && configured[device]) return PCU_B200_OK;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return pcu_host::set_cuda_error(e);
     }
+    cudaFuncAttributes attributes;
+    if (cudaError_t e = cudaFuncGetAttributes(&attributes, kernel); e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return pcu_host::set_cuda_error(e);
+    }
+    if (attributes.numRegs < registers) return PCU_B200_ERROR_UNSUPPORTED;
+    if (device < 64) configured[device] = true;
+    return PCU_B200_OK;
+}
+
+template <typename T> static TileParams<T> tile_params(const ProductParams<T> &p, bool row_form, int bm, int bn) {
     TileParams<T> t{};
     t.out = p;
-    t.p_rows = S::ROWS ? p.columns : p.rows;
-    t.q_rows = S::ROWS ? p.rows : p.columns;
-    t.p_scales = S::ROWS ? p.right_scales : p.left_scales;
-    t.q_scales = S::ROWS ? p.left_scales : p.right_scales;
-    t.tiles_p = (unsigned)((t.p_rows + S::BM - 1) / S::BM);
-    t.tiles_q = (unsigned)((t.q_rows + S::BN - 1) / S::BN);
+    t.p_rows = row_form ? p.columns : p.rows;
+    t.q_rows = row_form ? p.rows : p.columns;
+    t.p_scales = row_form ? p.right_scales : p.left_scales;
+    t.q_scales = row_form ? p.left_scales : p.right_scales;
+    t.tiles_p = (unsigned)((t.p_rows + bm - 1) / bm);
+    t.tiles_q = (unsigned)((t.q_rows + bn - 1) / bn);
     t.tiles = t.tiles_p * t.tiles_q;
     t.blocks = (int)((p.inner + kBlock - 1) / kBlock);
+    return t;
+}
+
+template <typename T>
+static int launch_batch(const ProductParams<T> &p, const CUtensorMap &left, const CUtensorMap &right, cudaStream_t stream) {
+    if (const int rc = allow_shared<product_kernel<T>>(Batch::SMEM_BYTES, Batch::LAUNCHED)) return rc;
+    const TileParams<T> t = tile_params(p, false, Batch::BM, Batch::BN);
+    const unsigned pairs = std::min(t.tiles, (unsigned)std::max(1, pcu_host::sm_count() / 2));
+    product_kernel<T><<<2 * pairs, Batch::THREADS, Batch::SMEM_BYTES, stream>>>(left, right, t);
+    return pcu_host::launch_status();
+}
+
+template <typename T, typename S>
+static int launch_rows(const ProductParams<T> &p, const CUtensorMap &left, const CUtensorMap &right, cudaStream_t stream) {
+    if (const int rc = allow_shared<product_rows_kernel<T, S>>(S::SMEM_BYTES)) return rc;
+    const TileParams<T> t = tile_params(p, true, S::BM, S::BN);
+    unsigned ranks = 1;
+    while (ranks < 8 && t.tiles * ranks * 2 <= 2 * (uint64_t)pcu_host::sm_count() && (unsigned)t.blocks >= 8 * ranks) ranks *= 2;
     cudaLaunchConfig_t config{};
-    config.gridDim = S::ROWS ? t.tiles * ranks : std::min(t.tiles, (unsigned)pcu_host::sm_count());
+    config.gridDim = t.tiles * ranks;
     config.blockDim = S::THREADS;
     config.dynamicSmemBytes = S::SMEM_BYTES;
     config.stream = stream;
@@ -539,8 +838,8 @@ static int launch_product(const ProductParams<T> &p, const CUtensorMap &map_p, c
     cluster.val.clusterDim.x = ranks;
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
-    config.numAttrs = S::ROWS ? 1 : 0;
-    if (cudaError_t e = cudaLaunchKernelEx(&config, product_kernel<T, S>, map_p, map_q, t); e != cudaSuccess) {
+    config.numAttrs = 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&config, product_rows_kernel<T, S>, right, left, t); e != cudaSuccess) {
         (void)cudaGetLastError();
         return pcu_host::set_cuda_error(e);
     }
@@ -548,22 +847,16 @@ static int launch_product(const ProductParams<T> &p, const CUtensorMap &map_p, c
 }
 
 template <typename T> static int product_typed(const ProductParams<T> &p, cudaStream_t stream) {
-    CUtensorMap map_left, map_right;
-    constexpr int kFew = 16;
-    if (p.inner && p.rows <= kFew) {
-        using S = ProductShape<kFew, true>;
-        if (code_map(&map_right, p.right, p.columns, p.inner, p.right_stride, S::BM) &&
-            code_map(&map_left, p.left, p.rows, p.inner, p.left_stride, S::BN)) {
-            const uint64_t tiles = (p.columns + S::BM - 1) / S::BM, blocks = (p.inner + kBlock - 1) / kBlock;
-            unsigned ranks = 1;
-            while (ranks < 8 && tiles * ranks * 2 <= 2 * (uint64_t)pcu_host::sm_count() && blocks >= 8 * ranks) ranks *= 2;
-            return launch_product<T, S>(p, map_right, map_left, ranks, stream);
-        }
+    CUtensorMap left, right;
+    if (p.inner && p.rows <= 32) {
+        const bool few = p.rows <= 16;
+        if (code_map(&right, p.right, p.columns, p.inner, p.right_stride, 128) &&
+            code_map(&left, p.left, p.rows, p.inner, p.left_stride, few ? 16 : 32))
+            return few ? launch_rows<T, Rows<16>>(p, left, right, stream) : launch_rows<T, Rows<32>>(p, left, right, stream);
     } else if (p.inner) {
-        using S = ProductShape<256, false>;
-        if (code_map(&map_left, p.left, p.rows, p.inner, p.left_stride, S::BM) &&
-            code_map(&map_right, p.right, p.columns, p.inner, p.right_stride, S::BN))
-            return launch_product<T, S>(p, map_left, map_right, 1, stream);
+        if (code_map(&left, p.left, p.rows, p.inner, p.left_stride, Batch::HALF) &&
+            code_map(&right, p.right, p.columns, p.inner, p.right_stride, Batch::UNIT / 2))
+            return launch_batch<T>(p, left, right, stream);
     }
     const uint64_t tiles = (p.rows + 15) / 16 * ((p.columns + 15) / 16);
     product_plain_kernel<T><<<(unsigned)tiles, 256, 0, stream>>>(p);

@@ -37,16 +37,38 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
     return done != 0;
 }
 
+// The same for barriers at which other CTAs of the cluster arrive without handing memory over:
+// relaxed, since an acquire at cluster scope drops the SM's cached lines.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // Bounded wait: false after kWaitLimitNs (the caller reports kWatchdog).
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
+template <typename Try> __device__ __forceinline__ bool bounded_wait(Try attempt) {
+    if (attempt()) return true;
     const unsigned long long t0 = global_ns();
     for (;;) {
 #pragma unroll 1
         for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
+            if (attempt()) return true;
         if (global_ns() - t0 > kWaitLimitNs) return false;
     }
+}
+
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
+    return bounded_wait([&] { return mbar_try_wait(bar, parity); });
+}
+
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
+    return bounded_wait([&] { return mbar_try_wait_cluster(bar, parity); });
 }
 
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
