@@ -328,22 +328,6 @@ __device__ __forceinline__ void tile_place(const TileParams<T> &t, unsigned id, 
     q = in / rows;
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t cluster_address(uint32_t address, uint32_t rank) {
-    uint32_t remote;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(rank));
-    return remote;
-}
-
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-
 // ---- batch form
 //
 // A pair of CTAs (a cluster of 2) owns 256 x 256 cells: each holds 128 rows of P and half of Q's rows,
@@ -776,29 +760,6 @@ static bool code_map(CUtensorMap *map, const unsigned char *base, uint64_t rows,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Once per device: the dynamic shared memory that a kernel may ask for, and whether it is launched
-// with the registers a thread that its warps share out.
-template <auto kernel> static int allow_shared(int bytes, int registers = 0) {
-    static std::mutex lock;
-    static bool configured[64] = {false};
-    int device = 0;
-    if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return pcu_host::set_cuda_error(e);
-    std::lock_guard<std::mutex> guard(lock);
-    if (device < 64 && configured[device]) return PCU_B200_OK;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess) {
-        (void)cudaGetLastError();
-        return pcu_host::set_cuda_error(e);
-    }
-    cudaFuncAttributes attributes;
-    if (cudaError_t e = cudaFuncGetAttributes(&attributes, kernel); e != cudaSuccess) {
-        (void)cudaGetLastError();
-        return pcu_host::set_cuda_error(e);
-    }
-    if (attributes.numRegs < registers) return PCU_B200_ERROR_UNSUPPORTED;
-    if (device < 64) configured[device] = true;
-    return PCU_B200_OK;
-}
-
 template <typename T> static TileParams<T> tile_params(const ProductParams<T> &p, bool row_form, int bm, int bn) {
     TileParams<T> t{};
     t.out = p;
@@ -815,7 +776,7 @@ template <typename T> static TileParams<T> tile_params(const ProductParams<T> &p
 
 template <typename T>
 static int launch_batch(const ProductParams<T> &p, const CUtensorMap &left, const CUtensorMap &right, cudaStream_t stream) {
-    if (const int rc = allow_shared<product_kernel<T>>(Batch::SMEM_BYTES, Batch::LAUNCHED)) return rc;
+    if (const int rc = pcu_host::allow_shared<product_kernel<T>>(Batch::SMEM_BYTES, Batch::LAUNCHED)) return rc;
     const TileParams<T> t = tile_params(p, false, Batch::BM, Batch::BN);
     const unsigned pairs = std::min(t.tiles, (unsigned)std::max(1, pcu_host::sm_count() / 2));
     product_kernel<T><<<2 * pairs, Batch::THREADS, Batch::SMEM_BYTES, stream>>>(left, right, t);
@@ -824,26 +785,12 @@ static int launch_batch(const ProductParams<T> &p, const CUtensorMap &left, cons
 
 template <typename T, typename S>
 static int launch_rows(const ProductParams<T> &p, const CUtensorMap &left, const CUtensorMap &right, cudaStream_t stream) {
-    if (const int rc = allow_shared<product_rows_kernel<T, S>>(S::SMEM_BYTES)) return rc;
+    if (const int rc = pcu_host::allow_shared<product_rows_kernel<T, S>>(S::SMEM_BYTES)) return rc;
     const TileParams<T> t = tile_params(p, true, S::BM, S::BN);
     unsigned ranks = 1;
     while (ranks < 8 && t.tiles * ranks * 2 <= 2 * (uint64_t)pcu_host::sm_count() && (unsigned)t.blocks >= 8 * ranks) ranks *= 2;
-    cudaLaunchConfig_t config{};
-    config.gridDim = t.tiles * ranks;
-    config.blockDim = S::THREADS;
-    config.dynamicSmemBytes = S::SMEM_BYTES;
-    config.stream = stream;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = ranks;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
-    if (cudaError_t e = cudaLaunchKernelEx(&config, product_rows_kernel<T, S>, right, left, t); e != cudaSuccess) {
-        (void)cudaGetLastError();
-        return pcu_host::set_cuda_error(e);
-    }
-    return PCU_B200_OK;
+    return pcu_host::launch_cluster(product_rows_kernel<T, S>, t.tiles * ranks, S::THREADS, S::SMEM_BYTES, ranks, stream,
+                                    right, left, t);
 }
 
 template <typename T> static int product_typed(const ProductParams<T> &p, cudaStream_t stream) {

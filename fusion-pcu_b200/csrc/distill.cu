@@ -6,12 +6,16 @@
 //   loss = w T^2 sum_j p_j (ln p_j - ln q[idx_j]),   d loss u / d z_v = u w T (q_v - sum_{idx_j = v} p_j).
 // The row statistics are m = max z and s = sum exp((z - m) / T): q_v = exp((z_v - m) / T) / s keeps
 // the relative precision of binary32, which a single log-sum-exp of magnitude 50 would not.
+#include <type_traits>
+
 #include "learn.cuh"
 #include "provider.h"
+#include "tma.cuh"
 
 namespace pcu {
 
 constexpr int kDistillThreads = 256;
+constexpr int kMostChunks = 14;  // of a slice; 16 KB each
 
 template <typename T> struct DistillParams {
     using W = WideOf<T>;
@@ -29,6 +33,8 @@ template <typename T> struct DistillParams {
     int upstream_uniform;
     T *gradient;             // null: loss only
     uint64_t gradient_stride;
+    int slice;            // elements of a row per CTA of its cluster (whole granules)
+    uint32_t slice_bytes;
     unsigned long long *status;
     ChainGuard guard;
 };
@@ -53,7 +59,7 @@ template <typename V> __device__ __forceinline__ V block_max(V v, V *scratch) {
     return v;
 }
 
-// One CTA per row.
+// Rows that no cluster holds: one CTA per row, which it reads twice.
 template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill_kernel(const DistillParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
@@ -174,10 +180,369 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill
     if (kind) record_fault(p.status, row, kind);
 }
 
+// ---- rows in shared memory
+//
+// A cluster of 1, 2, 4 or 8 CTAs takes a row, each a slice of the vocabulary that stays in its shared
+// memory: bulk copies bring it in once, the running maximum and sum are taken as it lands, the CTAs
+// join theirs through the cluster, and the gradient is formed from shared memory.  So a step reads
+// the logits once and writes the gradient once, which is what it cannot do without; with the rows
+// read a second time through L2, 592 resident rows of 256 KB were more than L2 holds.
+// Bulk copies move whole 16-byte granules; a row that starts or ends inside one has its edges copied
+// by threads, so any alignment keeps the wide loads.  The slice keeps the row's phase: the byte at
+// address a lies at (a - first granule's address).
+
+constexpr int kChunk = 16384;  // bytes per bulk copy, each with a barrier: 4 granules per thread
+
+// A running maximum and sum of 2^(c (x - m)).  With hi = c m rounded, c x - hi is one multiply-add;
+// the sum so formed is 2^d times the wanted one, d = hi - c m (known exactly), and it is set right at the end.
+// A maximum of 2^64 and more, where c x may overflow, takes the difference first.
+template <typename W> struct Running {
+    W m, s, hi;
+    bool far;
+};
+
+__device__ __forceinline__ void refer(Running<float> &r, float m, float c) {
+    r.m = m;
+    r.far = !(fabsf(m) < 0x1p64f);
+    r.hi = r.far ? 0.0f : m * c;
+}
+__device__ __forceinline__ void refer(Running<double> &r, double m, double) { r.m = m, r.far = true, r.hi = 0; }
+
+// The factor that the terms of r are too large by.
+__device__ __forceinline__ float excess(const Running<float> &r, float c) {
+    return r.far ? 1.0f : fast_exp2(fmaf(r.m, c, -r.hi));
+}
+__device__ __forceinline__ double excess(const Running<double> &, double) { return 1.0; }
+
+template <typename W> __device__ __forceinline__ W term(const Running<W> &r, W x, W c) {
+    return r.far ? fast_exp2((x - r.m) * c) : fast_exp2(fma(x, c, -r.hi));
+}
+
+// A new, larger maximum: the sum is taken relative to it.
+template <typename W> __device__ __forceinline__ void raise(Running<W> &r, W m, W c) {
+    const Running<W> old = r;
+    refer(r, m, c);
+    if (old.s != W(0)) r.s = old.s * (old.far || r.far ? fast_exp2((old.m - m) * c) : fast_exp2(old.hi - r.hi));
+}
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(dst)),
+        "l"(src), "r"(bytes), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// The joint maximum and sum of two shares (true sums, no excess).  A share without a finite logit has
+// m = -infinity and s = 0; a NaN sum stays.
+template <typename W> __device__ __forceinline__ void join(W &m, W &s, W m2, W s2, W c) {
+    const W top = fmax(m, m2);
+    s = (m == top || s == W(0) || isnan(s) ? s : s * fast_exp2((m - top) * c)) +
+        (m2 == top || s2 == W(0) || isnan(s2) ? s2 : s2 * fast_exp2((m2 - top) * c));
+    m = top;
+}
+
+template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) distill_slice_kernel(const DistillParams<T> p) {
+    using W = WideOf<T>;
+    constexpr int V = 16 / sizeof(T), WARPS = kDistillThreads / 32;
+    if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ uint64_t landed[kMostChunks];
+    __shared__ W part_m[WARPS], part_s[WARPS], share[2];
+    __shared__ double part_a[WARPS], part_mass[WARPS], part_terms[WARPS];
+    uint32_t ranks, rank;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    const uint64_t row = blockIdx.x / ranks;
+    const T *z = p.logits + row * p.stride;
+    // this CTA's elements [v0, v1) of the row, cut at the row's granules
+    const uint32_t phase = (uint32_t)(reinterpret_cast<uintptr_t>(z) % 16 / sizeof(T));
+    const int vocab = (int)p.vocab;
+    const int v0 = max(0, (int)((int64_t)rank * p.slice) - (int)phase);
+    const int v1 = min(vocab, (int)((int64_t)(rank + 1) * p.slice) - (int)phase);
+    const int lead = rank == 0 ? (int)phase : 0;  // elements of the first granule in front of v0
+    const int count = max(0, v1 - v0), granules = (lead + count + V - 1) / V;
+    T *slice = reinterpret_cast<T *>(smem);  // element v at slice[lead + v - v0]
+    double *prob = reinterpret_cast<double *>(smem + p.slice_bytes);
+    int *place = reinterpret_cast<int *>(prob + p.k);
+    const int chunks = (granules * 16 + kChunk - 1) / kChunk;
+    T *g = p.gradient ? p.gradient + row * p.gradient_stride : nullptr;
+    const W weight = p.weights ? p.weights[row] : W(1), c = p.to_log2;
+    const double t_inverse = 1.0 / (double)p.temperature;
+
+    if (tid == 0) {
+        for (int i = 0; i < chunks; ++i) mbar_init(&landed[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // the teacher's entries: exponents t / T, -infinity for absent ones
+    double a_max = -INFINITY;
+    int flags = 0;  // 1: an entry is present, 2: one is bad
+    for (int j = tid; j < p.k; j += kDistillThreads) {
+        const int64_t at = p.indices[row * p.k + j];
+        const double t = (double)p.top[row * p.k + j];
+        bool there = at >= 0 && t != -INFINITY;
+        if (there && (at >= vocab || !isfinite(t))) flags |= 2, there = false;
+        place[j] = there ? (int)at : -1;
+        prob[j] = there ? t * t_inverse : -INFINITY;
+        if (there) flags |= 1;
+        a_max = fmax(a_max, prob[j]);
+    }
+    const bool bad = __syncthreads_or(flags & 2);
+    if (weight == W(0) || (!__syncthreads_or(flags & 1) && !bad)) {  // nothing to learn from: the row is not read
+        if (tid == 0 && rank == 0) {
+            if (p.loss) p.loss[row] = W(0);
+            if (p.stats_out) p.stats_out[2 * row] = W(0), p.stats_out[2 * row + 1] = W(1);
+        }
+        if (g)
+            for (int v = v0 + tid; v < v1; v += kDistillThreads) g[v] = Elem<T>::round(W(0));
+        return;  // every CTA of the cluster
+    }
+
+    // whole granules by bulk copies, the elements of cut ones by threads
+    const int whole0 = lead ? 1 : 0, whole1 = (lead + count) / V;
+    if (tid == 0)
+        for (int i = 0; i < chunks; ++i) {
+            const int a = max(whole0, i * (kChunk / 16)), b = min(whole1, (i + 1) * (kChunk / 16));
+            if (b > a) {
+                mbar_expect_tx(&landed[i], (uint32_t)(b - a) * 16);
+                bulk_load(slice + a * V, z + v0 + (a * V - lead), (uint32_t)(b - a) * 16, &landed[i]);
+            } else {
+                mbar_arrive(&landed[i]);
+            }
+        }
+    if (tid < V) {
+        const W absent = -INFINITY;
+        if (lead) slice[tid] = tid < lead || tid - lead >= count ? Elem<T>::round(absent) : z[v0 + tid - lead];
+        const int at = whole1 * V + tid;  // the last granule, if it is cut
+        if (whole1 < granules && (whole1 > 0 || !lead))
+            slice[at] = at - lead < count ? z[v0 + at - lead] : Elem<T>::round(absent);
+    }
+    __syncthreads();
+
+    bool ok = true;
+    W m, s, inverse;
+    Running<W> run;
+    if (p.stats_in) {
+        m = p.stats_in[2 * row];
+        s = p.stats_in[2 * row + 1];
+    } else {
+        refer(run, -INFINITY, c);
+        run.s = W(0);
+        for (int i = 0; i < chunks; ++i) {
+            ok = ok && mbar_wait(&landed[i], 0);
+            W x[4][V];
+            W top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int at = i * (kChunk / 16) + q * kDistillThreads + tid;
+                uint4 raw;
+                if (at < granules) raw = *reinterpret_cast<const uint4 *>(slice + at * V);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[q][e] = at < granules ? Elem<T>::load(reinterpret_cast<const T *>(&raw)[e]) : W(-INFINITY);
+                    top = fmax(top, x[q][e]);
+                }
+            }
+            if (top > run.m) raise(run, top, c);
+            if (run.m == -INFINITY) {  // nothing but masked entries so far, or NaN
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (isnan(x[q][e])) run.s = x[q][e];
+            } else if (run.far) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) run.s += fast_exp2((x[q][e] - run.m) * c);
+            } else {
+                W sum[4] = {};
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) sum[q] += fast_exp2(fma(x[q][e], c, -run.hi));
+                run.s += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+        }
+        m = run.m;
+        s = run.s / excess(run, c);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const W m2 = __shfl_xor_sync(~0u, m, o), s2 = __shfl_xor_sync(~0u, s, o);
+            join(m, s, m2, s2, c);
+        }
+        if (lane == 0) part_m[warp] = m, part_s[warp] = s;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a_max = fmax(a_max, __shfl_xor_sync(~0u, a_max, o));
+    if (lane == 0) part_a[warp] = a_max;
+    __syncthreads();
+    a_max = part_a[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) a_max = fmax(a_max, part_a[i]);
+    if (!p.stats_in) {
+        m = part_m[0], s = part_s[0];
+#pragma unroll
+        for (int i = 1; i < WARPS; ++i) join(m, s, part_m[i], part_s[i], c);
+    }
+    // The logits that the teacher names.  For the loss from anywhere in the row, before any CTA of the
+    // cluster may overwrite it.
+    double here[(PCU_B200_DISTILL_TOP_MAX + kDistillThreads - 1) / kDistillThreads];
+    if (p.loss)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = tid + i * kDistillThreads;
+            if (j < p.k && place[j] >= 0) here[i] = (double)Elem<T>::load(z[place[j]]);
+        }
+    if (!p.stats_in && ranks > 1) {
+        if (tid == 0) share[0] = m, share[1] = s;
+        cluster_sync();
+        // in rank order in every CTA: the same bits everywhere
+        for (uint32_t r = 0; r < ranks; ++r) {
+            W m2, s2;
+            cluster_read(m2, smem_addr(&share[0]), r);
+            cluster_read(s2, smem_addr(&share[1]), r);
+            if (r == 0) m = m2, s = s2;
+            else join(m, s, m2, s2, c);
+        }
+    }
+    const W up = p.upstream ? p.upstream[p.upstream_uniform ? 0 : row] : W(1);
+    const bool invalid = bad || !isfinite(m) || !isfinite(s) || !(s > W(0)) || !isfinite(weight) || (g && !isfinite(up));
+
+    // with e_j = exp(a_j - a_max): loss / (w T^2) = sum e_j (a_j - a_max - ln q_j) / sum e_j - ln(sum e_j)
+    double mass = 0, terms = 0;
+    const double ln_s = p.loss && !invalid ? log((double)s) : 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = tid + i * kDistillThreads;
+        if (j < p.k && place[j] >= 0) {
+            const double a = prob[j] - a_max, e = exp(a);
+            mass += e;
+            if (p.loss && e > 0) terms += e * (a - ((here[i] - (double)m) * t_inverse - ln_s));
+            prob[j] = e;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        mass += __shfl_xor_sync(~0u, mass, o);
+        terms += __shfl_xor_sync(~0u, terms, o);
+    }
+    if (lane == 0) part_mass[warp] = mass, part_terms[warp] = terms;
+    __syncthreads();
+    mass = part_mass[0], terms = part_terms[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) mass += part_mass[i], terms += part_terms[i];
+
+    unsigned kind = invalid && tid == 0 ? (unsigned)PCU_B200_KIND_INVALID : 0u;
+    if (rank == 0 && tid == 0) {
+        if (p.loss) {
+            const double t = (double)p.temperature;
+            const W value = invalid ? W(NAN) : (W)((double)weight * t * t * (terms / mass - log(mass)));
+            p.loss[row] = value;
+            if (!kind) kind = result_kind(value);
+        }
+        if (p.stats_out) p.stats_out[2 * row] = m, p.stats_out[2 * row + 1] = s;
+    }
+    if (g && invalid) {
+        for (int v = v0 + tid; v < v1; v += kDistillThreads) g[v] = Elem<T>::round(W(NAN));
+    } else if (g) {
+        const W factor = up * weight * p.temperature;
+        refer(run, m, c);
+        inverse = W(1) / s / excess(run, c);
+        const W scale = factor * inverse;
+        // q is at most 1, so a result can only exceed its type where the factor does.  NaN and infinities
+        // among the logits, which a backward call meets here first, stay in the sum `seen`.
+        const bool check = !isfinite(Elem<T>::load(Elem<T>::round(factor)));
+        W seen = 0;
+        unsigned worst = 0;
+        const bool aligned = (reinterpret_cast<uintptr_t>(g + v0) - lead * sizeof(T)) % 16 == 0;
+        auto sweep = [&](auto plain_) {
+            constexpr bool plain = decltype(plain_)::value;  // neither far nor check: the case that counts
+            auto value = [&](T x) {
+                const W e = plain ? fast_exp2(fma(Elem<T>::load(x), c, -run.hi)) : term(run, Elem<T>::load(x), c);
+                if (p.stats_in) seen += e;
+                const T r = Elem<T>::round(scale * e);
+                if (!plain && check) worst = max(worst, result_kind(Elem<T>::load(r)));
+                return r;
+            };
+            if (aligned) {
+                for (int i = 0; i < chunks; ++i) {
+                    if (p.stats_in) ok = ok && mbar_wait(&landed[i], 0);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int at = i * (kChunk / 16) + q * kDistillThreads + tid;
+                        if (at >= granules) break;
+                        const uint4 raw = *reinterpret_cast<const uint4 *>(slice + at * V);
+                        alignas(16) T r[V];
+#pragma unroll
+                        for (int e = 0; e < V; ++e) r[e] = value(reinterpret_cast<const T *>(&raw)[e]);
+                        T *to = g + v0 + (at * V - lead);
+                        if (at >= whole0 && at < whole1) {
+                            __stcs(reinterpret_cast<uint4 *>(to), *reinterpret_cast<const uint4 *>(r));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < V; ++e)
+                                if (at * V + e >= lead && at * V + e - lead < count) to[e] = r[e];
+                        }
+                    }
+                }
+            } else {  // the gradient's rows lie differently: element by element, adjacent lanes adjacent elements
+                if (p.stats_in)
+                    for (int i = 0; i < chunks; ++i) ok = ok && mbar_wait(&landed[i], 0);
+#pragma unroll 8
+                for (int v = tid; v < count; v += kDistillThreads) g[v0 + v] = value(slice[lead + v]);
+            }
+        };
+        if (run.far || check) sweep(std::false_type{});
+        else sweep(std::true_type{});
+        if (!isfinite(seen) && !kind) kind = PCU_B200_KIND_INVALID;
+        __syncthreads();  // before the entries' elements are written again
+        for (int j = tid; j < p.k; j += kDistillThreads) {
+            const int at = place[j];
+            if (at < v0 || at >= v1) continue;
+            bool first = true;  // the first entry of an index carries the sum of all of them
+            for (int i = 0; i < j; ++i) first &= place[i] != at;
+            if (!first) continue;
+            double sum = prob[j];
+            for (int i = j + 1; i < p.k; ++i)
+                if (place[i] == at) sum += prob[i];
+            const W q = term(run, Elem<T>::load(slice[lead + at - v0]), c) * inverse;
+            const T r = Elem<T>::round(factor * (q - (W)(sum / mass)));
+            worst = max(worst, result_kind(Elem<T>::load(r)));
+            g[at] = r;
+        }
+        if (worst && !kind) kind = worst;
+    }
+    if (!ok) record_fault(p.status, 0, kWatchdog);
+    if (kind) record_fault(p.status, row, kind);
+    // nothing is left in flight towards this CTA's shared memory, and the cluster has read it
+    if (tid == 0)
+        for (int i = 0; i < chunks; ++i) mbar_wait(&landed[i], 0);
+    if (!p.stats_in && ranks > 1) {
+        __syncwarp();
+        cluster_sync();
+    }
+}
+
+// Rows go through shared memory where a cluster of 8 holds one.  The smallest cluster whose slices are
+// at most 64 KB is taken (three such CTAs per SM overlap each other's phases); with fewer rows than
+// fill the SMs twice, larger ones down to slices of 8 KB.
 template <typename T>
-static int launch_distill(const DistillParams<T> &p, uint64_t rows, cudaStream_t stream) {
-    distill_kernel<T><<<(unsigned)rows, kDistillThreads, 0, stream>>>(p);
-    return pcu_host::launch_status();
+static int launch_distill(DistillParams<T> p, uint64_t rows, cudaStream_t stream) {
+    const uint64_t bytes = p.vocab * sizeof(T) + 16, sms = (uint64_t)pcu_host::sm_count();
+    unsigned ranks = 1;
+    while (ranks < 8 && bytes > ranks * 65536ull) ranks *= 2;
+    while (ranks < 8 && rows * ranks < 2 * sms && bytes > ranks * 16384ull) ranks *= 2;
+    const uint64_t slice_bytes = (bytes + ranks - 1) / ranks / 16 * 16 + 16;
+    const uint64_t need = slice_bytes + (uint64_t)p.k * (sizeof(double) + sizeof(int));
+    if (slice_bytes > (uint64_t)kMostChunks * kChunk || need > 216 * 1024 || rows * ranks > 0x7fffffffull) {
+        distill_kernel<T><<<(unsigned)rows, kDistillThreads, 0, stream>>>(p);
+        return pcu_host::launch_status();
+    }
+    p.slice = (int)(slice_bytes / sizeof(T));
+    p.slice_bytes = (uint32_t)slice_bytes;
+    if (const int rc = pcu_host::allow_shared<distill_slice_kernel<T>>(216 * 1024)) return rc;
+    return pcu_host::launch_cluster(distill_slice_kernel<T>, (unsigned)(rows * ranks), kDistillThreads, need, ranks, stream, p);
 }
 
 // The arguments that the three calls share; a call leaves out what it does not have.

@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "pcu_b200.h"
 
 namespace pcu {
 
@@ -79,9 +80,77 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, u
         : "memory");
 }
 
+// ---- thread block clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t cluster_address(uint32_t address, uint32_t rank) {
+    uint32_t remote;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(rank));
+    return remote;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// A value of another CTA of the cluster at this CTA's shared address `address`.
+__device__ __forceinline__ void cluster_read(float &v, uint32_t address, uint32_t rank) {
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address(address, rank)) : "memory");
+}
+__device__ __forceinline__ void cluster_read(double &v, uint32_t address, uint32_t rank) {
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_address(address, rank)) : "memory");
+}
+
 }  // namespace pcu
 
 namespace pcu_host {
+
+// Once per device: the dynamic shared memory that a kernel may ask for, and whether it is launched
+// with the registers a thread that its warps share out.
+template <auto kernel> int allow_shared(int bytes, int registers = 0) {
+    static std::mutex lock;
+    static bool configured[64] = {false};
+    int device = 0;
+    if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return set_cuda_error(e);
+    std::lock_guard<std::mutex> guard(lock);
+    if (device < 64 && configured[device]) return PCU_B200_OK;
+    cudaFuncAttributes attributes;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attributes, kernel);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return set_cuda_error(e);
+    }
+    if (attributes.numRegs < registers) return PCU_B200_ERROR_UNSUPPORTED;
+    if (device < 64) configured[device] = true;
+    return PCU_B200_OK;
+}
+
+// A launch in clusters of `ranks` CTAs along x.
+template <typename... Params, typename... Args>
+int launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned block, size_t shared, unsigned ranks,
+                   cudaStream_t stream, const Args &...args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = ranks;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...); e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return set_cuda_error(e);
+    }
+    return PCU_B200_OK;
+}
 
 inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static std::once_flag once;
