@@ -35,6 +35,7 @@ template <typename T> struct DistillParams {
     uint64_t gradient_stride;
     int slice;            // elements of a row per CTA of its cluster (whole granules)
     uint32_t slice_bytes;
+    int claims;           // places of the table of claimed indices: a power of two, at least 2 k
     unsigned long long *status;
     ChainGuard guard;
 };
@@ -245,13 +246,14 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     using W = WideOf<T>;
     constexpr int V = 16 / sizeof(T), WARPS = kDistillThreads / 32;
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t landed[kMostChunks];
     __shared__ W part_m[WARPS], part_s[WARPS], share[2];
-    __shared__ double part_a[WARPS], part_mass[WARPS], part_terms[WARPS];
-    uint32_t ranks, rank;
+    __shared__ double part_a[WARPS], part_sums[3][WARPS];
+    __shared__ int part_flags[WARPS], repeated;
+    uint32_t ranks;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const uint32_t rank = cluster_rank();
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const uint64_t row = blockIdx.x / ranks;
     const T *z = p.logits + row * p.stride;
@@ -259,12 +261,13 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     const uint32_t phase = (uint32_t)(reinterpret_cast<uintptr_t>(z) % 16 / sizeof(T));
     const int vocab = (int)p.vocab;
     const int v0 = max(0, (int)((int64_t)rank * p.slice) - (int)phase);
-    const int v1 = min(vocab, (int)((int64_t)(rank + 1) * p.slice) - (int)phase);
+    const int v1 = (int)min((int64_t)vocab, (int64_t)(rank + 1) * p.slice - phase);
     const int lead = rank == 0 ? (int)phase : 0;  // elements of the first granule in front of v0
     const int count = max(0, v1 - v0), granules = (lead + count + V - 1) / V;
+    const int whole0 = lead ? 1 : 0, whole1 = (lead + count) / V;  // granules [whole0, whole1) are not cut
     T *slice = reinterpret_cast<T *>(smem);  // element v at slice[lead + v - v0]
     double *prob = reinterpret_cast<double *>(smem + p.slice_bytes);
-    int *place = reinterpret_cast<int *>(prob + p.k);
+    int *place = reinterpret_cast<int *>(prob + p.k), *claimed = place + p.k;
     const int chunks = (granules * 16 + kChunk - 1) / kChunk;
     T *g = p.gradient ? p.gradient + row * p.gradient_stride : nullptr;
     const W weight = p.weights ? p.weights[row] : W(1), c = p.to_log2;
@@ -273,6 +276,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     if (tid == 0) {
         for (int i = 0; i < chunks; ++i) mbar_init(&landed[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        repeated = 0;
     }
     // the teacher's entries: exponents t / T, -infinity for absent ones
     double a_max = -INFINITY;
@@ -287,8 +291,23 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         if (there) flags |= 1;
         a_max = fmax(a_max, prob[j]);
     }
-    const bool bad = __syncthreads_or(flags & 2);
-    if (weight == W(0) || (!__syncthreads_or(flags & 1) && !bad)) {  // nothing to learn from: the row is not read
+    for (int j = tid; j < p.claims; j += kDistillThreads) claimed[j] = -1;
+    if (tid < V) {  // the elements of cut granules; whole ones come by bulk copies below
+        const W absent = -INFINITY;
+        if (lead) slice[tid] = tid < lead || tid - lead >= count ? Elem<T>::round(absent) : z[v0 + tid - lead];
+        const int at = whole1 * V + tid;
+        if (whole1 < granules && (whole1 > 0 || !lead))
+            slice[at] = at - lead < count ? z[v0 + at - lead] : Elem<T>::round(absent);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a_max = fmax(a_max, __shfl_xor_sync(~0u, a_max, o));
+    flags = __reduce_or_sync(~0u, flags);
+    if (lane == 0) part_a[warp] = a_max, part_flags[warp] = flags;
+    __syncthreads();
+    a_max = part_a[0], flags = part_flags[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) a_max = fmax(a_max, part_a[i]), flags |= part_flags[i];
+    if (weight == W(0) || !flags) {  // nothing to learn from
         if (tid == 0 && rank == 0) {
             if (p.loss) p.loss[row] = W(0);
             if (p.stats_out) p.stats_out[2 * row] = W(0), p.stats_out[2 * row + 1] = W(1);
@@ -297,9 +316,6 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
             for (int v = v0 + tid; v < v1; v += kDistillThreads) g[v] = Elem<T>::round(W(0));
         return;  // every CTA of the cluster
     }
-
-    // whole granules by bulk copies, the elements of cut ones by threads
-    const int whole0 = lead ? 1 : 0, whole1 = (lead + count) / V;
     if (tid == 0)
         for (int i = 0; i < chunks; ++i) {
             const int a = max(whole0, i * (kChunk / 16)), b = min(whole1, (i + 1) * (kChunk / 16));
@@ -310,14 +326,37 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
                 mbar_arrive(&landed[i]);
             }
         }
-    if (tid < V) {
-        const W absent = -INFINITY;
-        if (lead) slice[tid] = tid < lead || tid - lead >= count ? Elem<T>::round(absent) : z[v0 + tid - lead];
-        const int at = whole1 * V + tid;  // the last granule, if it is cut
-        if (whole1 < granules && (whole1 > 0 || !lead))
-            slice[at] = at - lead < count ? z[v0 + at - lead] : Elem<T>::round(absent);
+
+    // While the slice is on its way, the sums over the entries, with e_j = exp(a_j - a_max):
+    //   mass = sum e_j, lean = sum e_j (a_j - a_max), named = sum e_j z_j,
+    // from which loss / (w T^2) = (lean - (named - m mass) / T) / mass + ln s - ln mass.  The logits that
+    // the teacher names are read here from anywhere in the row, before any CTA overwrites it in place.
+    // A table notes whether an index appears twice (see the end).
+    double mass = 0, lean = 0, named = 0;
+    for (int j = tid; j < p.k; j += kDistillThreads) {
+        const int at = place[j];
+        if (at < 0) continue;
+        const double a = prob[j] - a_max, e = exp(a);
+        mass += e;
+        if (p.loss && e > 0) lean += e * a, named += e * (double)Elem<T>::load(z[at]);
+        prob[j] = e;
+        if (g)
+            for (unsigned at_table = (unsigned)at * 2654435761u;; ++at_table) {  // at most half of it is taken
+                const int was = atomicCAS(&claimed[at_table & (p.claims - 1)], -1, at);
+                if (was == -1) break;
+                if (was == at) {
+                    repeated = 1;
+                    break;
+                }
+            }
     }
-    __syncthreads();
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        mass += __shfl_xor_sync(~0u, mass, o);
+        lean += __shfl_xor_sync(~0u, lean, o);
+        named += __shfl_xor_sync(~0u, named, o);
+    }
+    if (lane == 0) part_sums[0][warp] = mass, part_sums[1][warp] = lean, part_sums[2][warp] = named;
 
     bool ok = true;
     W m, s, inverse;
@@ -373,71 +412,41 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         }
         if (lane == 0) part_m[warp] = m, part_s[warp] = s;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) a_max = fmax(a_max, __shfl_xor_sync(~0u, a_max, o));
-    if (lane == 0) part_a[warp] = a_max;
     __syncthreads();
-    a_max = part_a[0];
+    mass = part_sums[0][0];
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) a_max = fmax(a_max, part_a[i]);
+    for (int i = 1; i < WARPS; ++i) mass += part_sums[0][i];
     if (!p.stats_in) {
         m = part_m[0], s = part_s[0];
 #pragma unroll
         for (int i = 1; i < WARPS; ++i) join(m, s, part_m[i], part_s[i], c);
-    }
-    // The logits that the teacher names.  For the loss from anywhere in the row, before any CTA of the
-    // cluster may overwrite it.
-    double here[(PCU_B200_DISTILL_TOP_MAX + kDistillThreads - 1) / kDistillThreads];
-    if (p.loss)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int j = tid + i * kDistillThreads;
-            if (j < p.k && place[j] >= 0) here[i] = (double)Elem<T>::load(z[place[j]]);
-        }
-    if (!p.stats_in && ranks > 1) {
-        if (tid == 0) share[0] = m, share[1] = s;
-        cluster_sync();
-        // in rank order in every CTA: the same bits everywhere
-        for (uint32_t r = 0; r < ranks; ++r) {
-            W m2, s2;
-            cluster_read(m2, smem_addr(&share[0]), r);
-            cluster_read(s2, smem_addr(&share[1]), r);
-            if (r == 0) m = m2, s = s2;
-            else join(m, s, m2, s2, c);
+        if (ranks > 1) {
+            if (tid == 0) share[0] = m, share[1] = s;
+            cluster_sync();
+            // in rank order in every CTA: the same bits everywhere
+            for (uint32_t r = 0; r < ranks; ++r) {
+                W m2, s2;
+                cluster_read(m2, smem_addr(&share[0]), r);
+                cluster_read(s2, smem_addr(&share[1]), r);
+                if (r == 0) m = m2, s = s2;
+                else join(m, s, m2, s2, c);
+            }
+            // read; this CTA waits for the others' readings when it ends
+            asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         }
     }
     const W up = p.upstream ? p.upstream[p.upstream_uniform ? 0 : row] : W(1);
-    const bool invalid = bad || !isfinite(m) || !isfinite(s) || !(s > W(0)) || !isfinite(weight) || (g && !isfinite(up));
-
-    // with e_j = exp(a_j - a_max): loss / (w T^2) = sum e_j (a_j - a_max - ln q_j) / sum e_j - ln(sum e_j)
-    double mass = 0, terms = 0;
-    const double ln_s = p.loss && !invalid ? log((double)s) : 0.0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int j = tid + i * kDistillThreads;
-        if (j < p.k && place[j] >= 0) {
-            const double a = prob[j] - a_max, e = exp(a);
-            mass += e;
-            if (p.loss && e > 0) terms += e * (a - ((here[i] - (double)m) * t_inverse - ln_s));
-            prob[j] = e;
-        }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        mass += __shfl_xor_sync(~0u, mass, o);
-        terms += __shfl_xor_sync(~0u, terms, o);
-    }
-    if (lane == 0) part_mass[warp] = mass, part_terms[warp] = terms;
-    __syncthreads();
-    mass = part_mass[0], terms = part_terms[0];
-#pragma unroll
-    for (int i = 1; i < WARPS; ++i) mass += part_mass[i], terms += part_terms[i];
-
+    const bool invalid = (flags & 2) || !isfinite(m) || !isfinite(s) || !(s > W(0)) || !isfinite(weight) || (g && !isfinite(up));
     unsigned kind = invalid && tid == 0 ? (unsigned)PCU_B200_KIND_INVALID : 0u;
     if (rank == 0 && tid == 0) {
         if (p.loss) {
+            lean = part_sums[1][0], named = part_sums[2][0];
+#pragma unroll
+            for (int i = 1; i < WARPS; ++i) lean += part_sums[1][i], named += part_sums[2][i];
             const double t = (double)p.temperature;
-            const W value = invalid ? W(NAN) : (W)((double)weight * t * t * (terms / mass - log(mass)));
+            const W value = invalid ? W(NAN)
+                                    : (W)((double)weight * t * t *
+                                          ((lean - (named - (double)m * mass) * t_inverse) / mass + log((double)s) - log(mass)));
             p.loss[row] = value;
             if (!kind) kind = result_kind(value);
         }
@@ -500,12 +509,14 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         for (int j = tid; j < p.k; j += kDistillThreads) {
             const int at = place[j];
             if (at < v0 || at >= v1) continue;
-            bool first = true;  // the first entry of an index carries the sum of all of them
-            for (int i = 0; i < j; ++i) first &= place[i] != at;
-            if (!first) continue;
             double sum = prob[j];
-            for (int i = j + 1; i < p.k; ++i)
-                if (place[i] == at) sum += prob[i];
+            if (repeated) {  // the first entry of an index carries the sum of all of them
+                bool first = true;
+                for (int i = 0; i < j; ++i) first &= place[i] != at;
+                if (!first) continue;
+                for (int i = j + 1; i < p.k; ++i)
+                    if (place[i] == at) sum += prob[i];
+            }
             const W q = term(run, Elem<T>::load(slice[lead + at - v0]), c) * inverse;
             const T r = Elem<T>::round(factor * (q - (W)(sum / mass)));
             worst = max(worst, result_kind(Elem<T>::load(r)));
@@ -518,10 +529,8 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     // nothing is left in flight towards this CTA's shared memory, and the cluster has read it
     if (tid == 0)
         for (int i = 0; i < chunks; ++i) mbar_wait(&landed[i], 0);
-    if (!p.stats_in && ranks > 1) {
-        __syncwarp();
-        cluster_sync();
-    }
+    __syncwarp();
+    if (!p.stats_in && ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // Rows go through shared memory where a cluster of 8 holds one.  The smallest cluster whose slices are
@@ -534,7 +543,9 @@ static int launch_distill(DistillParams<T> p, uint64_t rows, cudaStream_t stream
     while (ranks < 8 && bytes > ranks * 65536ull) ranks *= 2;
     while (ranks < 8 && rows * ranks < 2 * sms && bytes > ranks * 16384ull) ranks *= 2;
     const uint64_t slice_bytes = (bytes + ranks - 1) / ranks / 16 * 16 + 16;
-    const uint64_t need = slice_bytes + (uint64_t)p.k * (sizeof(double) + sizeof(int));
+    p.claims = 1;
+    while (p.claims < 2 * p.k) p.claims *= 2;
+    const uint64_t need = slice_bytes + (uint64_t)p.k * (sizeof(double) + sizeof(int)) + (uint64_t)p.claims * sizeof(int);
     if (slice_bytes > (uint64_t)kMostChunks * kChunk || need > 216 * 1024 || rows * ranks > 0x7fffffffull) {
         distill_kernel<T><<<(unsigned)rows, kDistillThreads, 0, stream>>>(p);
         return pcu_host::launch_status();
