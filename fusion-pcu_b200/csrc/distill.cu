@@ -367,20 +367,21 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     } else {
         refer(run, -INFINITY, c);
         run.s = W(0);
+        alignas(16) T nothing[V];
+        for (int e = 0; e < V; ++e) nothing[e] = Elem<T>::round(W(-INFINITY));
+        const uint4 absent = *reinterpret_cast<const uint4 *>(nothing);
         for (int i = 0; i < chunks; ++i) {
             ok = ok && mbar_wait(&landed[i], 0);
+            if (i * (kChunk / 16) + warp * 32 >= granules) break;  // the warp has no granule in this last chunk
             W x[4][V];
             W top = -INFINITY;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int at = i * (kChunk / 16) + q * kDistillThreads + tid;
-                uint4 raw;
+                uint4 raw = absent;
                 if (at < granules) raw = *reinterpret_cast<const uint4 *>(slice + at * V);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    x[q][e] = at < granules ? Elem<T>::load(reinterpret_cast<const T *>(&raw)[e]) : W(-INFINITY);
-                    top = fmax(top, x[q][e]);
-                }
+                unpack<T>(raw, x[q]);
+                top = fmax(top, largest<T>(raw, x[q]));
             }
             if (top > run.m) raise(run, top, c);
             if (run.m == -INFINITY) {  // nothing but masked entries so far, or NaN
@@ -465,45 +466,47 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         W seen = 0;
         unsigned worst = 0;
         const bool aligned = (reinterpret_cast<uintptr_t>(g + v0) - lead * sizeof(T)) % 16 == 0;
-        auto sweep = [&](auto plain_) {
-            constexpr bool plain = decltype(plain_)::value;  // neither far nor check: the case that counts
-            auto value = [&](T x) {
-                const W e = plain ? fast_exp2(fma(Elem<T>::load(x), c, -run.hi)) : term(run, Elem<T>::load(x), c);
-                if (p.stats_in) seen += e;
-                const T r = Elem<T>::round(scale * e);
-                if (!plain && check) worst = max(worst, result_kind(Elem<T>::load(r)));
-                return r;
+        // plain: neither far nor check; first: no pass has read the slice yet
+        auto sweep = [&](auto plain_, auto first_) {
+            constexpr bool plain = decltype(plain_)::value, first = decltype(first_)::value;
+            auto value = [&](W x) {
+                const W e = plain ? fast_exp2(fma(x, c, -run.hi)) : term(run, x, c);
+                if (first) seen += e;
+                if (!plain && check) worst = max(worst, result_kind(Elem<T>::load(Elem<T>::round(scale * e))));
+                return scale * e;
             };
             if (aligned) {
                 for (int i = 0; i < chunks; ++i) {
-                    if (p.stats_in) ok = ok && mbar_wait(&landed[i], 0);
+                    if (first) ok = ok && mbar_wait(&landed[i], 0);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int at = i * (kChunk / 16) + q * kDistillThreads + tid;
                         if (at >= granules) break;
-                        const uint4 raw = *reinterpret_cast<const uint4 *>(slice + at * V);
-                        alignas(16) T r[V];
+                        W x[V];
+                        unpack<T>(*reinterpret_cast<const uint4 *>(slice + at * V), x);
 #pragma unroll
-                        for (int e = 0; e < V; ++e) r[e] = value(reinterpret_cast<const T *>(&raw)[e]);
+                        for (int e = 0; e < V; ++e) x[e] = value(x[e]);
+                        const uint4 packed = pack<T>(x);
                         T *to = g + v0 + (at * V - lead);
                         if (at >= whole0 && at < whole1) {
-                            __stcs(reinterpret_cast<uint4 *>(to), *reinterpret_cast<const uint4 *>(r));
+                            __stcs(reinterpret_cast<uint4 *>(to), packed);
                         } else {
 #pragma unroll
                             for (int e = 0; e < V; ++e)
-                                if (at * V + e >= lead && at * V + e - lead < count) to[e] = r[e];
+                                if (at * V + e >= lead && at * V + e - lead < count) to[e] = reinterpret_cast<const T *>(&packed)[e];
                         }
                     }
                 }
             } else {  // the gradient's rows lie differently: element by element, adjacent lanes adjacent elements
-                if (p.stats_in)
+                if (first)
                     for (int i = 0; i < chunks; ++i) ok = ok && mbar_wait(&landed[i], 0);
 #pragma unroll 8
-                for (int v = tid; v < count; v += kDistillThreads) g[v0 + v] = value(slice[lead + v]);
+                for (int v = tid; v < count; v += kDistillThreads)
+                    g[v0 + v] = Elem<T>::round(value(Elem<T>::load(slice[lead + v])));
             }
         };
-        if (run.far || check) sweep(std::false_type{});
-        else sweep(std::true_type{});
+        if (run.far || check) p.stats_in ? sweep(std::false_type{}, std::true_type{}) : sweep(std::false_type{}, std::false_type{});
+        else p.stats_in ? sweep(std::true_type{}, std::true_type{}) : sweep(std::true_type{}, std::false_type{});
         if (!isfinite(seen) && !kind) kind = PCU_B200_KIND_INVALID;
         __syncthreads();  // before the entries' elements are written again
         for (int j = tid; j < p.k; j += kDistillThreads) {
@@ -538,11 +541,13 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
 // fill the SMs twice, larger ones down to slices of 8 KB.
 template <typename T>
 static int launch_distill(DistillParams<T> p, uint64_t rows, cudaStream_t stream) {
-    const uint64_t bytes = p.vocab * sizeof(T) + 16, sms = (uint64_t)pcu_host::sm_count();
+    // the bytes that a row's granules span: 16 more where rows can start inside one
+    const bool cut = reinterpret_cast<uintptr_t>(p.logits) % 16 || (rows > 1 && p.stride * sizeof(T) % 16);
+    const uint64_t bytes = (p.vocab * sizeof(T) + 15) / 16 * 16 + (cut ? 16 : 0), sms = (uint64_t)pcu_host::sm_count();
     unsigned ranks = 1;
     while (ranks < 8 && bytes > ranks * 65536ull) ranks *= 2;
     while (ranks < 8 && rows * ranks < 2 * sms && bytes > ranks * 16384ull) ranks *= 2;
-    const uint64_t slice_bytes = (bytes + ranks - 1) / ranks / 16 * 16 + 16;
+    const uint64_t slice_bytes = (bytes / 16 + ranks - 1) / ranks * 16;
     p.claims = 1;
     while (p.claims < 2 * p.k) p.claims *= 2;
     const uint64_t need = slice_bytes + (uint64_t)p.k * (sizeof(double) + sizeof(int)) + (uint64_t)p.claims * sizeof(int);

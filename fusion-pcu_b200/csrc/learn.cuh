@@ -39,6 +39,62 @@ template <> struct Elem<__nv_bfloat16> {
 };
 template <typename T> using WideOf = typename Elem<T>::Wide;
 
+// 16 bytes of elements to wide values and back, two to a word where the types are 16 bits wide.
+template <typename T> __device__ __forceinline__ void unpack(uint4 raw, WideOf<T> (&v)[16 / sizeof(T)]) {
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); ++i) v[i] = Elem<T>::load(reinterpret_cast<const T *>(&raw)[i]);
+}
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint4 raw, float (&v)[8]) {
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void unpack<__half>(uint4 raw, float (&v)[8]) {
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+
+template <typename T> __device__ __forceinline__ uint4 pack(const WideOf<T> (&v)[16 / sizeof(T)]) {
+    alignas(16) T r[16 / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); ++i) r[i] = Elem<T>::round(v[i]);
+    return *reinterpret_cast<const uint4 *>(r);
+}
+template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float (&v)[8]) {
+    __nv_bfloat162 r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    return *reinterpret_cast<const uint4 *>(r);
+}
+template <> __device__ __forceinline__ uint4 pack<__half>(const float (&v)[8]) {
+    __half2 r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    return *reinterpret_cast<const uint4 *>(r);
+}
+
+// The largest of 16 bytes of elements; NaN loses against a number.
+template <typename T> __device__ __forceinline__ WideOf<T> largest(uint4 raw, const WideOf<T> (&v)[16 / sizeof(T)]) {
+    WideOf<T> top = v[0];
+#pragma unroll
+    for (int i = 1; i < (int)(16 / sizeof(T)); ++i) top = fmax(top, v[i]);
+    return top;
+}
+template <> __device__ __forceinline__ float largest<__nv_bfloat16>(uint4 raw, const float (&)[8]) {
+    const __nv_bfloat162 *w = reinterpret_cast<const __nv_bfloat162 *>(&raw);
+    const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+template <> __device__ __forceinline__ float largest<__half>(uint4 raw, const float (&)[8]) {
+    const __half2 *w = reinterpret_cast<const __half2 *>(&raw);
+    const __half2 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+
 // 2^x.  binary32: the hardware's approximation (2 ulp), results below 2^-126 flushed to zero --
 // these are softmax terms, summed with one that is 1.  binary64: the library function.
 __device__ __forceinline__ float fast_exp2(float x) {
