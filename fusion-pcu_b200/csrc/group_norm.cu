@@ -5,8 +5,19 @@
 //   z = h w + b, y = act(z);
 // backward: dz = dy act'(z), db = sum dz, dw = sum dz h (over n and s),
 //   c1 = sum_g dz w / m, c2 = sum_g dz w h / m, dx = r (dz w - c1 - h c2).
+//
+// All of it is bound by memory: x (and dy) in, y (dx) out.  Three ways to read the inputs once:
+//   * warp form: a group of at most 512 elements sits in the registers of 4 to 32 lanes;
+//   * slab form: a block of whole groups of one n sits in the shared memory of a cluster of CTAs;
+//   * stream form, for what fits neither: one pass for sums of row chunks, one that applies them.
+// The variance is taken about the mean in every form (in the stream form within each thread about
+// its first element, joined about the joint means).
+#include <algorithm>
+#include <numeric>
+
 #include "learn.cuh"
 #include "provider.h"
+#include "tma.cuh"
 
 namespace pcu {
 
@@ -19,6 +30,21 @@ template <typename T> struct Maps {
     __device__ __forceinline__ T *at(uint64_t n, uint64_t s, uint64_t c) const { return base + n * batch + s * row + c; }
 };
 
+// How a call is carried out; a function of the sizes and of whether 16-byte accesses are possible.
+struct NormPlan {
+    enum Form { kWarp, kSlab, kStream } form;
+    int vector;                // elements per access
+    int per_lane, lanes;       // warp form: accesses per lane, lanes per group (a power of two)
+    unsigned items, slices;    // accesses per group; parts of the batch
+    unsigned block_groups, blocks, ranks, threads;  // slab form: groups per cluster, of one n; CTAs
+    unsigned slab_rows;
+    size_t shared;
+    unsigned tiles, tile, chunks;  // stream form: column tiles of `tile` accesses, row chunks
+    uint64_t chunk_rows;
+    uint64_t partial_rows, partial_split;  // parameters' gradients: partial sums [rows][2][groups][split][width]
+    uint64_t workspace;                    // elements of the wide type
+};
+
 template <typename T> struct NormParams {
     using W = WideOf<T>;
     Maps<const T> x, dy;
@@ -26,43 +52,582 @@ template <typename T> struct NormParams {
     const W *weight, *bias;
     W *stats_out;
     const W *stats;
-    W *sums;  // workspace: (c1, c2) for each (n, g)
+    W *partial;  // workspace: partial sums
+    W *sums;     // workspace: (c1, c2) for each (n, g), stream form
     W *dweight, *dbias;
     uint64_t batch, positions, channels, groups, width;
     W eps;
+    int activation;
+    NormPlan plan;
     unsigned long long *status;
     ChainGuard guard;
 };
 
-template <int ACT, typename W> __device__ __forceinline__ W activate(W z) {
-    if (ACT == PCU_B200_ACTIVATION_RELU) return z < W(0) ? W(0) : z;  // NaN stays
-    if (ACT == PCU_B200_ACTIVATION_SILU) return z / (W(1) + exp(-z));
-    if (ACT == PCU_B200_ACTIVATION_GELU) return z * W(0.5) * erfc(z * W(-0.70710678118654752440));
-    return z;
-}
+// ---- activations, over the V elements of one access (the choice is the same for a whole launch)
 
-template <int ACT, typename W> __device__ __forceinline__ W slope(W z) {
-    if (ACT == PCU_B200_ACTIVATION_RELU) return z > W(0) ? W(1) : W(0);
-    if (ACT == PCU_B200_ACTIVATION_SILU) {
-        const W q = W(1) / (W(1) + exp(-z));
-        return q * (W(1) + z * (W(1) - q));
+__device__ __forceinline__ float logistic(float z) {
+    return __fdividef(1.0f, 1.0f + fast_exp2(z * -1.4426950408889634f));
+}
+__device__ __forceinline__ double logistic(double z) { return 1.0 / (1.0 + exp(-z)); }
+__device__ __forceinline__ float normal_density(float z) {
+    return fast_exp2(z * z * -0.72134752044448170f) * 0.39894228040143267794f;
+}
+__device__ __forceinline__ double normal_density(double z) { return exp(-0.5 * z * z) * 0.39894228040143267794; }
+
+template <int V, typename W> __device__ __forceinline__ void activate(int act, W (&z)[V]) {
+    if (act == PCU_B200_ACTIVATION_RELU) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] = z[e] < W(0) ? W(0) : z[e];  // NaN stays
+    } else if (act == PCU_B200_ACTIVATION_SILU) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] *= logistic(z[e]);
+    } else if (act == PCU_B200_ACTIVATION_GELU) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] *= W(0.5) * erfc(z[e] * W(-0.70710678118654752440));
     }
-    if (ACT == PCU_B200_ACTIVATION_GELU)
-        return W(0.5) * erfc(z * W(-0.70710678118654752440)) + z * exp(W(-0.5) * z * z) * W(0.39894228040143267794);
-    return W(1);
 }
 
-// act'(z) at z = h w + b, h = (x - mean) r.  ReLU's slope is a step, so a z within its own rounding
-// error of 0 (h and the product are each off by a few 2^-24) is decided in binary64.
-template <int ACT, typename W>
-__device__ __forceinline__ W slope_at(W x, W mean, W r, W h, W w, W b) {
-    const W z = h * w + b;
-    if (ACT == PCU_B200_ACTIVATION_RELU && sizeof(W) == 4 && fabs(z) <= (fabs(h * w) + fabs(b)) * W(0x1p-20))
-        return ((double)x - (double)mean) * (double)r * (double)w + (double)b > 0.0 ? W(1) : W(0);
-    return slope<ACT>(z);
+// h and k = dy act'(h w + b) w.  ReLU's slope is a step, so a z within its own rounding error of 0 (h
+// and the product are each off by a few 2^-24) is decided in binary64; dz = dy act' goes to `dz`.
+template <int V, typename W>
+__device__ __forceinline__ void bend(int act, const W (&x)[V], const W (&dy)[V], const W (&mean)[V], const W (&r)[V],
+                                     const W (&w)[V], const W (&b)[V], W (&h)[V], W (&dz)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[e] = (x[e] - mean[e]) * r[e], dz[e] = dy[e];
+    if (act == PCU_B200_ACTIVATION_RELU) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const W hw = h[e] * w[e], z = hw + b[e];
+            bool above = z > W(0);
+            if (sizeof(W) == 4 && fabs(z) <= (fabs(hw) + fabs(b[e])) * W(0x1p-20))
+                above = ((double)x[e] - (double)mean[e]) * (double)r[e] * (double)w[e] + (double)b[e] > 0.0;
+            dz[e] = above ? dz[e] : dz[e] * W(0);  // an infinite or NaN upstream shows
+        }
+    } else if (act == PCU_B200_ACTIVATION_SILU) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const W z = h[e] * w[e] + b[e], q = logistic(z);
+            dz[e] *= q * (W(1) + z * (W(1) - q));
+        }
+    } else if (act == PCU_B200_ACTIVATION_GELU) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const W z = h[e] * w[e] + b[e];
+            dz[e] *= W(0.5) * erfc(z * W(-0.70710678118654752440)) + z * normal_density(z);
+        }
+    }
 }
 
-template <typename V> __device__ __forceinline__ V norm_block_sum(V v, V *scratch) {
+// ---- accesses of V elements: 16 bytes, or one element
+
+template <typename T, int V> struct Access {
+    using W = WideOf<T>;
+    uint4 raw;
+    static __device__ __forceinline__ Access load(const T *p) { return {__ldcs(reinterpret_cast<const uint4 *>(p))}; }
+    __device__ __forceinline__ void open(W (&v)[V]) const { unpack<T>(raw, v); }
+};
+template <typename T> struct Access<T, 1> {
+    using W = WideOf<T>;
+    T raw;
+    static __device__ __forceinline__ Access load(const T *p) { return {*p}; }
+    __device__ __forceinline__ void open(W (&v)[1]) const { v[0] = Elem<T>::load(raw); }
+};
+
+// Stores V elements; what is not finite is recorded with its event.
+template <typename T, int V>
+__device__ __forceinline__ void put(T *to, const WideOf<T> (&v)[V], uint64_t event, unsigned long long *status) {
+    if constexpr (V == 1) {
+        const T y = Elem<T>::round(v[0]);
+        *to = y;
+        if (const unsigned kind = result_kind(Elem<T>::load(y))) record_fault(status, event, kind);
+    } else {
+        const uint4 y = pack<T>(v);
+        __stcs(reinterpret_cast<uint4 *>(to), y);
+        if (not_finite<T>(y))
+            for (int e = 0; e < V; ++e)
+                if (const unsigned kind = result_kind(Elem<T>::load(reinterpret_cast<const T *>(&y)[e])))
+                    record_fault(status, event + e, kind);
+    }
+}
+
+template <int V, typename W> __device__ __forceinline__ void parameters(const W *p, uint64_t c, W none, W (&v)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = p ? p[c + e] : none;
+}
+
+template <typename W> __device__ __forceinline__ W root(W var, W eps) {
+    // a variance that is not finite has no reciprocal root to scale by: NaN, not 0
+    return isfinite(var) ? W(1) / sqrt(var + eps) : W(NAN);
+}
+
+// ---- warp form
+//
+// `lanes` lanes hold a group, K accesses each; 32 / lanes adjacent groups per warp.  A warp keeps its
+// groups and walks over the batch, U at a time for loads in flight, so that the parameters stay in
+// registers, and their gradients too: each warp ends with one partial sum per element of its groups.
+template <typename T, int V, int K> struct WarpGroup {
+    using W = WideOf<T>;
+    int sub, slice;
+    uint64_t g;
+    bool active, there[K];
+    uint64_t row[K], channel[K];
+    W w[K][V], b[K][V];
+
+    __device__ __forceinline__ bool place(const NormParams<T> &p) {
+        const NormPlan &plan = p.plan;
+        const int lane = threadIdx.x % 32, per = 32 / plan.lanes;
+        const uint64_t warp = (uint64_t)blockIdx.x * (kNormThreads / 32) + threadIdx.x / 32;
+        const uint64_t sets = (p.groups + per - 1) / per;
+        if (warp >= sets * plan.slices) return false;
+        sub = lane % plan.lanes;
+        slice = (int)(warp / sets);
+        g = warp % sets * per + lane / plan.lanes;
+        active = g < p.groups;
+        const unsigned across = (unsigned)(p.width / V);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const unsigned item = sub + k * plan.lanes;
+            there[k] = active && item < plan.items;
+            row[k] = there[k] ? item / across : 0;
+            channel[k] = there[k] ? g * p.width + item % across * V : 0;
+            parameters<V>(p.weight, channel[k], W(1), w[k]);
+            parameters<V>(p.bias, channel[k], W(0), b[k]);
+        }
+        return true;
+    }
+};
+
+template <int U, typename W> __device__ __forceinline__ void lanes_sum(W (&v)[U], int lanes) {
+    for (int o = lanes / 2; o; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(~0u, v[u], o);
+}
+
+template <typename T, int V, int K, int U>
+__global__ void __launch_bounds__(kNormThreads) norm_warp_kernel(const NormParams<T> p) {
+    using W = WideOf<T>;
+    if (!chain_admits(p.guard)) return;
+    WarpGroup<T, V, K> at;
+    if (!at.place(p)) return;
+    const W inverse = W(1) / (W)(p.positions * p.width);
+    for (uint64_t n = (uint64_t)at.slice * U; n < p.batch; n += (uint64_t)p.plan.slices * U) {
+        W x[U][K][V], mean[U] = {}, square[U] = {};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (at.there[k] && n + u < p.batch) Access<T, V>::load(p.x.at(n + u, at.row[k], at.channel[k])).open(x[u][k]);
+                else
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[u][k][e] = W(0);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) mean[u] += x[u][k][e];
+        lanes_sum(mean, p.plan.lanes);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            mean[u] *= inverse;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[u][k][e] -= mean[u];
+                    if (at.there[k]) square[u] += x[u][k][e] * x[u][k][e];
+                }
+        }
+        lanes_sum(square, p.plan.lanes);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (n + u >= p.batch) break;
+            const W r = root(square[u] * inverse, p.eps);
+            if (at.sub == 0 && at.active) {
+                p.stats_out[2 * ((n + u) * p.groups + at.g)] = mean[u];
+                p.stats_out[2 * ((n + u) * p.groups + at.g) + 1] = r;
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!at.there[k]) continue;
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[u][k][e] = x[u][k][e] * r * at.w[k][e] + at.b[k][e];
+                activate<V>(p.activation, x[u][k]);
+                put<T, V>(p.out.at(n + u, at.row[k], at.channel[k]), x[u][k],
+                          ((n + u) * p.positions + at.row[k]) * p.channels + at.channel[k], p.status);
+            }
+        }
+    }
+}
+
+template <typename T, int V, int K, int U>
+__global__ void __launch_bounds__(kNormThreads) norm_warp_backward_kernel(const NormParams<T> p) {
+    using W = WideOf<T>;
+    if (!chain_admits(p.guard)) return;
+    WarpGroup<T, V, K> at;
+    if (!at.place(p)) return;
+    const W inverse = W(1) / (W)(p.positions * p.width);
+    W dw[K][V] = {}, db[K][V] = {};
+    for (uint64_t n = (uint64_t)at.slice * U; n < p.batch; n += (uint64_t)p.plan.slices * U) {
+        W x[U][K][V], dy[U][K][V], c1[U] = {}, c2[U] = {}, r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (at.there[k] && n + u < p.batch) {
+                    Access<T, V>::load(p.x.at(n + u, at.row[k], at.channel[k])).open(x[u][k]);
+                    Access<T, V>::load(p.dy.at(n + u, at.row[k], at.channel[k])).open(dy[u][k]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[u][k][e] = dy[u][k][e] = W(0);
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool live = at.active && n + u < p.batch;
+            const W mean = live ? p.stats[2 * ((n + u) * p.groups + at.g)] : W(0);
+            r[u] = live ? p.stats[2 * ((n + u) * p.groups + at.g) + 1] : W(0);
+            W means[V], rs[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) means[e] = mean, rs[e] = r[u];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!at.there[k] || !live) continue;
+                W h[V], dz[V];
+                bend<V>(p.activation, x[u][k], dy[u][k], means, rs, at.w[k], at.b[k], h, dz);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    dw[k][e] += dz[e] * h[e];
+                    db[k][e] += dz[e];
+                    const W d = dz[e] * at.w[k][e];
+                    c1[u] += d;
+                    c2[u] += d * h[e];
+                    x[u][k][e] = h[e], dy[u][k][e] = d;
+                }
+            }
+        }
+        lanes_sum(c1, p.plan.lanes);
+        lanes_sum(c2, p.plan.lanes);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (n + u >= p.batch) break;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!at.there[k]) continue;
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    x[u][k][e] = r[u] * (dy[u][k][e] - c1[u] * inverse - x[u][k][e] * (c2[u] * inverse));
+                put<T, V>(p.out.at(n + u, at.row[k], at.channel[k]), x[u][k],
+                          ((n + u) * p.positions + at.row[k]) * p.channels + at.channel[k], p.status);
+            }
+        }
+    }
+    if (!p.partial) return;
+    const uint64_t whole = p.groups * p.plan.items * V;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (at.there[k]) {
+            const uint64_t to = 2 * at.slice * whole + (at.g * p.plan.items + at.sub + k * p.plan.lanes) * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) p.partial[to + e] = dw[k][e], p.partial[to + whole + e] = db[k][e];
+        }
+}
+
+// ---- columns: the thread mapping of the slab and stream forms
+//
+// A thread keeps one access of columns and takes every `deep`-th row, so a channel's parameters,
+// statistics and sums stay in its registers.
+
+// Sums over the rows' threads and a group's channels: `v` (one value per channel of each thread's
+// access) to total[group] in shared memory.  One warp per group, in a fixed order.
+template <int V, typename W>
+__device__ __forceinline__ void group_sums(const W (&v)[V], bool active, int tx, int ty, int across, int deep, int groups,
+                                           int width, W *scratch, W *total) {
+    __syncthreads();
+    if (active)
+#pragma unroll
+        for (int e = 0; e < V; ++e) scratch[(ty * across + tx) * V + e] = v[e];
+    __syncthreads();
+    const int warps = blockDim.x / 32;
+    for (int g = threadIdx.x / 32; g < groups; g += warps) {
+        W sum = 0;
+        for (int i = threadIdx.x % 32; i < deep * width; i += 32) sum += scratch[i / width * across * V + g * width + i % width];
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (threadIdx.x % 32 == 0) total[g] = sum;
+    }
+    __syncthreads();
+}
+
+// ---- slab form
+//
+// A cluster's CTAs hold `slab_rows` rows each of a block of whole groups of one n in shared memory.  A
+// thread copies in and reads back only its own accesses.  Sums are joined through the cluster in
+// rank order.
+template <typename T, int V> struct Slab {
+    using W = WideOf<T>;
+    uint64_t n, c0, s0;
+    int groups, across, deep, tx, ty, rows;
+    uint32_t rank, ranks;
+    bool active;
+    unsigned char *data;
+    W *scratch, *total, *joined;
+
+    __device__ __forceinline__ void place(const NormParams<T> &p, unsigned char *smem, int tensors) {
+        const NormPlan &plan = p.plan;
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+        rank = cluster_rank();
+        const unsigned cluster = blockIdx.x / ranks, block = cluster % plan.blocks;
+        n = cluster / plan.blocks;
+        const uint64_t g0 = (uint64_t)block * plan.block_groups;
+        groups = (int)min((uint64_t)plan.block_groups, p.groups - g0);
+        c0 = g0 * p.width;
+        across = (int)(groups * p.width / V);
+        deep = (int)blockDim.x / across;
+        tx = (int)threadIdx.x % across;
+        ty = (int)threadIdx.x / across;
+        active = ty < deep;
+        s0 = (uint64_t)rank * plan.slab_rows;
+        rows = s0 < p.positions ? (int)min((uint64_t)plan.slab_rows, p.positions - s0) : 0;
+        data = smem;
+        scratch = reinterpret_cast<W *>(smem + (size_t)tensors * slab_bytes(plan, p));
+        total = scratch + blockDim.x * V;
+        joined = total + 2 * plan.block_groups;
+    }
+    static __host__ __device__ __forceinline__ size_t slab_bytes(const NormPlan &plan, uint64_t width) {
+        return ((size_t)plan.slab_rows * plan.block_groups * width * sizeof(T) + 15) / 16 * 16;
+    }
+    __device__ __forceinline__ size_t slab_bytes(const NormPlan &plan, const NormParams<T> &p) const {
+        return slab_bytes(plan, p.width);
+    }
+    __device__ __forceinline__ T *element(int tensor, const NormParams<T> &p, int r) const {
+        return reinterpret_cast<T *>(data + (size_t)tensor * slab_bytes(p.plan, p)) + ((size_t)r * across + tx) * V;
+    }
+    __device__ __forceinline__ void bring(int tensor, const NormParams<T> &p, const Maps<const T> &from) const {
+        if (!active) return;
+        for (int r = ty; r < rows; r += deep) {
+            const T *src = from.at(n, s0 + r, c0 + (uint64_t)tx * V);
+            T *dst = element(tensor, p, r);
+            if (V > 1)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+            else
+                *dst = *src;
+        }
+    }
+    __device__ __forceinline__ void read(int tensor, const NormParams<T> &p, int r, W (&v)[V]) const {
+        if constexpr (V > 1) unpack<T>(*reinterpret_cast<const uint4 *>(element(tensor, p, r)), v);
+        else v[0] = Elem<T>::load(*element(tensor, p, r));
+    }
+    // sums `slot` of all the cluster's CTAs, in every CTA
+    __device__ __forceinline__ void sum(const W (&v)[V], int slot, const NormParams<T> &p) const {
+        W *mine = total + slot * p.plan.block_groups;
+        group_sums<V>(v, active, tx, ty, across, deep, groups, (int)p.width, scratch, mine);
+        if (ranks > 1) cluster_sync();
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+            W all = ranks > 1 ? W(0) : mine[g];
+            if (ranks > 1)
+                for (uint32_t r = 0; r < ranks; ++r) {
+                    W v2;
+                    cluster_read(v2, smem_addr(mine + g), r);
+                    all += v2;
+                }
+            joined[slot * p.plan.block_groups + g] = all;
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ W sum_of(int slot, int e, const NormParams<T> &p) const {
+        return joined[slot * p.plan.block_groups + (tx * V + e) / (int)p.width];
+    }
+};
+
+template <typename T, int V> __global__ void __launch_bounds__(512) norm_slab_kernel(const NormParams<T> p) {
+    using W = WideOf<T>;
+    if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
+    extern __shared__ __align__(16) unsigned char smem[];
+    Slab<T, V> at;
+    at.place(p, smem, 1);
+    at.bring(0, p, p.x);
+    const uint64_t c = at.c0 + (uint64_t)at.tx * V;
+    W w[V], b[V];
+    if (at.active) parameters<V>(p.weight, c, W(1), w), parameters<V>(p.bias, c, W(0), b);
+    const W inverse = W(1) / ((W)p.positions * (W)p.width);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    W v[V] = {}, x[V], mean[V], r[V];
+    if (at.active)
+        for (int i = at.ty; i < at.rows; i += at.deep) {
+            at.read(0, p, i, x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += x[e];
+        }
+    at.sum(v, 0, p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) mean[e] = at.active ? at.sum_of(0, e, p) * inverse : W(0), v[e] = W(0);
+    if (at.active)
+        for (int i = at.ty; i < at.rows; i += at.deep) {
+            at.read(0, p, i, x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += (x[e] - mean[e]) * (x[e] - mean[e]);
+        }
+    at.sum(v, 1, p);
+    if (at.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // read; see the end
+    if (at.rank == 0)
+        for (int g = threadIdx.x; g < at.groups; g += blockDim.x) {
+            W *to = p.stats_out + 2 * (at.n * p.groups + at.c0 / p.width + g);
+            to[0] = at.joined[g] * inverse;
+            to[1] = root(at.joined[p.plan.block_groups + g] * inverse, p.eps);
+        }
+    if (at.active) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[e] = root(at.sum_of(1, e, p) * inverse, p.eps);
+        for (int i = at.ty; i < at.rows; i += at.deep) {
+            at.read(0, p, i, x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = (x[e] - mean[e]) * r[e] * w[e] + b[e];
+            activate<V>(p.activation, x);
+            put<T, V>(p.out.at(at.n, at.s0 + i, c), x, (at.n * p.positions + at.s0 + i) * p.channels + c, p.status);
+        }
+    }
+    __syncwarp();
+    // the other CTAs may still read this one's sums
+    if (at.ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+template <typename T, int V> __global__ void __launch_bounds__(512) norm_slab_backward_kernel(const NormParams<T> p) {
+    using W = WideOf<T>;
+    if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
+    extern __shared__ __align__(16) unsigned char smem[];
+    Slab<T, V> at;
+    at.place(p, smem, 2);
+    at.bring(0, p, p.x);
+    at.bring(1, p, p.dy);
+    const uint64_t c = at.c0 + (uint64_t)at.tx * V;
+    W w[V], b[V], mean[V], r[V], dw[V] = {}, db[V] = {}, x[V], dy[V], h[V], dz[V];
+    if (at.active) {
+        parameters<V>(p.weight, c, W(1), w), parameters<V>(p.bias, c, W(0), b);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const W *st = p.stats + 2 * (at.n * p.groups + (c + e) / p.width);
+            mean[e] = st[0], r[e] = st[1];
+        }
+    }
+    const W inverse = W(1) / ((W)p.positions * (W)p.width);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (at.active)
+        for (int i = at.ty; i < at.rows; i += at.deep) {
+            at.read(0, p, i, x);
+            at.read(1, p, i, dy);
+            bend<V>(p.activation, x, dy, mean, r, w, b, h, dz);
+#pragma unroll
+            for (int e = 0; e < V; ++e) dw[e] += dz[e] * h[e], db[e] += dz[e];
+        }
+    if (p.partial) {  // this CTA's share of the parameters' gradients, summed over its rows' threads
+        W *to = p.partial + 2 * (at.n * at.ranks + at.rank) * p.channels + at.c0;
+        for (int q = 0; q < 2; ++q) {
+            __syncthreads();
+            if (at.active)
+#pragma unroll
+                for (int e = 0; e < V; ++e) at.scratch[(at.ty * at.across + at.tx) * V + e] = q ? db[e] : dw[e];
+            __syncthreads();
+            for (int i = threadIdx.x; i < at.across * V; i += blockDim.x) {
+                W sum = 0;
+                for (int d = 0; d < at.deep; ++d) sum += at.scratch[d * at.across * V + i];
+                to[q * p.channels + i] = sum;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[e] = at.active ? dw[e] * w[e] : W(0), db[e] = at.active ? db[e] * w[e] : W(0);
+    at.sum(db, 0, p);
+    at.sum(dw, 1, p);
+    if (at.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // read; see the end
+    if (at.active) {
+        W c1[V], c2[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) c1[e] = at.sum_of(0, e, p) * inverse, c2[e] = at.sum_of(1, e, p) * inverse;
+        for (int i = at.ty; i < at.rows; i += at.deep) {
+            at.read(0, p, i, x);
+            at.read(1, p, i, dy);
+            bend<V>(p.activation, x, dy, mean, r, w, b, h, dz);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = r[e] * (dz[e] * w[e] - c1[e] - h[e] * c2[e]);
+            put<T, V>(p.out.at(at.n, at.s0 + i, c), x, (at.n * p.positions + at.s0 + i) * p.channels + c, p.status);
+        }
+    }
+    __syncwarp();
+    // the other CTAs may still read this one's sums
+    if (at.ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// ---- stream form
+template <typename T, int V> struct Stream {
+    uint64_t n, s0, s1, c;
+    int across, deep, tx, ty;
+    unsigned chunk;
+    bool active;
+    __device__ __forceinline__ Stream(const NormParams<T> &p) {
+        const NormPlan &plan = p.plan;
+        chunk = blockIdx.x % plan.chunks;
+        const unsigned tile = blockIdx.x / plan.chunks % plan.tiles;
+        n = blockIdx.x / plan.chunks / plan.tiles;
+        const uint64_t first = (uint64_t)tile * plan.tile, all = p.channels / V;
+        across = (int)min((uint64_t)plan.tile, all - first);
+        deep = (int)blockDim.x / across;
+        tx = (int)threadIdx.x % across;
+        ty = (int)threadIdx.x / across;
+        active = ty < deep;
+        c = (first + tx) * V;
+        s0 = chunk * plan.chunk_rows;
+        s1 = min(p.positions, s0 + plan.chunk_rows);
+    }
+};
+
+// (mean, sum of squares about it) of each channel over a chunk's rows: partial[n][chunk][channel][2].
+template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_stats_kernel(const NormParams<T> p) {
+    using W = WideOf<T>;
+    if (!chain_admits(p.guard)) return;
+    __shared__ W means[kNormThreads * V], squares[kNormThreads * V];
+    const Stream<T, V> at(p);
+    W first[V], sum[V] = {}, square[V] = {}, x[V];
+    int count = 0;
+    if (at.active)
+        for (uint64_t s = at.s0 + at.ty; s < at.s1; s += at.deep) {
+            Access<T, V>::load(p.x.at(at.n, s, at.c)).open(x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (count == 0) first[e] = x[e];
+                const W d = x[e] - first[e];
+                sum[e] += d;
+                square[e] += d * d;
+            }
+            ++count;
+        }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const int to = threadIdx.x * V + e;
+        const W shift = count ? sum[e] / (W)count : W(0);
+        means[to] = count ? first[e] + shift : W(0);
+        squares[to] = count ? square[e] - sum[e] * shift : W(0);
+    }
+    __syncthreads();
+    const uint64_t rows = at.s1 - at.s0;
+    for (int i = threadIdx.x; i < at.across * V; i += kNormThreads) {
+        W mean = 0, all = 0;
+        for (int d = 0; d < at.deep; ++d) {
+            const W here = (W)((rows + at.deep - 1 - d) / at.deep);  // rows of the d-th thread
+            mean += here * means[d * at.across * V + i];
+        }
+        mean /= (W)rows;
+        for (int d = 0; d < at.deep; ++d) {
+            const W here = (W)((rows + at.deep - 1 - d) / at.deep), off = means[d * at.across * V + i] - mean;
+            if (here > W(0)) all += squares[d * at.across * V + i] + here * off * off;
+        }
+        const uint64_t channel = at.c - (uint64_t)at.tx * V + i;
+        W *to = p.partial + 2 * ((at.n * p.plan.chunks + at.chunk) * p.channels + channel);
+        to[0] = mean, to[1] = all;
+    }
+}
+
+template <typename W> __device__ __forceinline__ W norm_block_sum(W v, W *scratch) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     __syncthreads();
     if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = v;
@@ -72,114 +637,174 @@ template <typename V> __device__ __forceinline__ V norm_block_sum(V v, V *scratc
     return v;
 }
 
-// One CTA per (n, g): the group's statistics.
-template <typename T> __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const NormParams<T> p) {
+// One CTA per (n, g): the group's statistics from its chunks'.  Also what a call without positions gets.
+template <typename T> __global__ void __launch_bounds__(kNormThreads) norm_join_stats_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
     __shared__ W scratch[kNormThreads / 32];
-    const uint64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups, m = p.positions * p.width;
-    W sum = 0, square = 0;
-    for (uint64_t i = threadIdx.x; i < m; i += kNormThreads)
-        sum += Elem<T>::load(*p.x.at(n, i / p.width, g * p.width + i % p.width));
-    const W mean = m ? norm_block_sum(sum, scratch) / (W)m : W(0);
-    for (uint64_t i = threadIdx.x; i < m; i += kNormThreads) {
-        const W d = Elem<T>::load(*p.x.at(n, i / p.width, g * p.width + i % p.width)) - mean;
-        square += d * d;
+    const uint64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups, parts = p.plan.chunks * p.width;
+    const W inverse = p.positions ? W(1) / ((W)p.positions * (W)p.width) : W(0);
+    W mean = 0, square = 0;
+    if (p.positions) {
+        auto part = [&](uint64_t i, W &count) {
+            const uint64_t chunk = i / p.width;
+            count = (W)(min(p.positions, (chunk + 1) * p.plan.chunk_rows) - chunk * p.plan.chunk_rows);
+            return p.partial + 2 * ((n * p.plan.chunks + chunk) * p.channels + g * p.width + i % p.width);
+        };
+        W count;
+        for (uint64_t i = threadIdx.x; i < parts; i += kNormThreads) {
+            const W *from = part(i, count);
+            mean += count * from[0];
+        }
+        mean = norm_block_sum(mean, scratch) * inverse;
+        for (uint64_t i = threadIdx.x; i < parts; i += kNormThreads) {
+            const W *from = part(i, count);
+            square += from[1] + count * (from[0] - mean) * (from[0] - mean);
+        }
+        square = norm_block_sum(square, scratch);
     }
-    const W var = m ? norm_block_sum(square, scratch) / (W)m : W(0);
     if (threadIdx.x == 0) {
         p.stats_out[2 * blockIdx.x] = mean;
-        // a variance that is not finite has no reciprocal root to scale by: NaN, not 0
-        p.stats_out[2 * blockIdx.x + 1] = isfinite(var) ? W(1) / sqrt(var + p.eps) : W(NAN);
+        p.stats_out[2 * blockIdx.x + 1] = root(square * inverse, p.eps);
     }
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const NormParams<T> p) {
+template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_apply_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
-    const uint64_t total = p.batch * p.positions * p.channels;
-    for (uint64_t i = blockIdx.x * (uint64_t)kNormThreads + threadIdx.x; i < total;
-         i += (uint64_t)gridDim.x * kNormThreads) {
-        const uint64_t c = i % p.channels, s = i / p.channels % p.positions, n = i / p.channels / p.positions;
-        const W *st = p.stats + 2 * (n * p.groups + c / p.width);
-        const W h = (Elem<T>::load(*p.x.at(n, s, c)) - st[0]) * st[1];
-        const W z = h * (p.weight ? p.weight[c] : W(1)) + (p.bias ? p.bias[c] : W(0));
-        const T y = Elem<T>::round(activate<ACT>(z));
-        *p.out.at(n, s, c) = y;
-        if (const unsigned kind = result_kind(Elem<T>::load(y))) record_fault(p.status, i, kind);
+    const Stream<T, V> at(p);
+    if (!at.active) return;
+    W w[V], b[V], mean[V], r[V], x[V];
+    parameters<V>(p.weight, at.c, W(1), w), parameters<V>(p.bias, at.c, W(0), b);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const W *st = p.stats + 2 * (at.n * p.groups + (at.c + e) / p.width);
+        mean[e] = st[0], r[e] = st[1];
+    }
+    for (uint64_t s = at.s0 + at.ty; s < at.s1; s += at.deep) {
+        Access<T, V>::load(p.x.at(at.n, s, at.c)).open(x);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = (x[e] - mean[e]) * r[e] * w[e] + b[e];
+        activate<V>(p.activation, x);
+        put<T, V>(p.out.at(at.n, s, at.c), x, (at.n * p.positions + s) * p.channels + at.c, p.status);
     }
 }
 
-// One CTA per (n, g): c1 and c2.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_sums_kernel(const NormParams<T> p) {
+// Sums of dz h and dz of each channel over a chunk's rows: partial[n][chunk][2][channel].
+template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_sums_kernel(const NormParams<T> p) {
+    using W = WideOf<T>;
+    if (!chain_admits(p.guard)) return;
+    __shared__ W scratch[kNormThreads * V];
+    const Stream<T, V> at(p);
+    W dw[V] = {}, db[V] = {};
+    if (at.active) {
+        W w[V], b[V], mean[V], r[V], x[V], dy[V], h[V], dz[V];
+        parameters<V>(p.weight, at.c, W(1), w), parameters<V>(p.bias, at.c, W(0), b);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const W *st = p.stats + 2 * (at.n * p.groups + (at.c + e) / p.width);
+            mean[e] = st[0], r[e] = st[1];
+        }
+        for (uint64_t s = at.s0 + at.ty; s < at.s1; s += at.deep) {
+            Access<T, V>::load(p.x.at(at.n, s, at.c)).open(x);
+            Access<T, V>::load(p.dy.at(at.n, s, at.c)).open(dy);
+            bend<V>(p.activation, x, dy, mean, r, w, b, h, dz);
+#pragma unroll
+            for (int e = 0; e < V; ++e) dw[e] += dz[e] * h[e], db[e] += dz[e];
+        }
+    }
+    W *to = p.partial + 2 * (at.n * p.plan.chunks + at.chunk) * p.channels + (at.c - (uint64_t)at.tx * V);
+    for (int q = 0; q < 2; ++q) {
+        __syncthreads();
+        if (at.active)
+#pragma unroll
+            for (int e = 0; e < V; ++e) scratch[threadIdx.x * V + e] = q ? db[e] : dw[e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < at.across * V; i += kNormThreads) {
+            W sum = 0;
+            for (int d = 0; d < at.deep; ++d) sum += scratch[d * at.across * V + i];
+            to[q * p.channels + i] = sum;
+        }
+    }
+}
+
+// One CTA per (n, g): c1 and c2 from its channels' sums.
+template <typename T> __global__ void __launch_bounds__(kNormThreads) norm_join_sums_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
     __shared__ W scratch[kNormThreads / 32];
-    const uint64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups, m = p.positions * p.width;
-    const W mean = p.stats[2 * blockIdx.x], r = p.stats[2 * blockIdx.x + 1];
+    const uint64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
     W c1 = 0, c2 = 0;
-    for (uint64_t i = threadIdx.x; i < m; i += kNormThreads) {
-        const uint64_t s = i / p.width, c = g * p.width + i % p.width;
-        const W w = p.weight ? p.weight[c] : W(1), b = p.bias ? p.bias[c] : W(0);
-        const W x = Elem<T>::load(*p.x.at(n, s, c)), h = (x - mean) * r;
-        const W k = Elem<T>::load(*p.dy.at(n, s, c)) * slope_at<ACT>(x, mean, r, h, w, b) * w;
-        c1 += k;
-        c2 += k * h;
+    for (uint64_t i = threadIdx.x; i < p.plan.chunks * p.width; i += kNormThreads) {
+        const uint64_t c = g * p.width + i % p.width;
+        const W *from = p.partial + 2 * (n * p.plan.chunks + i / p.width) * p.channels + c;
+        const W w = p.weight ? p.weight[c] : W(1);
+        c2 += w * from[0];
+        c1 += w * from[p.channels];
     }
     c1 = norm_block_sum(c1, scratch);
     c2 = norm_block_sum(c2, scratch);
-    if (threadIdx.x == 0) p.sums[2 * blockIdx.x] = c1 / (W)m, p.sums[2 * blockIdx.x + 1] = c2 / (W)m;
+    const W inverse = W(1) / ((W)p.positions * (W)p.width);
+    if (threadIdx.x == 0) p.sums[2 * blockIdx.x] = c1 * inverse, p.sums[2 * blockIdx.x + 1] = c2 * inverse;
 }
 
-// One CTA per channel: the parameters' gradients.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_parameters_kernel(const NormParams<T> p) {
+template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_gradient_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
-    __shared__ W scratch[kNormThreads / 32];
-    const uint64_t c = blockIdx.x, rows = p.batch * p.positions;
-    const W w = p.weight ? p.weight[c] : W(1), b = p.bias ? p.bias[c] : W(0);
-    W dw = 0, db = 0;
-    for (uint64_t i = threadIdx.x; i < rows; i += kNormThreads) {
-        const uint64_t n = i / p.positions, s = i % p.positions;
-        const W *st = p.stats + 2 * (n * p.groups + c / p.width);
-        const W x = Elem<T>::load(*p.x.at(n, s, c)), h = (x - st[0]) * st[1];
-        const W dz = Elem<T>::load(*p.dy.at(n, s, c)) * slope_at<ACT>(x, st[0], st[1], h, w, b);
-        dw += dz * h;
-        db += dz;
+    const Stream<T, V> at(p);
+    if (!at.active) return;
+    W w[V], b[V], mean[V], r[V], c1[V], c2[V], x[V], dy[V], h[V], dz[V];
+    parameters<V>(p.weight, at.c, W(1), w), parameters<V>(p.bias, at.c, W(0), b);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const uint64_t st = 2 * (at.n * p.groups + (at.c + e) / p.width);
+        mean[e] = p.stats[st], r[e] = p.stats[st + 1], c1[e] = p.sums[st], c2[e] = p.sums[st + 1];
     }
-    dw = norm_block_sum(dw, scratch);
-    db = norm_block_sum(db, scratch);
-    if (threadIdx.x != 0) return;
-    const uint64_t first = rows * p.channels + c;
+    for (uint64_t s = at.s0 + at.ty; s < at.s1; s += at.deep) {
+        Access<T, V>::load(p.x.at(at.n, s, at.c)).open(x);
+        Access<T, V>::load(p.dy.at(at.n, s, at.c)).open(dy);
+        bend<V>(p.activation, x, dy, mean, r, w, b, h, dz);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = r[e] * (dz[e] * w[e] - c1[e] - h[e] * c2[e]);
+        put<T, V>(p.out.at(at.n, s, at.c), x, (at.n * p.positions + s) * p.channels + at.c, p.status);
+    }
+}
+
+// ---- the parameters' gradients from partial sums [rows][2][groups][split][width], in a fixed order:
+// 32 channels by 32 threads each per CTA
+template <typename T> __global__ void __launch_bounds__(1024) norm_parameters_kernel(const NormParams<T> p) {
+    using W = WideOf<T>;
+    if (!chain_admits(p.guard)) return;
+    __shared__ W scratch[2][32][33];
+    const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x % 32;
+    const uint64_t split = p.plan.partial_split, rows = p.batch * p.positions ? p.plan.partial_rows : 0;
+    W dw = 0, db = 0;
+    if (c < p.channels) {
+        const W *from = p.partial + c / p.width * split * p.width + c % p.width;
+        const uint64_t whole = p.channels * split;
+#pragma unroll 4
+        for (uint64_t i = threadIdx.x / 32; i < rows * split; i += 32) {
+            const W *at = from + i / split * 2 * whole + i % split * p.width;
+            dw += at[0];
+            db += at[whole];
+        }
+    }
+    scratch[0][threadIdx.x / 32][threadIdx.x % 32] = dw;
+    scratch[1][threadIdx.x / 32][threadIdx.x % 32] = db;
+    __syncthreads();
+    const int which = threadIdx.x / 32, lane = threadIdx.x % 32;  // a warp per channel
+    dw = scratch[0][lane][which], db = scratch[1][lane][which];
+    for (int o = 16; o; o >>= 1) dw += __shfl_xor_sync(~0u, dw, o), db += __shfl_xor_sync(~0u, db, o);
+    const uint64_t channel = (uint64_t)blockIdx.x * 32 + which;
+    if (lane != 0 || channel >= p.channels) return;
+    const uint64_t first = p.batch * p.positions * p.channels + channel;
     if (p.dweight) {
-        p.dweight[c] = dw;
+        p.dweight[channel] = dw;
         if (const unsigned kind = result_kind(dw)) record_fault(p.status, first, kind);
     }
     if (p.dbias) {
-        p.dbias[c] = db;
+        p.dbias[channel] = db;
         if (const unsigned kind = result_kind(db)) record_fault(p.status, first + p.channels, kind);
-    }
-}
-
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_gradient_kernel(const NormParams<T> p) {
-    using W = WideOf<T>;
-    if (!chain_admits(p.guard)) return;
-    const uint64_t total = p.batch * p.positions * p.channels;
-    for (uint64_t i = blockIdx.x * (uint64_t)kNormThreads + threadIdx.x; i < total;
-         i += (uint64_t)gridDim.x * kNormThreads) {
-        const uint64_t c = i % p.channels, s = i / p.channels % p.positions, n = i / p.channels / p.positions;
-        const uint64_t at = 2 * (n * p.groups + c / p.width);
-        const W mean = p.stats[at], r = p.stats[at + 1];
-        const W w = p.weight ? p.weight[c] : W(1), b = p.bias ? p.bias[c] : W(0);
-        const W x = Elem<T>::load(*p.x.at(n, s, c)), h = (x - mean) * r;
-        const W k = Elem<T>::load(*p.dy.at(n, s, c)) * slope_at<ACT>(x, mean, r, h, w, b) * w;
-        const T dx = Elem<T>::round(r * (k - p.sums[at] - h * p.sums[at + 1]));
-        *p.out.at(n, s, c) = dx;
-        if (const unsigned kind = result_kind(Elem<T>::load(dx))) record_fault(p.status, i, kind);
     }
 }
 
@@ -212,44 +837,147 @@ bool shape_fits(uint64_t batch, uint64_t positions, uint64_t channels, uint64_t 
            pcu_host::multiply_fits(positions * channels, batch, kMost);
 }
 
-// 0 for what the calls refuse
-size_t workspace_size(int dtype, uint64_t batch, uint64_t positions, uint64_t channels, uint64_t groups, bool backward) {
-    if (!pcu_host::element_bytes(dtype) || groups == 0 || channels % groups != 0 ||
-        !shape_fits(batch, positions, channels, groups))
-        return 0;
-    if (!backward) return 0;
-    return (size_t)(2 * batch * groups * (dtype == PCU_B200_F64 ? 8 : 4));
+constexpr size_t kSlabMost = 200 * 1024;  // shared memory of a CTA for a slab
+
+// `vector`: elements per access, 16 bytes' worth or 1.  No extent is 0.
+NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, uint64_t channels, uint64_t groups,
+                   bool backward) {
+    NormPlan p{};
+    const uint64_t width = channels / groups, bytes = pcu_host::element_bytes(dtype), wide = dtype == PCU_B200_F64 ? 8 : 4;
+    const uint64_t sms = (uint64_t)pcu_host::sm_count();
+    p.vector = vector;
+    p.partial_split = 1;
+    // Warp form: 16 elements of a lane are in registers (and as many of dy, and four parameters' worth), so
+    // a group has at most 512 of them.
+    if (width % vector == 0 && positions <= 512 && positions * (width / vector) * vector <= 512) {
+        p.form = NormPlan::kWarp;
+        p.items = (unsigned)(positions * (width / vector));
+        p.lanes = 1;
+        while (p.lanes < 32 && (unsigned)p.lanes < p.items) p.lanes *= 2;
+        p.per_lane = (int)((p.items + p.lanes - 1) / p.lanes);
+        const uint64_t per = 32 / p.lanes, sets = (groups + per - 1) / per;
+        // Each warp takes several of the batch where there are enough: 32 warps per SM walk.
+        p.slices = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(batch, (sms * 32 + sets - 1) / sets));
+        p.partial_rows = p.slices;
+        p.partial_split = positions;
+        p.workspace = backward ? 2 * p.partial_rows * channels * positions : 0;
+        return p;
+    }
+    // Slab form: blocks of whole groups whose rows are at least 128 bytes and whole accesses.  The smallest
+    // cluster whose slabs are at most 64 KB (three CTAs per SM overlap loading, sums and stores), or 200 KB in
+    // a cluster of 8; more CTAs, down to 16 KB each, when they do not fill the SMs twice.
+    const uint64_t tensors = backward ? 2 : 1;
+    const uint64_t step = (uint64_t)vector / std::gcd(width, (uint64_t)vector);
+    auto try_slab = [&](uint64_t block) {
+        block = std::min(block, groups);
+        const uint64_t across = block * width / vector;
+        if (across > 512 || block * width % vector != 0) return false;
+        const uint64_t row = block * width * bytes * tensors;
+        uint64_t ranks = 1;
+        while (ranks < 8 && (positions + ranks - 1) / ranks * row > 65536) ranks *= 2;
+        const uint64_t blocks = (groups + block - 1) / block;
+        while (ranks < 8 && batch * blocks * ranks < 2 * sms && (positions + ranks - 1) / ranks * row > 16384) ranks *= 2;
+        const uint64_t rows = (positions + ranks - 1) / ranks;
+        const uint64_t threads = across > 256 ? 512 : 256;
+        const uint64_t extra = threads * vector * wide + 4 * block * wide + 64;
+        if (rows > 0x7fffffffull || rows * row + extra + 32 > kSlabMost || batch * blocks * ranks > 0x7fffffffull) return false;
+        p.form = NormPlan::kSlab;
+        p.block_groups = (unsigned)block;
+        p.blocks = (unsigned)blocks;
+        p.ranks = (unsigned)ranks;
+        p.threads = (unsigned)threads;
+        p.slab_rows = (unsigned)rows;
+        p.shared = tensors * ((rows * block * width * bytes + 15) / 16 * 16) + extra;
+        p.partial_rows = batch * ranks;
+        p.workspace = backward ? 2 * p.partial_rows * channels : 0;
+        return true;
+    };
+    const uint64_t need = (128 + width * bytes - 1) / (width * bytes);
+    const uint64_t block = (need + step - 1) / step * step;
+    if (try_slab(block) || (block > step && try_slab(step))) return p;
+    // Stream form: column tiles of a CTA's threads, row chunks to fill the SMs four times.
+    p.form = NormPlan::kStream;
+    const uint64_t across = channels / vector;
+    p.tile = (unsigned)std::min<uint64_t>(across, kNormThreads);
+    p.tiles = (unsigned)((across + p.tile - 1) / p.tile);
+    const uint64_t deep = kNormThreads / p.tile;
+    uint64_t chunks = std::max<uint64_t>(1, std::min<uint64_t>(4 * sms / std::max<uint64_t>(1, batch * p.tiles),
+                                                               (positions + 4 * deep - 1) / (4 * deep)));
+    p.chunk_rows = (positions + chunks - 1) / chunks;
+    p.chunks = (unsigned)((positions + p.chunk_rows - 1) / p.chunk_rows);
+    p.partial_rows = batch * p.chunks;
+    p.workspace = 2 * p.partial_rows * channels + (backward ? 2 * batch * groups : 0);
+    return p;
 }
 
-template <typename T, int ACT> int run_norm(const NormCall &c, NormParams<T> p, cudaStream_t stream) {
-    const uint64_t total = c.batch * c.positions * c.channels;
-    const uint64_t want = (total + kNormThreads - 1) / kNormThreads, cap = (uint64_t)pcu_host::sm_count() * 8;
-    const unsigned blocks = (unsigned)(want < cap ? (want ? want : 1) : cap);
-    const unsigned groups = (unsigned)(c.batch * c.groups);
-    int rc = PCU_B200_OK;
-    if (!c.backward) {
-        norm_stats_kernel<T><<<groups, kNormThreads, 0, stream>>>(p);
-        if ((rc = pcu_host::launch_status())) return rc;
-        p.guard = chain_follow(p.guard);
-        norm_apply_kernel<T, ACT><<<blocks, kNormThreads, 0, stream>>>(p);
-        return pcu_host::launch_status();
-    }
-    if (total) {
-        norm_sums_kernel<T, ACT><<<groups, kNormThreads, 0, stream>>>(p);
-        if ((rc = pcu_host::launch_status())) return rc;
-        p.guard = chain_follow(p.guard);
-    }
-    if (p.dweight || p.dbias) {  // before the gradient, which may overwrite input or upstream
-        norm_parameters_kernel<T, ACT><<<(unsigned)c.channels, kNormThreads, 0, stream>>>(p);
-        if ((rc = pcu_host::launch_status())) return rc;
-        p.guard = chain_follow(p.guard);
-    }
-    if (total) norm_gradient_kernel<T, ACT><<<blocks, kNormThreads, 0, stream>>>(p);
+// 0 for what the calls refuse.  Enough for either access width.
+size_t workspace_size(int dtype, uint64_t batch, uint64_t positions, uint64_t channels, uint64_t groups, bool backward) {
+    const size_t bytes = pcu_host::element_bytes(dtype);
+    if (!bytes || groups == 0 || channels % groups != 0 || !shape_fits(batch, positions, channels, groups)) return 0;
+    if (batch == 0 || positions == 0 || channels == 0) return 0;
+    uint64_t need = plan_norm(dtype, 1, batch, positions, channels, groups, backward).workspace;
+    const int vector = (int)(16 / bytes);
+    if (channels % vector == 0)
+        need = std::max(need, plan_norm(dtype, vector, batch, positions, channels, groups, backward).workspace);
+    return need * (dtype == PCU_B200_F64 ? 8 : 4);
+}
+
+#define PCU_LAUNCHED(call)               \
+    do {                                 \
+        call;                            \
+        rc = pcu_host::launch_status();  \
+        if (rc) return rc;               \
+        p.guard = chain_follow(p.guard); \
+    } while (0)
+
+template <typename T, int V, int K> int run_warp(NormParams<T> p, bool backward, cudaStream_t stream) {
+    constexpr int U = std::max(1, 16 / (V * K)), UB = std::max(1, 8 / (V * K));
+    const uint64_t per = 32 / p.plan.lanes, warps = (p.groups + per - 1) / per * p.plan.slices;
+    const unsigned blocks = (unsigned)((warps + kNormThreads / 32 - 1) / (kNormThreads / 32));
+    if (backward) norm_warp_backward_kernel<T, V, K, UB><<<blocks, kNormThreads, 0, stream>>>(p);
+    else norm_warp_kernel<T, V, K, U><<<blocks, kNormThreads, 0, stream>>>(p);
     return pcu_host::launch_status();
+}
+
+template <typename T, int V> int run_norm(NormParams<T> p, bool backward, cudaStream_t stream) {
+    int rc = PCU_B200_OK;
+    const NormPlan &plan = p.plan;
+    if (plan.form == NormPlan::kWarp) {
+        // accesses per lane: 1, or what 16 elements make
+        if (plan.per_lane == 1) rc = run_warp<T, V, 1>(p, backward, stream);
+        else if (V * 4 <= 16 && plan.per_lane <= 4) rc = run_warp<T, V, std::min(4, 16 / V)>(p, backward, stream);
+        else rc = run_warp<T, V, 16 / V>(p, backward, stream);
+        if (rc) return rc;
+        p.guard = chain_follow(p.guard);
+    } else if (plan.form == NormPlan::kSlab) {
+        const unsigned grid = (unsigned)(p.batch * plan.blocks * plan.ranks);
+        if (backward) {
+            if ((rc = pcu_host::allow_shared<norm_slab_backward_kernel<T, V>>((int)kSlabMost))) return rc;
+            rc = pcu_host::launch_cluster(norm_slab_backward_kernel<T, V>, grid, plan.threads, plan.shared, plan.ranks, stream, p);
+        } else {
+            if ((rc = pcu_host::allow_shared<norm_slab_kernel<T, V>>((int)kSlabMost))) return rc;
+            rc = pcu_host::launch_cluster(norm_slab_kernel<T, V>, grid, plan.threads, plan.shared, plan.ranks, stream, p);
+        }
+        if (rc) return rc;
+        p.guard = chain_follow(p.guard);
+    } else {
+        const unsigned grid = (unsigned)(p.batch * plan.tiles * plan.chunks), groups = (unsigned)(p.batch * p.groups);
+        if (backward) {
+            PCU_LAUNCHED((norm_stream_sums_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
+            PCU_LAUNCHED((norm_join_sums_kernel<T><<<groups, kNormThreads, 0, stream>>>(p)));
+            PCU_LAUNCHED((norm_stream_gradient_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
+        } else {
+            PCU_LAUNCHED((norm_stream_stats_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
+            PCU_LAUNCHED((norm_join_stats_kernel<T><<<groups, kNormThreads, 0, stream>>>(p)));
+            PCU_LAUNCHED((norm_stream_apply_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
+        }
+    }
+    return PCU_B200_OK;
 }
 
 template <typename T> int typed_norm(const NormCall &c, const ChainGuard &guard) {
     using W = WideOf<T>;
+    constexpr int V = 16 / sizeof(T);
     NormParams<T> p{};
     p.x = {(const T *)c.input, c.input_batch_stride, c.input_stride};
     p.dy = {(const T *)c.upstream, c.upstream_batch_stride, c.upstream_stride};
@@ -258,7 +986,6 @@ template <typename T> int typed_norm(const NormCall &c, const ChainGuard &guard)
     p.bias = (const W *)c.bias;
     p.stats_out = (W *)c.stats_out;
     p.stats = c.backward ? (const W *)c.stats_in : (const W *)c.stats_out;
-    p.sums = (W *)c.workspace;
     p.dweight = (W *)c.dweight;
     p.dbias = (W *)c.dbias;
     p.batch = c.batch;
@@ -267,15 +994,40 @@ template <typename T> int typed_norm(const NormCall &c, const ChainGuard &guard)
     p.groups = c.groups;
     p.width = c.channels / c.groups;
     p.eps = (W)pcu_host::rate_f32(c.eps_bits);
+    p.activation = c.activation;
     p.status = reinterpret_cast<unsigned long long *>(c.status);
     p.guard = guard;
     cudaStream_t stream = pcu_host::as_stream(c.stream);
-    switch (c.activation) {
-    case PCU_B200_ACTIVATION_RELU: return run_norm<T, PCU_B200_ACTIVATION_RELU>(c, p, stream);
-    case PCU_B200_ACTIVATION_SILU: return run_norm<T, PCU_B200_ACTIVATION_SILU>(c, p, stream);
-    case PCU_B200_ACTIVATION_GELU: return run_norm<T, PCU_B200_ACTIVATION_GELU>(c, p, stream);
-    default: return run_norm<T, PCU_B200_ACTIVATION_NONE>(c, p, stream);
+    int rc = PCU_B200_OK;
+    if (c.batch && c.positions) {
+        // 16-byte accesses where every row of every tensor starts on 16 bytes and ends with whole ones
+        auto whole = [&](const void *base, uint64_t batch_stride, uint64_t stride) {
+            return pcu_host::aligned(base, 16) && (c.batch == 1 || batch_stride % V == 0) &&
+                   (c.positions == 1 || stride % V == 0);
+        };
+        const bool wide = c.channels % V == 0 && whole(c.input, c.input_batch_stride, c.input_stride) &&
+                          whole(c.out, c.out_batch_stride, c.out_stride) &&
+                          (!c.backward || whole(c.upstream, c.upstream_batch_stride, c.upstream_stride));
+        p.plan = plan_norm(c.dtype, wide ? V : 1, c.batch, c.positions, c.channels, c.groups, c.backward);
+        p.partial = (W *)c.workspace;
+        p.sums = p.partial + 2 * p.plan.partial_rows * p.channels;  // stream form
+        // partial sums are for the stream form's groups, or for gradients that are wanted
+        if (c.backward && p.plan.form != NormPlan::kStream && !c.dweight && !c.dbias) p.partial = nullptr;
+        if (p.plan.form == NormPlan::kStream &&
+            !pcu_host::multiply_fits(c.batch * p.plan.tiles, p.plan.chunks, 0x7fffffffull))
+            return PCU_B200_ERROR_SIZE_OVERFLOW;
+        rc = wide ? run_norm<T, V>(p, c.backward, stream) : run_norm<T, 1>(p, c.backward, stream);
+        if (rc) return rc;
+        p.guard = chain_follow(p.guard);
+    } else if (!c.backward) {
+        norm_join_stats_kernel<T><<<(unsigned)(c.batch * c.groups), kNormThreads, 0, stream>>>(p);
+        return pcu_host::launch_status();
     }
+    if (c.backward && (c.dweight || c.dbias)) {
+        norm_parameters_kernel<T><<<(unsigned)((c.channels + 31) / 32), 1024, 0, stream>>>(p);
+        rc = pcu_host::launch_status();
+    }
+    return rc;
 }
 
 // Rows of `channels` elements: a batch's rows lie within its stride, so no two rows overlap.

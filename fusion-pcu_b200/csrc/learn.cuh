@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "pcu_b200_learn.h"
@@ -93,6 +94,19 @@ template <> __device__ __forceinline__ float largest<__half>(uint4 raw, const fl
     const __half2 *w = reinterpret_cast<const __half2 *>(&raw);
     const __half2 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
     return fmaxf(__low2float(m), __high2float(m));
+}
+
+// Not 0 where an element of the 16 bytes is an infinity or a NaN: a full exponent field, the largest,
+// carries into the sign's place when one is added to it.
+template <typename T> __device__ __forceinline__ unsigned not_finite(uint4 raw) {
+    constexpr unsigned field = sizeof(T) == 2 ? (std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u)
+                               : sizeof(T) == 4 ? 0x7f800000u : 0x7ff00000u;
+    constexpr unsigned one = sizeof(T) == 2 ? (std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u)
+                             : sizeof(T) == 4 ? 0x00800000u : 0x00100000u;
+    constexpr unsigned sign = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+    unsigned bad = ((raw.y & field) + one) | ((raw.w & field) + one);
+    if (sizeof(T) < 8) bad |= ((raw.x & field) + one) | ((raw.z & field) + one);
+    return bad & sign;
 }
 
 // 2^x.  binary32: the hardware's approximation (2 ulp), results below 2^-126 flushed to zero --
