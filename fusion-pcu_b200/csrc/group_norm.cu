@@ -22,6 +22,11 @@
 namespace pcu {
 
 constexpr int kNormThreads = 256;
+// Warp form: CTAs per SM that walk over the batch at once, by what a lane keeps in registers (elements of
+// the wide type, four bytes each counted).
+__host__ __device__ constexpr int warp_form_ctas(int elements, int wide_bytes) {
+    return elements * wide_bytes > 32 ? (elements * wide_bytes > 64 ? 1 : 2) : 3;
+}
 
 // A channels-last tensor: element (n, s, c) at n * batch + s * row + c.
 template <typename T> struct Maps {
@@ -38,7 +43,7 @@ struct NormPlan {
     unsigned items, slices;    // accesses per group; parts of the batch
     unsigned block_groups, blocks, ranks, threads;  // slab form: groups per cluster, of one n; CTAs
     unsigned slab_rows;
-    size_t shared;
+    size_t slab_bytes, shared;  // of one tensor's slab; of the CTA
     unsigned tiles, tile, chunks;  // stream form: column tiles of `tile` accesses, row chunks
     uint64_t chunk_rows;
     uint64_t partial_rows, partial_split;  // parameters' gradients: partial sums [rows][2][groups][split][width]
@@ -65,8 +70,11 @@ template <typename T> struct NormParams {
 
 // ---- activations, over the V elements of one access (the choice is the same for a whole launch)
 
+// binary32: the hardware's exponential and reciprocal (each within 2 ulp)
 __device__ __forceinline__ float logistic(float z) {
-    return __fdividef(1.0f, 1.0f + fast_exp2(z * -1.4426950408889634f));
+    float q;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.0f + fast_exp2(z * -1.4426950408889634f)));
+    return q;
 }
 __device__ __forceinline__ double logistic(double z) { return 1.0 / (1.0 + exp(-z)); }
 __device__ __forceinline__ float normal_density(float z) {
@@ -133,20 +141,30 @@ template <typename T> struct Access<T, 1> {
     __device__ __forceinline__ void open(W (&v)[1]) const { v[0] = Elem<T>::load(raw); }
 };
 
-// Stores V elements; what is not finite is recorded with its event.
-template <typename T, int V>
-__device__ __forceinline__ void put(T *to, const WideOf<T> (&v)[V], uint64_t event, unsigned long long *status) {
+// Stores V elements; what is not finite is recorded, the first of them being event().
+template <typename T, int V, typename E>
+__device__ __forceinline__ void put(T *to, const WideOf<T> (&v)[V], unsigned long long *status, E event) {
+    unsigned bad;
     if constexpr (V == 1) {
         const T y = Elem<T>::round(v[0]);
         *to = y;
-        if (const unsigned kind = result_kind(Elem<T>::load(y))) record_fault(status, event, kind);
+        bad = result_kind(Elem<T>::load(y));
     } else {
         const uint4 y = pack<T>(v);
         __stcs(reinterpret_cast<uint4 *>(to), y);
-        if (not_finite<T>(y))
-            for (int e = 0; e < V; ++e)
-                if (const unsigned kind = result_kind(Elem<T>::load(reinterpret_cast<const T *>(&y)[e])))
-                    record_fault(status, event + e, kind);
+        if constexpr (sizeof(T) >= 4) {  // 0 times an infinity or NaN is NaN, and stays
+            WideOf<T> sum = 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum = fma(v[e], WideOf<T>(0), sum);
+            bad = sum != WideOf<T>(0);
+        } else {
+            bad = not_finite<T>(y);  // rounding can make an infinity
+        }
+    }
+    if (bad) {
+        const uint64_t first = event();
+        for (int e = 0; e < V; ++e)
+            if (const unsigned kind = result_kind(Elem<T>::load(Elem<T>::round(v[e])))) record_fault(status, first + e, kind);
     }
 }
 
@@ -155,10 +173,10 @@ template <int V, typename W> __device__ __forceinline__ void parameters(const W 
     for (int e = 0; e < V; ++e) v[e] = p ? p[c + e] : none;
 }
 
-template <typename W> __device__ __forceinline__ W root(W var, W eps) {
-    // a variance that is not finite has no reciprocal root to scale by: NaN, not 0
-    return isfinite(var) ? W(1) / sqrt(var + eps) : W(NAN);
-}
+// 1 / sqrt(var + eps), within 2 ulp in binary32.  A variance that is not finite has no reciprocal root to
+// scale by: NaN, not 0.
+__device__ __forceinline__ float root(float var, float eps) { return isfinite(var) ? rsqrtf(var + eps) : NAN; }
+__device__ __forceinline__ double root(double var, double eps) { return isfinite(var) ? 1.0 / sqrt(var + eps) : NAN; }
 
 // ---- warp form
 //
@@ -167,8 +185,8 @@ template <typename W> __device__ __forceinline__ W root(W var, W eps) {
 // registers, and their gradients too: each warp ends with one partial sum per element of its groups.
 template <typename T, int V, int K> struct WarpGroup {
     using W = WideOf<T>;
-    int sub, slice;
-    uint64_t g;
+    int sub;
+    uint64_t slice, g;
     bool active, there[K];
     uint64_t row[K], channel[K];
     W w[K][V], b[K][V];
@@ -180,7 +198,7 @@ template <typename T, int V, int K> struct WarpGroup {
         const uint64_t sets = (p.groups + per - 1) / per;
         if (warp >= sets * plan.slices) return false;
         sub = lane % plan.lanes;
-        slice = (int)(warp / sets);
+        slice = warp / sets;
         g = warp % sets * per + lane / plan.lanes;
         active = g < p.groups;
         const unsigned across = (unsigned)(p.width / V);
@@ -195,6 +213,13 @@ template <typename T, int V, int K> struct WarpGroup {
         }
         return true;
     }
+    // where access k of sample n begins; absent ones point at the sample's first element
+    template <typename M> __device__ __forceinline__ auto first(const M &maps, int k, uint64_t n) const {
+        return maps.at(n, row[k], channel[k]);
+    }
+    __device__ __forceinline__ uint64_t event(const NormParams<T> &p, int k, uint64_t n) const {
+        return (n * p.positions + row[k]) * p.channels + channel[k];
+    }
 };
 
 template <int U, typename W> __device__ __forceinline__ void lanes_sum(W (&v)[U], int lanes) {
@@ -204,19 +229,26 @@ template <int U, typename W> __device__ __forceinline__ void lanes_sum(W (&v)[U]
 }
 
 template <typename T, int V, int K, int U>
-__global__ void __launch_bounds__(kNormThreads) norm_warp_kernel(const NormParams<T> p) {
+__global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K, sizeof(WideOf<T>))) norm_warp_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
     WarpGroup<T, V, K> at;
     if (!at.place(p)) return;
     const W inverse = W(1) / (W)(p.positions * p.width);
-    for (uint64_t n = (uint64_t)at.slice * U; n < p.batch; n += (uint64_t)p.plan.slices * U) {
+    const uint64_t stride = (uint64_t)p.plan.slices * U;
+    const T *from[K];
+    T *to[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) from[k] = at.first(p.x, k, at.slice * U), to[k] = at.first(p.out, k, at.slice * U);
+    W *stats = p.stats_out + 2 * (at.slice * U * p.groups + at.g);
+    for (uint64_t n = at.slice * U; n < p.batch; n += stride) {
+        const int here = (int)min((uint64_t)U, p.batch - n);
         W x[U][K][V], mean[U] = {}, square[U] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (at.there[k] && n + u < p.batch) Access<T, V>::load(p.x.at(n + u, at.row[k], at.channel[k])).open(x[u][k]);
+                if (at.there[k] && u < here) Access<T, V>::load(from[k] + u * p.x.batch).open(x[u][k]);
                 else
 #pragma unroll
                     for (int e = 0; e < V; ++e) x[u][k][e] = W(0);
@@ -233,67 +265,78 @@ __global__ void __launch_bounds__(kNormThreads) norm_warp_kernel(const NormParam
             mean[u] *= inverse;
 #pragma unroll
             for (int k = 0; k < K; ++k)
+                if (at.there[k])
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    x[u][k][e] -= mean[u];
-                    if (at.there[k]) square[u] += x[u][k][e] * x[u][k][e];
-                }
+                    for (int e = 0; e < V; ++e) {
+                        x[u][k][e] -= mean[u];
+                        square[u] += x[u][k][e] * x[u][k][e];
+                    }
         }
         lanes_sum(square, p.plan.lanes);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (n + u >= p.batch) break;
+            if (u >= here) break;
             const W r = root(square[u] * inverse, p.eps);
-            if (at.sub == 0 && at.active) {
-                p.stats_out[2 * ((n + u) * p.groups + at.g)] = mean[u];
-                p.stats_out[2 * ((n + u) * p.groups + at.g) + 1] = r;
-            }
+            if (at.sub == 0 && at.active) stats[2 * u * p.groups] = mean[u], stats[2 * u * p.groups + 1] = r;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (!at.there[k]) continue;
 #pragma unroll
                 for (int e = 0; e < V; ++e) x[u][k][e] = x[u][k][e] * r * at.w[k][e] + at.b[k][e];
                 activate<V>(p.activation, x[u][k]);
-                put<T, V>(p.out.at(n + u, at.row[k], at.channel[k]), x[u][k],
-                          ((n + u) * p.positions + at.row[k]) * p.channels + at.channel[k], p.status);
+                put<T, V>(to[k] + u * p.out.batch, x[u][k], p.status, [&] { return at.event(p, k, n + u); });
             }
         }
+#pragma unroll
+        for (int k = 0; k < K; ++k) from[k] += stride * p.x.batch, to[k] += stride * p.out.batch;
+        stats += 2 * stride * p.groups;
     }
 }
 
 template <typename T, int V, int K, int U>
-__global__ void __launch_bounds__(kNormThreads) norm_warp_backward_kernel(const NormParams<T> p) {
+__global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K, sizeof(WideOf<T>))) norm_warp_backward_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
     WarpGroup<T, V, K> at;
     if (!at.place(p)) return;
     const W inverse = W(1) / (W)(p.positions * p.width);
-    W dw[K][V] = {}, db[K][V] = {};
-    for (uint64_t n = (uint64_t)at.slice * U; n < p.batch; n += (uint64_t)p.plan.slices * U) {
-        W x[U][K][V], dy[U][K][V], c1[U] = {}, c2[U] = {}, r[U];
+    const uint64_t stride = (uint64_t)p.plan.slices * U;
+    const T *from[K], *up[K];
+    T *to[K];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+    for (int k = 0; k < K; ++k) {
+        from[k] = at.first(p.x, k, at.slice * U);
+        up[k] = at.first(p.dy, k, at.slice * U);
+        to[k] = at.first(p.out, k, at.slice * U);
+    }
+    const W *stats = p.stats + 2 * (at.slice * U * p.groups + (at.active ? at.g : 0));
+    W dw[K][V] = {}, db[K][V] = {};
+    for (uint64_t n = at.slice * U; n < p.batch; n += stride) {
+        const int here = (int)min((uint64_t)U, p.batch - n);
+        W x[U][K][V], dy[U][K][V], c1[U] = {}, c2[U] = {}, mean[U], r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (at.there[k] && n + u < p.batch) {
-                    Access<T, V>::load(p.x.at(n + u, at.row[k], at.channel[k])).open(x[u][k]);
-                    Access<T, V>::load(p.dy.at(n + u, at.row[k], at.channel[k])).open(dy[u][k]);
+                if (at.there[k] && u < here) {
+                    Access<T, V>::load(from[k] + u * p.x.batch).open(x[u][k]);
+                    Access<T, V>::load(up[k] + u * p.dy.batch).open(dy[u][k]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < V; ++e) x[u][k][e] = dy[u][k][e] = W(0);
                 }
             }
+            mean[u] = u < here ? stats[2 * u * p.groups] : W(0);
+            r[u] = u < here ? stats[2 * u * p.groups + 1] : W(0);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool live = at.active && n + u < p.batch;
-            const W mean = live ? p.stats[2 * ((n + u) * p.groups + at.g)] : W(0);
-            r[u] = live ? p.stats[2 * ((n + u) * p.groups + at.g) + 1] : W(0);
             W means[V], rs[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) means[e] = mean, rs[e] = r[u];
+            for (int e = 0; e < V; ++e) means[e] = mean[u], rs[e] = r[u];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (!at.there[k] || !live) continue;
+                if (!at.there[k] || u >= here) continue;
                 W h[V], dz[V];
                 bend<V>(p.activation, x[u][k], dy[u][k], means, rs, at.w[k], at.b[k], h, dz);
 #pragma unroll
@@ -311,26 +354,28 @@ __global__ void __launch_bounds__(kNormThreads) norm_warp_backward_kernel(const 
         lanes_sum(c2, p.plan.lanes);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (n + u >= p.batch) break;
+            if (u >= here) break;
+            c1[u] *= inverse, c2[u] *= inverse;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (!at.there[k]) continue;
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    x[u][k][e] = r[u] * (dy[u][k][e] - c1[u] * inverse - x[u][k][e] * (c2[u] * inverse));
-                put<T, V>(p.out.at(n + u, at.row[k], at.channel[k]), x[u][k],
-                          ((n + u) * p.positions + at.row[k]) * p.channels + at.channel[k], p.status);
+                for (int e = 0; e < V; ++e) x[u][k][e] = r[u] * (dy[u][k][e] - c1[u] - x[u][k][e] * c2[u]);
+                put<T, V>(to[k] + u * p.out.batch, x[u][k], p.status, [&] { return at.event(p, k, n + u); });
             }
         }
+#pragma unroll
+        for (int k = 0; k < K; ++k) from[k] += stride * p.x.batch, up[k] += stride * p.dy.batch, to[k] += stride * p.out.batch;
+        stats += 2 * stride * p.groups;
     }
     if (!p.partial) return;
     const uint64_t whole = p.groups * p.plan.items * V;
 #pragma unroll
     for (int k = 0; k < K; ++k)
         if (at.there[k]) {
-            const uint64_t to = 2 * at.slice * whole + (at.g * p.plan.items + at.sub + k * p.plan.lanes) * V;
+            W *sums = p.partial + 2 * at.slice * whole + (at.g * p.plan.items + at.sub + k * p.plan.lanes) * V;
 #pragma unroll
-            for (int e = 0; e < V; ++e) p.partial[to + e] = dw[k][e], p.partial[to + whole + e] = db[k][e];
+            for (int e = 0; e < V; ++e) sums[e] = dw[k][e], sums[whole + e] = db[k][e];
         }
 }
 
@@ -339,152 +384,174 @@ __global__ void __launch_bounds__(kNormThreads) norm_warp_backward_kernel(const 
 // A thread keeps one access of columns and takes every `deep`-th row, so a channel's parameters,
 // statistics and sums stay in its registers.
 
-// Sums over the rows' threads and a group's channels: `v` (one value per channel of each thread's
-// access) to total[group] in shared memory.  One warp per group, in a fixed order.
-template <int V, typename W>
-__device__ __forceinline__ void group_sums(const W (&v)[V], bool active, int tx, int ty, int across, int deep, int groups,
-                                           int width, W *scratch, W *total) {
-    __syncthreads();
-    if (active)
-#pragma unroll
-        for (int e = 0; e < V; ++e) scratch[(ty * across + tx) * V + e] = v[e];
-    __syncthreads();
-    const int warps = blockDim.x / 32;
-    for (int g = threadIdx.x / 32; g < groups; g += warps) {
-        W sum = 0;
-        for (int i = threadIdx.x % 32; i < deep * width; i += 32) sum += scratch[i / width * across * V + g * width + i % width];
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (threadIdx.x % 32 == 0) total[g] = sum;
-    }
-    __syncthreads();
-}
-
 // ---- slab form
 //
 // A cluster's CTAs hold `slab_rows` rows each of a block of whole groups of one n in shared memory.  A
 // thread copies in and reads back only its own accesses.  Sums are joined through the cluster in
 // rank order.
-template <typename T, int V> struct Slab {
+template <typename T, int V, int TENSORS> struct Slab {
     using W = WideOf<T>;
     uint64_t n, c0, s0;
-    int groups, across, deep, tx, ty, rows;
+    int groups, width, across, deep, tx, ty, rows;
     uint32_t rank, ranks;
     bool active;
-    unsigned char *data;
+    T *mine[TENSORS];  // this thread's first access of each tensor; its next ones are `deep` rows on
     W *scratch, *total, *joined;
 
-    __device__ __forceinline__ void place(const NormParams<T> &p, unsigned char *smem, int tensors) {
+    __device__ __forceinline__ void place(const NormParams<T> &p, unsigned char *smem) {
         const NormPlan &plan = p.plan;
         asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
         rank = cluster_rank();
         const unsigned cluster = blockIdx.x / ranks, block = cluster % plan.blocks;
         n = cluster / plan.blocks;
         const uint64_t g0 = (uint64_t)block * plan.block_groups;
+        width = (int)p.width;
         groups = (int)min((uint64_t)plan.block_groups, p.groups - g0);
         c0 = g0 * p.width;
-        across = (int)(groups * p.width / V);
+        across = groups * width / V;
         deep = (int)blockDim.x / across;
         tx = (int)threadIdx.x % across;
         ty = (int)threadIdx.x / across;
         active = ty < deep;
         s0 = (uint64_t)rank * plan.slab_rows;
         rows = s0 < p.positions ? (int)min((uint64_t)plan.slab_rows, p.positions - s0) : 0;
-        data = smem;
-        scratch = reinterpret_cast<W *>(smem + (size_t)tensors * slab_bytes(plan, p));
-        total = scratch + blockDim.x * V;
+#pragma unroll
+        for (int t = 0; t < TENSORS; ++t)
+            mine[t] = reinterpret_cast<T *>(smem + t * plan.slab_bytes) + (ty * across + tx) * V;
+        scratch = reinterpret_cast<W *>(smem + TENSORS * plan.slab_bytes);
+        total = scratch + TENSORS * blockDim.x * V;
         joined = total + 2 * plan.block_groups;
     }
-    static __host__ __device__ __forceinline__ size_t slab_bytes(const NormPlan &plan, uint64_t width) {
-        return ((size_t)plan.slab_rows * plan.block_groups * width * sizeof(T) + 15) / 16 * 16;
-    }
-    __device__ __forceinline__ size_t slab_bytes(const NormPlan &plan, const NormParams<T> &p) const {
-        return slab_bytes(plan, p.width);
-    }
-    __device__ __forceinline__ T *element(int tensor, const NormParams<T> &p, int r) const {
-        return reinterpret_cast<T *>(data + (size_t)tensor * slab_bytes(p.plan, p)) + ((size_t)r * across + tx) * V;
-    }
-    __device__ __forceinline__ void bring(int tensor, const NormParams<T> &p, const Maps<const T> &from) const {
+    __device__ __forceinline__ uint64_t channel() const { return c0 + (uint64_t)tx * V; }
+    __device__ __forceinline__ int step() const { return deep * across * V; }  // from one access to the next
+    __device__ __forceinline__ void bring(int tensor, const Maps<const T> &from) const {
         if (!active) return;
-        for (int r = ty; r < rows; r += deep) {
-            const T *src = from.at(n, s0 + r, c0 + (uint64_t)tx * V);
-            T *dst = element(tensor, p, r);
+        const T *src = from.at(n, s0 + ty, channel());
+        T *dst = mine[tensor];
+        const uint64_t stride = deep * from.row;
+        for (int r = ty; r < rows; r += deep, src += stride, dst += step()) {
             if (V > 1)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
             else
                 *dst = *src;
         }
     }
-    __device__ __forceinline__ void read(int tensor, const NormParams<T> &p, int r, W (&v)[V]) const {
-        if constexpr (V > 1) unpack<T>(*reinterpret_cast<const uint4 *>(element(tensor, p, r)), v);
-        else v[0] = Elem<T>::load(*element(tensor, p, r));
+    __device__ __forceinline__ static void read(const T *at, W (&v)[V]) {
+        if constexpr (V > 1) unpack<T>(*reinterpret_cast<const uint4 *>(at), v);
+        else v[0] = Elem<T>::load(*at);
     }
-    // sums `slot` of all the cluster's CTAs, in every CTA
-    __device__ __forceinline__ void sum(const W (&v)[V], int slot, const NormParams<T> &p) const {
-        W *mine = total + slot * p.plan.block_groups;
-        group_sums<V>(v, active, tx, ty, across, deep, groups, (int)p.width, scratch, mine);
+    // One value per channel of each thread's access, for Q quantities, summed over the rows' threads and
+    // given to each(quantity, channel of the block, sum); then, times what it returns, over each group's
+    // channels and the cluster's CTAs to joined[slot + quantity].
+    template <int Q, typename F> __device__ __forceinline__ void sum(const W (&v)[Q][V], int slot, unsigned block_groups, F each) const {
+        const int wide = across * V;
+        __syncthreads();
+        if (active)
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int e = 0; e < V; ++e) scratch[(q * deep + ty) * wide + tx * V + e] = v[q][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < Q * wide; i += blockDim.x) {
+            const int q = i >= wide ? 1 : 0, c = i - q * wide;
+            W all = 0;
+#pragma unroll 4
+            for (int d = 0; d < deep; ++d) all += scratch[(q * deep + d) * wide + c];
+            scratch[q * deep * wide + c] = each(q, c, all);  // the first row's place: only this thread reads it
+        }
+        __syncthreads();
+        const int warps = blockDim.x / 32;
+        for (int i = threadIdx.x / 32; i < Q * groups; i += warps) {
+            const int q = i >= groups ? 1 : 0, g = i - q * groups;
+            W all = 0;
+            for (int d = threadIdx.x % 32; d < width; d += 32) all += scratch[q * deep * wide + g * width + d];
+            for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
+            if (threadIdx.x % 32 == 0) total[(slot + q) * block_groups + g] = all;
+        }
         if (ranks > 1) cluster_sync();
-        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-            W all = ranks > 1 ? W(0) : mine[g];
-            if (ranks > 1)
+        else __syncthreads();
+        for (int i = threadIdx.x; i < Q * groups; i += blockDim.x) {
+            const int q = i >= groups ? 1 : 0, to = (slot + q) * (int)block_groups + i - q * groups;
+            W all = total[to];
+            if (ranks > 1) {
+                all = 0;
                 for (uint32_t r = 0; r < ranks; ++r) {
-                    W v2;
-                    cluster_read(v2, smem_addr(mine + g), r);
-                    all += v2;
+                    W other;
+                    cluster_read(other, smem_addr(total + to), r);
+                    all += other;
                 }
-            joined[slot * p.plan.block_groups + g] = all;
+            }
+            joined[to] = all;
         }
         __syncthreads();
     }
-    __device__ __forceinline__ W sum_of(int slot, int e, const NormParams<T> &p) const {
-        return joined[slot * p.plan.block_groups + (tx * V + e) / (int)p.width];
+    // a quantity's joint sum for each channel of this thread's access
+    __device__ __forceinline__ void sums_of(int slot, unsigned block_groups, W (&v)[V]) const {
+        int g = tx * V / width, left = (g + 1) * width - tx * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            v[e] = joined[slot * block_groups + g];
+            if (--left == 0) ++g, left = width;
+        }
     }
 };
 
-template <typename T, int V> __global__ void __launch_bounds__(512) norm_slab_kernel(const NormParams<T> p) {
+template <typename T, int V> __global__ void __launch_bounds__(512, sizeof(WideOf<T>) == 8 ? 1 : 2) norm_slab_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ __align__(16) unsigned char smem[];
-    Slab<T, V> at;
-    at.place(p, smem, 1);
-    at.bring(0, p, p.x);
-    const uint64_t c = at.c0 + (uint64_t)at.tx * V;
-    W w[V], b[V];
-    if (at.active) parameters<V>(p.weight, c, W(1), w), parameters<V>(p.bias, c, W(0), b);
+    Slab<T, V, 1> at;
+    at.place(p, smem);
+    at.bring(0, p.x);
+    const uint64_t c = at.channel();
+    const unsigned bg = p.plan.block_groups;
     const W inverse = W(1) / ((W)p.positions * (W)p.width);
+    auto same = [](int, int, W v) { return v; };
     asm volatile("cp.async.wait_all;" ::: "memory");
-    W v[V] = {}, x[V], mean[V], r[V];
-    if (at.active)
-        for (int i = at.ty; i < at.rows; i += at.deep) {
-            at.read(0, p, i, x);
+    W v[1][V] = {}, x[V], mean[V] = {}, r[V], w[V], b[V];
+    const int step = at.step();
+    if (at.active) {
+        const T *from = at.mine[0];
+        for (int i = at.ty; i < at.rows; i += at.deep, from += step) {
+            at.read(from, x);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] += x[e];
+            for (int e = 0; e < V; ++e) v[0][e] += x[e];
         }
-    at.sum(v, 0, p);
+    }
+    at.sum(v, 0, bg, same);
+    if (at.active) at.sums_of(0, bg, mean);
 #pragma unroll
-    for (int e = 0; e < V; ++e) mean[e] = at.active ? at.sum_of(0, e, p) * inverse : W(0), v[e] = W(0);
-    if (at.active)
-        for (int i = at.ty; i < at.rows; i += at.deep) {
-            at.read(0, p, i, x);
+    for (int e = 0; e < V; ++e) mean[e] *= inverse, v[0][e] = W(0);
+    if (at.active) {
+        const T *from = at.mine[0];
+        for (int i = at.ty; i < at.rows; i += at.deep, from += step) {
+            at.read(from, x);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] += (x[e] - mean[e]) * (x[e] - mean[e]);
+            for (int e = 0; e < V; ++e) v[0][e] += (x[e] - mean[e]) * (x[e] - mean[e]);
         }
-    at.sum(v, 1, p);
+    }
+    at.sum(v, 1, bg, same);
     if (at.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // read; see the end
     if (at.rank == 0)
         for (int g = threadIdx.x; g < at.groups; g += blockDim.x) {
             W *to = p.stats_out + 2 * (at.n * p.groups + at.c0 / p.width + g);
             to[0] = at.joined[g] * inverse;
-            to[1] = root(at.joined[p.plan.block_groups + g] * inverse, p.eps);
+            to[1] = root(at.joined[bg + g] * inverse, p.eps);
         }
     if (at.active) {
+        parameters<V>(p.weight, c, W(1), w), parameters<V>(p.bias, c, W(0), b);
+        at.sums_of(1, bg, r);
 #pragma unroll
-        for (int e = 0; e < V; ++e) r[e] = root(at.sum_of(1, e, p) * inverse, p.eps);
-        for (int i = at.ty; i < at.rows; i += at.deep) {
-            at.read(0, p, i, x);
+        for (int e = 0; e < V; ++e) r[e] = root(r[e] * inverse, p.eps);
+        const T *from = at.mine[0];
+        T *to = p.out.at(at.n, at.s0 + at.ty, c);
+        const uint64_t stride = at.deep * p.out.row;
+        for (int i = at.ty; i < at.rows; i += at.deep, from += step, to += stride) {
+            at.read(from, x);
 #pragma unroll
             for (int e = 0; e < V; ++e) x[e] = (x[e] - mean[e]) * r[e] * w[e] + b[e];
             activate<V>(p.activation, x);
-            put<T, V>(p.out.at(at.n, at.s0 + i, c), x, (at.n * p.positions + at.s0 + i) * p.channels + c, p.status);
+            put<T, V>(to, x, p.status, [&] { return (at.n * p.positions + at.s0 + i) * p.channels + c; });
         }
     }
     __syncwarp();
@@ -496,61 +563,58 @@ template <typename T, int V> __global__ void __launch_bounds__(512) norm_slab_ba
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ __align__(16) unsigned char smem[];
-    Slab<T, V> at;
-    at.place(p, smem, 2);
-    at.bring(0, p, p.x);
-    at.bring(1, p, p.dy);
-    const uint64_t c = at.c0 + (uint64_t)at.tx * V;
-    W w[V], b[V], mean[V], r[V], dw[V] = {}, db[V] = {}, x[V], dy[V], h[V], dz[V];
+    Slab<T, V, 2> at;
+    at.place(p, smem);
+    at.bring(0, p.x);
+    at.bring(1, p.dy);
+    const uint64_t c = at.channel();
+    const unsigned bg = p.plan.block_groups;
+    W w[V], b[V], mean[V], r[V], sums[2][V] = {}, x[V], dy[V], h[V], dz[V];
     if (at.active) {
         parameters<V>(p.weight, c, W(1), w), parameters<V>(p.bias, c, W(0), b);
+        const W *st = p.stats + 2 * (at.n * p.groups + c / p.width);
+        int left = (int)(p.width - c % p.width);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const W *st = p.stats + 2 * (at.n * p.groups + (c + e) / p.width);
             mean[e] = st[0], r[e] = st[1];
+            if (--left == 0 && e + 1 < V) st += 2, left = at.width;
         }
     }
     const W inverse = W(1) / ((W)p.positions * (W)p.width);
+    const int step = at.step();
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (at.active)
-        for (int i = at.ty; i < at.rows; i += at.deep) {
-            at.read(0, p, i, x);
-            at.read(1, p, i, dy);
+    if (at.active) {
+        const T *from = at.mine[0], *up = at.mine[1];
+        for (int i = at.ty; i < at.rows; i += at.deep, from += step, up += step) {
+            at.read(from, x);
+            at.read(up, dy);
             bend<V>(p.activation, x, dy, mean, r, w, b, h, dz);
 #pragma unroll
-            for (int e = 0; e < V; ++e) dw[e] += dz[e] * h[e], db[e] += dz[e];
-        }
-    if (p.partial) {  // this CTA's share of the parameters' gradients, summed over its rows' threads
-        W *to = p.partial + 2 * (at.n * at.ranks + at.rank) * p.channels + at.c0;
-        for (int q = 0; q < 2; ++q) {
-            __syncthreads();
-            if (at.active)
-#pragma unroll
-                for (int e = 0; e < V; ++e) at.scratch[(at.ty * at.across + at.tx) * V + e] = q ? db[e] : dw[e];
-            __syncthreads();
-            for (int i = threadIdx.x; i < at.across * V; i += blockDim.x) {
-                W sum = 0;
-                for (int d = 0; d < at.deep; ++d) sum += at.scratch[d * at.across * V + i];
-                to[q * p.channels + i] = sum;
-            }
+            for (int e = 0; e < V; ++e) sums[0][e] += dz[e] * h[e], sums[1][e] += dz[e];
         }
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) dw[e] = at.active ? dw[e] * w[e] : W(0), db[e] = at.active ? db[e] * w[e] : W(0);
-    at.sum(db, 0, p);
-    at.sum(dw, 1, p);
+    // c2 and c1 of each group; on the way, this CTA's share of the parameters' gradients
+    W *share = p.partial ? p.partial + 2 * (at.n * at.ranks + at.rank) * p.channels + at.c0 : nullptr;
+    at.sum(sums, 0, bg, [&](int q, int i, W v) {
+        if (share) share[q * p.channels + i] = v;
+        return p.weight ? v * p.weight[at.c0 + i] : v;
+    });
     if (at.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // read; see the end
     if (at.active) {
         W c1[V], c2[V];
+        at.sums_of(0, bg, c2), at.sums_of(1, bg, c1);
 #pragma unroll
-        for (int e = 0; e < V; ++e) c1[e] = at.sum_of(0, e, p) * inverse, c2[e] = at.sum_of(1, e, p) * inverse;
-        for (int i = at.ty; i < at.rows; i += at.deep) {
-            at.read(0, p, i, x);
-            at.read(1, p, i, dy);
+        for (int e = 0; e < V; ++e) c1[e] *= inverse, c2[e] *= inverse;
+        const T *from = at.mine[0], *up = at.mine[1];
+        T *to = p.out.at(at.n, at.s0 + at.ty, c);
+        const uint64_t stride = at.deep * p.out.row;
+        for (int i = at.ty; i < at.rows; i += at.deep, from += step, up += step, to += stride) {
+            at.read(from, x);
+            at.read(up, dy);
             bend<V>(p.activation, x, dy, mean, r, w, b, h, dz);
 #pragma unroll
             for (int e = 0; e < V; ++e) x[e] = r[e] * (dz[e] * w[e] - c1[e] - h[e] * c2[e]);
-            put<T, V>(p.out.at(at.n, at.s0 + i, c), x, (at.n * p.positions + at.s0 + i) * p.channels + c, p.status);
+            put<T, V>(to, x, p.status, [&] { return (at.n * p.positions + at.s0 + i) * p.channels + c; });
         }
     }
     __syncwarp();
@@ -686,7 +750,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] = (x[e] - mean[e]) * r[e] * w[e] + b[e];
         activate<V>(p.activation, x);
-        put<T, V>(p.out.at(at.n, s, at.c), x, (at.n * p.positions + s) * p.channels + at.c, p.status);
+        put<T, V>(p.out.at(at.n, s, at.c), x, p.status, [&] { return (at.n * p.positions + s) * p.channels + at.c; });
     }
 }
 
@@ -766,7 +830,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
         bend<V>(p.activation, x, dy, mean, r, w, b, h, dz);
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] = r[e] * (dz[e] * w[e] - c1[e] - h[e] * c2[e]);
-        put<T, V>(p.out.at(at.n, s, at.c), x, (at.n * p.positions + s) * p.channels + at.c, p.status);
+        put<T, V>(p.out.at(at.n, s, at.c), x, p.status, [&] { return (at.n * p.positions + s) * p.channels + at.c; });
     }
 }
 
@@ -856,8 +920,9 @@ NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, ui
         while (p.lanes < 32 && (unsigned)p.lanes < p.items) p.lanes *= 2;
         p.per_lane = (int)((p.items + p.lanes - 1) / p.lanes);
         const uint64_t per = 32 / p.lanes, sets = (groups + per - 1) / per;
-        // Each warp takes several of the batch where there are enough: 32 warps per SM walk.
-        p.slices = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(batch, (sms * 32 + sets - 1) / sets));
+        const uint64_t ctas = p.per_lane > 4 ? 1 : warp_form_ctas(vector * p.per_lane, (int)wide);
+        // Each warp walks over a slice of the batch; as many warps as are resident at once.
+        p.slices = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(batch, sms * ctas * (kNormThreads / 32) / sets));
         p.partial_rows = p.slices;
         p.partial_split = positions;
         p.workspace = backward ? 2 * p.partial_rows * channels * positions : 0;
@@ -878,16 +943,17 @@ NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, ui
         const uint64_t blocks = (groups + block - 1) / block;
         while (ranks < 8 && batch * blocks * ranks < 2 * sms && (positions + ranks - 1) / ranks * row > 16384) ranks *= 2;
         const uint64_t rows = (positions + ranks - 1) / ranks;
-        const uint64_t threads = across > 256 ? 512 : 256;
-        const uint64_t extra = threads * vector * wide + 4 * block * wide + 64;
-        if (rows > 0x7fffffffull || rows * row + extra + 32 > kSlabMost || batch * blocks * ranks > 0x7fffffffull) return false;
+        const uint64_t threads = across > 256 || (!backward && batch * blocks * ranks <= 2 * sms) ? 512 : 256;
+        const uint64_t extra = tensors * threads * vector * wide + 4 * block * wide + 64;
+        if (rows > 0x7fffffffull || rows * row + extra + 64 > kSlabMost || batch * blocks * ranks > 0x7fffffffull) return false;
         p.form = NormPlan::kSlab;
         p.block_groups = (unsigned)block;
         p.blocks = (unsigned)blocks;
         p.ranks = (unsigned)ranks;
         p.threads = (unsigned)threads;
         p.slab_rows = (unsigned)rows;
-        p.shared = tensors * ((rows * block * width * bytes + 15) / 16 * 16) + extra;
+        p.slab_bytes = (rows * block * width * bytes + 15) / 16 * 16;
+        p.shared = tensors * p.slab_bytes + extra;
         p.partial_rows = batch * ranks;
         p.workspace = backward ? 2 * p.partial_rows * channels : 0;
         return true;
