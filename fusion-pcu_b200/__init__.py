@@ -179,12 +179,18 @@ def _declare(L):
     L.pcu_b200_comm_strict_mse.argtypes = [vp, i32, i32, vp, vp, u64, u64, u64, vp, vp, sz, vp, vp]
 
 
-def _torch():
-    import torch
+_torch_module = None  # torch, once a CUDA device has been seen (asking again costs microseconds a call)
 
-    if not torch.cuda.is_available():
-        raise ProviderUnavailable("no CUDA device: the strict provider has no CPU fallback")
-    return torch
+
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
+        if not torch.cuda.is_available():
+            raise ProviderUnavailable("no CUDA device: the strict provider has no CPU fallback")
+        _torch_module = torch
+    return _torch_module
 
 
 def _check(rc):

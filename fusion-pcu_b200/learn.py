@@ -11,13 +11,17 @@ worked on on their own device.  The reference has no counterpart of these operat
 import functools
 import inspect
 
-from . import _check, _node, _ptr, _rate_bits, _torch, library, new_status
+from . import _check, _rate_bits, _torch, library, new_status
 
 __all__ = ["ACTIVATIONS", "group_norm", "group_norm_backward", "distill_loss", "distill_loss_backward",
            "distill_loss_step", "block_quantize", "block_matmul"]
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 DISTILL_TOP_MAX = 1024
+
+# The kernels of small calls take a few microseconds, so the host's part is kept short: pointers go as
+# plain integers, devices are compared by index, what depends on numbers alone is remembered.
+_bits = functools.lru_cache(maxsize=None)(_rate_bits)
 
 
 @functools.lru_cache(maxsize=None)
@@ -26,6 +30,33 @@ def _types():
     codes = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloat16: 3}
     wide = {t: torch.float64 if t == torch.float64 else torch.float32 for t in codes}
     return codes, wide
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name, guarded):
+    return getattr(library(), ("pcu_b200_guarded_" if guarded else "pcu_b200_") + name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _need(name, device, *sizes):
+    """Workspace bytes of a call on `device` (which is current)."""
+    return getattr(library(), f"pcu_b200_{name}_workspace_size")(*sizes)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(name, args, status, chain, like):
+    """pcu_b200_<name>(*args, status, stream) on the current stream; with chain=(records, stage), its
+    guarded form."""
+    stream = _torch()._C._cuda_getCurrentRawStream(like.get_device())
+    if chain is None:
+        rc = _entry(name, False)(*args, status.data_ptr(), stream)
+    else:
+        rc = _entry(name, True)(*args, chain[0].data_ptr(), int(chain[1]), stream)
+    if rc:
+        _check(rc)
 
 
 def _code(t):
@@ -44,7 +75,7 @@ def _on_device(call):
     def wrapped(*args, **kwargs):
         torch = _torch()
         first = args[0] if args else kwargs[name]
-        if first.device.type != "cuda":
+        if not first.is_cuda:
             raise ValueError(f"{name}: a CUDA tensor is wanted, got one on {first.device}")
         stream = kwargs.get("stream")
         if stream is not None:
@@ -52,7 +83,7 @@ def _on_device(call):
                 raise ValueError(f"stream is on {stream.device}, {name} on {first.device}")
             with torch.cuda.stream(stream):
                 return call(*args, **kwargs)
-        if first.device.index != torch.cuda.current_device():
+        if first.get_device() != torch._C._cuda_getDevice():
             with torch.cuda.device(first.device):
                 return call(*args, **kwargs)
         return call(*args, **kwargs)
@@ -63,22 +94,30 @@ def _want(name, t, like, shape=None, dtype=None):
     """`t` is a dense tensor of the given shape and type on the device of `like`."""
     if t is None:
         return
-    if t.device != like.device:
+    if not t.is_cuda or t.get_device() != like.get_device():
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}, {dtype} is wanted")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, {tuple(shape)} is wanted")
     if not t.is_contiguous():
         raise ValueError(f"{name} is not contiguous")
 
 
+def _alike(name, t, like):
+    if t.shape != like.shape or t.dtype != like.dtype or not t.is_cuda or t.get_device() != like.get_device():
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}, "
+                         f"{tuple(like.shape)} {like.dtype} on {like.device} is wanted")
+
+
 def _status(status, chain, like):
     if chain is not None:
+        if not chain[0].is_cuda or chain[0].get_device() != like.get_device():
+            raise ValueError(f"the chain's records are on {chain[0].device}, not on {like.device}")
         return status
     if status is None:
         return new_status(device=like.device)
-    if status.device != like.device or status.element_size() != 8 or status.numel() < 1:
+    if not status.is_cuda or status.get_device() != like.get_device() or status.element_size() != 8 or status.numel() < 1:
         raise ValueError(f"status is one 64-bit word on {like.device}")
     return status
 
@@ -90,9 +129,8 @@ def _maps(name, t, like=None):
     positions, channels], or [batch, channels] with one position."""
     if t.dim() not in (2, 3):
         raise ValueError(f"{name} is [batch, positions, channels] or [batch, channels], got {tuple(t.shape)}")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}, "
-                         f"{tuple(like.shape)} {like.dtype} on {like.device} is wanted")
+    if like is not None:
+        _alike(name, t, like)
     n, c = t.shape[0], t.shape[-1]
     if t.dim() == 2:
         s, batch_stride, stride = 1, t.stride(0), max(c, t.stride(0))
@@ -118,8 +156,8 @@ def _norm_shape(x, groups, weight, bias, activation):
 
 def _workspace(workspace, need, like):
     if workspace is None:
-        return _torch().empty(max(need, 1), dtype=_torch().uint8, device=like.device) if need else None
-    if workspace.device != like.device or workspace.numel() * workspace.element_size() < need:
+        return _torch().empty(need, dtype=_torch().uint8, device=like.device) if need else None
+    if not workspace.is_cuda or workspace.get_device() != like.get_device() or workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace holds {need} bytes on {like.device}")
     return workspace
 
@@ -141,11 +179,11 @@ def group_norm(x, groups, weight=None, bias=None, activation="none", eps=1e-5, o
     _want("stats", stats, x, (n, groups, 2), wide)
     _, _, _, out_batch, out_stride = _maps("out", out, x)
     status = _status(status, chain, x)
-    need = library().pcu_b200_group_norm_workspace_size(code, n, s, c, groups)
+    need = _need("group_norm", x.get_device(), code, n, s, c, groups)
     workspace = _workspace(workspace, need, x)
-    _check(_node("group_norm", (code, ACTIVATIONS[activation], _ptr(x), _ptr(weight), _ptr(bias), _ptr(out),
-                                _ptr(stats), n, s, c, groups, batch_stride, stride, out_batch, out_stride,
-                                _rate_bits(eps), _ptr(workspace), need), status, chain, stream))
+    _call("group_norm", (code, ACTIVATIONS[activation], _ptr(x), _ptr(weight), _ptr(bias), _ptr(out), _ptr(stats),
+          n, s, c, groups, batch_stride, stride, out_batch, out_stride, _bits(eps), _ptr(workspace), need), status,
+          chain, x)
     return out, stats
 
 
@@ -169,12 +207,11 @@ def group_norm_backward(x, upstream, groups, stats, weight=None, bias=None, acti
     _want("dweight", dweight, x, (c,), wide)
     _want("dbias", dbias, x, (c,), wide)
     status = _status(status, chain, x)
-    need = library().pcu_b200_group_norm_backward_workspace_size(code, n, s, c, groups)
+    need = _need("group_norm_backward", x.get_device(), code, n, s, c, groups)
     workspace = _workspace(workspace, need, x)
-    _check(_node("group_norm_backward",
-                 (code, ACTIVATIONS[activation], _ptr(x), _ptr(upstream), _ptr(weight), _ptr(bias), _ptr(stats),
-                  _ptr(dx), _ptr(dweight), _ptr(dbias), n, s, c, groups, batch_stride, stride, up_batch, up_stride,
-                  dx_batch, dx_stride, _ptr(workspace), need), status, chain, stream))
+    _call("group_norm_backward", (code, ACTIVATIONS[activation], _ptr(x), _ptr(upstream), _ptr(weight),
+          _ptr(bias), _ptr(stats), _ptr(dx), _ptr(dweight), _ptr(dbias), n, s, c, groups, batch_stride, stride,
+          up_batch, up_stride, dx_batch, dx_stride, _ptr(workspace), need), status, chain, x)
     return dx, dweight, dbias
 
 
@@ -184,9 +221,8 @@ def _rows(name, t, like=None):
     """Row stride of a matrix with adjacent columns."""
     if t.dim() != 2:
         raise ValueError(f"{name} is a matrix, got {tuple(t.shape)}")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}, "
-                         f"{tuple(like.shape)} {like.dtype} on {like.device} is wanted")
+    if like is not None:
+        _alike(name, t, like)
     if t.numel() and t.shape[1] > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: columns must be adjacent")
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -208,7 +244,7 @@ def _distill(logits, top_indices, top_logits, temperature, row_weights):
     _want("top_logits", top_logits, logits, (rows, k), wide)
     _want("row_weights", row_weights, logits, (rows,), wide)
     return wide, (code, _ptr(logits), rows, vocab, stride, _ptr(top_indices), _ptr(top_logits), k, _ptr(row_weights),
-                  _rate_bits(temperature))
+                  _bits(temperature))
 
 
 def _upstream(upstream, logits, wide):
@@ -217,7 +253,7 @@ def _upstream(upstream, logits, wide):
     _want("upstream", upstream, logits, dtype=wide)
     if upstream.numel() == 1:
         return (_ptr(upstream), 1)
-    if tuple(upstream.shape) != (logits.shape[0],):
+    if upstream.shape != (logits.shape[0],):
         raise ValueError(f"upstream is one value or one for each of {logits.shape[0]} rows, got {tuple(upstream.shape)}")
     return (_ptr(upstream), 0)
 
@@ -239,7 +275,7 @@ def distill_loss(logits, top_indices, top_logits, temperature=1.0, row_weights=N
     _want("loss", loss, logits, (rows,), wide)
     _want("stats", stats, logits, (rows, 2), wide)
     status = _status(status, chain, logits)
-    _check(_node("distill_loss", inputs + (_ptr(loss), _ptr(stats)), status, chain, stream))
+    _call("distill_loss", inputs + (_ptr(loss), _ptr(stats)), status, chain, logits)
     return loss, stats
 
 
@@ -256,8 +292,8 @@ def distill_loss_backward(logits, top_indices, top_logits, stats, upstream=None,
     stride = _rows("gradient", gradient, logits)
     up, uniform = _upstream(upstream, logits, wide)
     status = _status(status, chain, logits)
-    _check(_node("distill_loss_backward", inputs + (_ptr(stats), up, uniform, _ptr(gradient), stride), status, chain,
-                 stream))
+    _call("distill_loss_backward", inputs + (_ptr(stats), up, uniform, _ptr(gradient), stride), status, chain,
+          logits)
     return gradient
 
 
@@ -280,8 +316,8 @@ def distill_loss_step(logits, top_indices, top_logits, upstream=None, temperatur
     stride = _rows("gradient", gradient, logits)
     up, uniform = _upstream(upstream, logits, wide)
     status = _status(status, chain, logits)
-    _check(_node("distill_loss_step", inputs + (_ptr(loss), _ptr(stats), up, uniform, _ptr(gradient), stride), status,
-                 chain, stream))
+    _call("distill_loss_step", inputs + (_ptr(loss), _ptr(stats), up, uniform, _ptr(gradient), stride), status,
+          chain, logits)
     return loss, stats, gradient
 
 
@@ -291,7 +327,7 @@ def _codes(name, t, like=None):
     torch = _torch()
     if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
         raise TypeError(f"{name} is {t.dtype}, float8_e4m3fn (or its bytes, uint8) is wanted")
-    if like is not None and t.device != like.device:
+    if like is not None and (not t.is_cuda or t.get_device() != like.get_device()):
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
     return _rows(name, t)
 
@@ -320,8 +356,8 @@ def block_quantize(x, block_rows=1, codes=None, scales=None, status=None, *, str
     codes_stride = _codes("codes", codes, x)
     _want("scales", scales, x, shape, torch.float32)
     status = _status(status, chain, x)
-    _check(_node("block_quantize", (code, _ptr(x), rows, columns, stride, block_rows, _ptr(codes), codes_stride,
-                                    _ptr(scales)), status, chain, stream))
+    _call("block_quantize", (code, _ptr(x), rows, columns, stride, block_rows, _ptr(codes), codes_stride,
+          _ptr(scales)), status, chain, x)
     return codes, scales
 
 
@@ -343,11 +379,11 @@ def block_matmul(left, left_scales, right, right_scales, out=None, dtype=None, s
         out = torch.empty((rows, columns), dtype=dtype or torch.bfloat16, device=left.device)
     elif dtype is not None and out.dtype != dtype:
         raise TypeError(f"out is {out.dtype}, {dtype} is wanted")
-    if out.dtype == torch.float64 or tuple(out.shape) != (rows, columns) or out.device != left.device:
+    if out.dtype == torch.float64 or out.shape != (rows, columns) or not out.is_cuda or out.get_device() != left.get_device():
         raise ValueError(f"out is a {rows} x {columns} float32/float16/bfloat16 matrix on {left.device}")
     code = _code(out)
     out_stride = _rows("out", out)
     status = _status(status, chain, left)
-    _check(_node("block_matmul", (code, _ptr(left), _ptr(left_scales), _ptr(right), _ptr(right_scales), _ptr(out),
-                                  rows, inner, columns, left_stride, right_stride, out_stride), status, chain, stream))
+    _call("block_matmul", (code, _ptr(left), _ptr(left_scales), _ptr(right), _ptr(right_scales), _ptr(out), rows,
+          inner, columns, left_stride, right_stride, out_stride), status, chain, left)
     return out
