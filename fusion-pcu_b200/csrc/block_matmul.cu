@@ -146,6 +146,12 @@ template <typename T> struct ProductParams {
     ChainGuard guard;
 };
 
+// A scale as the product takes it: a power of two from 2^-126 on, NaN for anything else.
+__device__ __forceinline__ float checked_scale(float scale) {
+    const unsigned bits = __float_as_uint(scale);
+    return (bits & 0x807fffffu) == 0 && bits >= 0x00800000u && bits < 0x7f800000u ? scale : NAN;
+}
+
 template <typename T> __device__ __forceinline__ void store_cell(const ProductParams<T> &p, uint64_t r, uint64_t c, float v) {
     const T y = Elem<T>::round(v);
     p.out[r * p.out_stride + c] = y;
@@ -205,21 +211,19 @@ template <typename T> __global__ void __launch_bounds__(256) product_plain_kerne
             __syncthreads();
         }
         if (r < p.rows && c < p.columns)
-            acc = fmaf(part, p.left_scales[r * blocks + kb] * p.right_scales[c / kBlock * blocks + kb], acc);
+            acc += part * checked_scale(p.left_scales[r * blocks + kb]) * checked_scale(p.right_scales[c / kBlock * blocks + kb]);
     }
     if (r < p.rows && c < p.columns) store_cell(p, r, c, acc);
 }
 
 // ------------------------------------------------------------------ tensor core product
 //
-// D = P . Q^T over blocks of 128 of the inner dimension.  The tensor core cannot apply a scale that
-// changes from block to block of its accumulator, so each block's product goes to a TMEM buffer of
-// its own and the epilogue warps add it, scaled, to binary32 sums in registers while the next
-// blocks' products run.
+// D = P . Q^T over blocks of 128 of the inner dimension.
 //   * batch form (product_kernel): P = left, Q = right.  A pair of CTAs works on 256 x 256 cells.
 //   * row form (product_rows_kernel), few rows: P = right, Q = left, 128 columns x BN rows, so that
 //     the weights, which are all the traffic there is, fill the instruction's 128 rows.  The blocks
-//     of one tile are split over a cluster's CTAs; the first CTA adds their sums, in rank order.
+//     of one tile are split over a cluster's CTAs; the first CTA adds their sums, in rank order.  Each
+//     block's product goes to a TMEM buffer of its own and is added, scaled, to sums in registers.
 // All waits are bounded (mbar_wait); one that runs out records the watchdog kind, and the CTA still
 // waits for its own copies and products before it frees TMEM and returns.
 
@@ -297,15 +301,6 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
                  : "memory");
 }
 
-// Two binary32 multiply-adds in one instruction: sum += (a0 f0, a1 f1).
-__device__ __forceinline__ void fma_two(uint64_t &sum, uint32_t a0, uint32_t a1, float f0, float f1) {
-    asm("{\n\t.reg .b64 a, f;\n\t"
-        "mov.b64 a, {%1, %2};\n\tmov.b64 f, {%3, %4};\n\t"
-        "fma.rn.f32x2 %0, a, f, %0;\n\t}"
-        : "+l"(sum)
-        : "r"(a0), "r"(a1), "f"(f0), "f"(f1));
-}
-
 // A whole warp waits, with one answer.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
     return __all_sync(~0u, mbar_wait(bar, parity));
@@ -332,25 +327,24 @@ __device__ __forceinline__ void tile_place(const TileParams<T> &t, unsigned id, 
 //
 // A pair of CTAs (a cluster of 2) owns 256 x 256 cells: each holds 128 rows of P and half of Q's rows,
 // and one tcgen05.mma of the pair reads both, so each SM brings 32 KB per block of 128 from L2 where a
-// CTA by itself, with 128 x 256 cells, brings 48 KB (and was bound by that, at 10 TB/s of L2 reads).  A
-// block's product is two units of 128 columns, each with one of four TMEM buffers: a unit is drained
-// while others are computed or wait.
-// Warps: 0 TMA loads, 1 tcgen05.mma (first CTA only), 2 and 3 the rows' scales into shared memory (read
-// by each epilogue thread for itself they were 32 cache lines a load), 4 to 19 drain TMEM: warp w the
-// lanes from 32 (w % 4), every other unit and 64 of its columns.  A TMEM load takes some 200 cycles and a
-// wait waits for all of a warp's, so the drain is a chain of loads in each warp: about 550 cycles a block
-// with sixteen warps that take a unit in turn, 1,400 with eight that take half of every unit.
+// CTA by itself, with 128 x 256 cells, brings 48 KB (and was bound by that, at 10 TB/s of L2 reads).  The
+// scales are powers of two, so the tensor cores apply them (kind::mxf8f6f4, an exponent byte for each
+// 32 codes: a block's byte four times) and sum over all blocks in TMEM.  Scales of any kind had to be
+// applied in registers, a block's product at a time: that drained 256 KB of TMEM per pair and block, and
+// ran at 36 % of the tensor cores' rate (165 us for 8192 x 4096 x 4096) however the drain was spread.
+// Warps: 0 TMA loads, 1 tcgen05.cp of the exponents and tcgen05.mma (first CTA only), 2 and 3 exponents
+// into shared memory, 4 to 11 bring the sums to registers, 128 columns each, give TMEM back and store.
 struct Batch {
-    static constexpr int HALF = 128, BM = 2 * HALF, BN = 256, UNIT = 128, UNITS = BN / UNIT, BUFFERS = 4;
-    static constexpr int EPILOGUE = 16, COLUMNS = UNIT / (EPILOGUE / 4 / UNITS), PIECE = 32, THREADS = (4 + EPILOGUE) * 32;
-    // Registers a thread: of the first four warps, and of the others (64 sums, 32 on their way).  The
-    // launch gives every thread what the bounds allow, LAUNCHED, and the warps share it anew.
-    static constexpr int LAUNCHED = 96, SERVING = 32, DRAINING = 112;
-    static_assert(4 * SERVING + EPILOGUE * DRAINING <= (4 + EPILOGUE) * LAUNCHED, "a larger share would wait forever");
-    static constexpr int TMEM_COLUMNS = BUFFERS * UNIT;
+    static constexpr int HALF = 128, BM = 2 * HALF, BN = 256;
+    static constexpr int EPILOGUE = 8, COLUMNS = BN / (EPILOGUE / 4), THREADS = (4 + EPILOGUE) * 32;
     static constexpr int P_BYTES = HALF * kBlock, Q_BYTES = BN / 2 * kBlock, STAGE_BYTES = P_BYTES + Q_BYTES;
-    static constexpr int STAGES = 6, CHUNK = 16;  // blocks of scales per chunk
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+    static constexpr int STAGES = 6;
+    // exponents: 512 bytes per 128 rows and block, CHUNK blocks at a time, two chunks
+    static constexpr int CHUNK = 8, EXPONENTS = 512 * (1 + BN / 128);
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * CHUNK * EXPONENTS + 1024;
+    // TMEM columns: the sums, then the exponents of four blocks (4 columns per 128 rows)
+    static constexpr int TMEM_COLUMNS = 512, SCALES_AT = BN, SCALES_STEP = 16, SCALES = 4;
+    static_assert(SCALES_AT + SCALES * SCALES_STEP <= TMEM_COLUMNS && 4 * (1 + BN / 128) <= SCALES_STEP, "TMEM");
 };
 
 // A load by either CTA of a pair that signals the first CTA's barrier.
@@ -362,16 +356,26 @@ __device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map,
         : "memory");
 }
 
-__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
+// D (binary32, TMEM of both CTAs) = or += A . B^T for 256 x N x 32 codes with their exponents in TMEM
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t sa, uint32_t sb,
+                                         uint32_t add) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(shape), "r"(add)
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(shape), "r"(sa), "r"(sb), "r"(add)
         : "memory");
 }
 
-// The barrier at this place in both CTAs completes when the pair's products issued before have.
+// 32 rows of 16 bytes (512 adjacent bytes) of each CTA's shared memory to 4 columns of its TMEM, to each
+// quarter of the lanes.  In order with the products issued before and after it.
+__device__ __forceinline__ void exponents_to_tmem(uint32_t to, uint32_t from) {
+    // no swizzle, 8 x 16-byte pieces 128 bytes apart, descriptor version 1
+    const uint64_t desc = (uint64_t)(from >> 4) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(desc) : "memory");
+}
+
+// The barrier at this place in both CTAs completes when the pair's tensor core work issued before has.
 __device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
@@ -380,11 +384,20 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
         : "memory");
 }
 
-// An arrival at a barrier of any CTA of the cluster, for a TMEM buffer that has been read: nothing in
-// memory is handed over (the loads have ended and tcgen05.fence orders them), so it is relaxed.  A
-// release at cluster scope waits for all of the thread's memory accesses, 1,000 cycles here.
+// An arrival at a barrier of any CTA of the cluster.  Relaxed for TMEM that has been read: nothing in memory
+// is handed over (the loads have ended and tcgen05.fence orders them), and a release at cluster scope
+// waits for all of the thread's memory accesses, 1,000 cycles here.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_release_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// A scale's exponent byte, four times.  What is no power of two from 2^-126 on gives NaN.
+__device__ __forceinline__ uint32_t exponent_word(float scale) {
+    const uint32_t bits = __float_as_uint(scale), e = bits >> 23;
+    return ((bits & 0x807fffffu) == 0 && e >= 1 && e <= 254 ? e : 0xffu) * 0x01010101u;
 }
 
 template <typename T>
@@ -396,10 +409,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ unsigned char smem_raw[];
     unsigned char *const tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], ready[S::BUFFERS], drained[S::BUFFERS], scaled[2], spent[2];
-    __shared__ uint64_t finished;
+    uint32_t *const exponents = reinterpret_cast<uint32_t *>(tiles + S::STAGES * S::STAGE_BYTES);
+    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], scaled[2], spent[2], ready, drained, finished;
     __shared__ uint32_t tmem_base;
-    __shared__ float row_scale[2][S::CHUNK][S::HALF + 1], column_scale[2][S::CHUNK][S::UNITS];
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // uniform, for the compiler too
     const uint32_t rank = cluster_rank();
     const unsigned first = blockIdx.x / 2, step = gridDim.x / 2;
@@ -407,9 +419,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int i = 0; i < S::BUFFERS; ++i) mbar_init(&ready[i], 1), mbar_init(&drained[i], 2 * S::EPILOGUE / S::UNITS);
-        for (int i = 0; i < 2; ++i) mbar_init(&scaled[i], 2), mbar_init(&spent[i], S::EPILOGUE);
-        mbar_init(&finished, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&scaled[i], 4), mbar_init(&spent[i], 1);
+        mbar_init(&ready, 1), mbar_init(&drained, 2 * S::EPILOGUE), mbar_init(&finished, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -424,143 +435,131 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = __shfl_sync(~0u, tmem_base, 0);
 
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::SERVING));
-        if (warp == 0) {
-            if (lane == 0) {
-                int it = 0;
-                bool ok = true;
-                for (unsigned id = first; ok && id < t.tiles; id += step) {
-                    unsigned tp, tq;
-                    tile_place(t, id, tp, tq);
-                    const int p0 = (int)(tp * S::BM + rank * S::HALF), q0 = (int)(tq * S::BN + rank * (S::UNIT / 2));
-                    for (int kb = 0; kb < KB; ++kb, ++it) {
-                        const int s = it % S::STAGES;
-                        if (!(ok = mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1))) break;
-                        unsigned char *to = tiles + s * S::STAGE_BYTES;
-                        const uint32_t bar = cluster_address(smem_addr(&full[s]), 0);
-                        if (rank == 0) mbar_expect_tx(&full[s], 2 * S::STAGE_BYTES);  // both CTAs' loads
-                        tma_load_pair(to, &map_p, bar, kb * kBlock, p0);
-#pragma unroll
-                        for (int u = 0; u < S::UNITS; ++u)  // this CTA's half of each unit's columns
-                            tma_load_pair(to + S::P_BYTES + u * (S::UNIT / 2) * kBlock, &map_q, bar, kb * kBlock, q0 + u * S::UNIT);
-                    }
-                }
-                if (!ok) record_fault(p.status, 0, kWatchdog);
-                // Nothing is left in flight towards either CTA's shared memory when the pair ends.
-                if (rank == 0)
-                    for (int i = it > S::STAGES ? it - S::STAGES : 0; i < it; ++i)
-                        mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
-            }
-        } else if (warp == 1) {
-            if (rank == 0) {
-                constexpr uint32_t shape = 1u << 4 | (uint32_t)(S::UNIT / 8) << 17 | (uint32_t)(S::BM / 16) << 24;
-                const uint32_t stage0 = smem_addr(tiles);
-                int it = 0, unit = 0;
-                bool ok = true;
-                for (unsigned id = first; ok && id < t.tiles; id += step)
-                    for (int kb = 0; ok && kb < KB; ++kb, ++it) {
-                        const int s = it % S::STAGES;
-                        if (!(ok = warp_wait(&full[s], (it / S::STAGES) & 1))) break;
-                        const uint64_t pd = k_major_descriptor(stage0 + s * S::STAGE_BYTES);
-#pragma unroll
-                        for (int u = 0; u < S::UNITS; ++u, ++unit) {
-                            const int b = unit % S::BUFFERS;
-                            if (!(ok = __all_sync(~0u, mbar_wait_cluster(&drained[b], ((unit / S::BUFFERS) & 1) ^ 1)))) break;
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            const uint64_t qd = pd + ((S::P_BYTES + u * (S::UNIT / 2) * kBlock) >> 4);
-                            if (elect_one()) {
-#pragma unroll
-                                for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further along the swizzled rows
-                                    mma_pair(tmem + b * S::UNIT, pd + 2 * k, qd + 2 * k, shape, k != 0);
-                                mma_commit_pair(&ready[b]);
-                                if (u + 1 == S::UNITS) mma_commit_pair(&empty[s]);
-                            }
-                            __syncwarp();
-                        }
-                    }
-                if (elect_one()) mma_commit_pair(&finished);
-                __syncwarp();
-                ok = warp_wait(&finished, 0) && ok;
-                if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
-            }
-        } else {
-            int chunk = 0;
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
             bool ok = true;
             for (unsigned id = first; ok && id < t.tiles; id += step) {
                 unsigned tp, tq;
                 tile_place(t, id, tp, tq);
-                const uint64_t row0 = (uint64_t)tp * S::BM + rank * S::HALF + (warp - 2) * (S::HALF / 2);
-                for (int k0 = 0; k0 < KB; k0 += S::CHUNK, ++chunk) {
-                    const int c = chunk & 1, kb = k0 + lane % S::CHUNK;
-                    if (!(ok = warp_wait(&spent[c], ((chunk / 2) & 1) ^ 1))) break;
-#pragma unroll 8
-                    for (int r = lane / S::CHUNK; r < S::HALF / 2; r += 32 / S::CHUNK)
-                        row_scale[c][lane % S::CHUNK][(warp - 2) * (S::HALF / 2) + r] =
-                            kb < KB && row0 + r < t.p_rows ? t.p_scales[(row0 + r) * KB + kb] : 0.0f;
-                    if (warp == 2) {
-                        const uint64_t block = (uint64_t)tq * S::UNITS + lane / S::CHUNK;
-                        static_assert(32 / S::CHUNK == S::UNITS, "a lane for each unit's scale of each block");
-                        column_scale[c][lane % S::CHUNK][lane / S::CHUNK] =
-                            kb < KB && block * kBlock < t.q_rows ? t.q_scales[block * KB + kb] : 0.0f;
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&scaled[c]);
+                const int p0 = (int)(tp * S::BM + rank * S::HALF), q0 = (int)(tq * S::BN + rank * (S::BN / 2));
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const int s = it % S::STAGES;
+                    if (!(ok = mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1))) break;
+                    unsigned char *to = tiles + s * S::STAGE_BYTES;
+                    const uint32_t bar = cluster_address(smem_addr(&full[s]), 0);
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * S::STAGE_BYTES);  // both CTAs' loads
+                    tma_load_pair(to, &map_p, bar, kb * kBlock, p0);
+                    tma_load_pair(to + S::P_BYTES, &map_q, bar, kb * kBlock, q0);
                 }
             }
+            if (!ok) record_fault(p.status, 0, kWatchdog);
+            // Nothing is left in flight towards either CTA's shared memory when the pair ends.
+            if (rank == 0)
+                for (int i = it > S::STAGES ? it - S::STAGES : 0; i < it; ++i)
+                    mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
+        }
+    } else if (warp == 1) {
+        // The whole warp runs the loop, so that descriptors stay in uniform registers; one lane issues.
+        if (rank == 0) {
+            constexpr uint32_t shape = 1u << 23 | (uint32_t)(S::BN / 8) << 17 | (uint32_t)(S::BM / 16) << 24;
+            const uint32_t stage0 = smem_addr(tiles), exponents0 = smem_addr(exponents);
+            int it = 0, chunk = 0, tile = 0;
+            bool ok = true;
+            for (unsigned id = first; ok && id < t.tiles; id += step, ++tile) {
+                ok = __all_sync(~0u, mbar_wait_cluster(&drained, (tile & 1) ^ 1));
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int kb = 0; ok && kb < KB; ++kb, ++it) {
+                    const int s = it % S::STAGES, in = kb % S::CHUNK, c = chunk & 1;
+                    if (in == 0 && !(ok = __all_sync(~0u, mbar_acquire_cluster(&scaled[c], (chunk / 2) & 1)))) break;
+                    if (!(ok = warp_wait(&full[s], (it / S::STAGES) & 1))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t pd = k_major_descriptor(stage0 + s * S::STAGE_BYTES), qd = pd + (S::P_BYTES >> 4);
+                    const uint32_t scales = tmem + S::SCALES_AT + it % S::SCALES * S::SCALES_STEP;
+                    const uint32_t from = exponents0 + (c * S::CHUNK + in) * S::EXPONENTS;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < 1 + S::BN / 128; ++i) exponents_to_tmem(scales + 4 * i, from + 512 * i);
+#pragma unroll
+                        for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further along the swizzled rows
+                            mma_pair(tmem, pd + 2 * k, qd + 2 * k, shape, scales, scales + 4, kb > 0 || k > 0);
+                        mma_commit_pair(&empty[s]);
+                        if (in == S::CHUNK - 1 || kb == KB - 1) mma_commit_pair(&spent[c]);
+                        if (kb == KB - 1) mma_commit_pair(&ready);
+                    }
+                    __syncwarp();
+                    if (in == S::CHUNK - 1 || kb == KB - 1) ++chunk;
+                }
+            }
+            if (elect_one()) mma_commit_pair(&finished);
+            __syncwarp();
+            ok = warp_wait(&finished, 0) && ok;
             if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::DRAINING));
-        const int quarter = warp % 4, local = quarter * 32 + lane;  // this thread's row of the CTA's half
-        const int u = (warp - 4) / (S::EPILOGUE / S::UNITS);        // the unit of each block that this warp takes
-        const int from = (warp - 4) / 4 % (S::EPILOGUE / 4 / S::UNITS) * S::COLUMNS;  // its first column in it
-        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + from;
-        const uint32_t drained0 = cluster_address(smem_addr(&drained[0]), 0);
-        int unit = u, chunk = 0;
-        bool ok = true;  // after a wait that ran out nothing more is waited for, and nothing stored
+    } else if (warp < 4) {
+        // Word (r % 32) * 4 + r / 32 of a piece is row r's exponent.  A warp takes half of this CTA's rows of P,
+        // 4 rows by 8 adjacent blocks a load, and one of the two pieces of Q, whose 128 rows share a scale.
+        const int half = warp - 2, in = lane % S::CHUNK;
+        const uint32_t scaled0 = cluster_address(smem_addr(&scaled[0]), 0);
+        int chunk = 0;
+        bool ok = true;
         for (unsigned id = first; ok && id < t.tiles; id += step) {
-            uint64_t pair[S::COLUMNS / 2];  // two binary32 sums each, for two-lane multiply-adds
+            unsigned tp, tq;
+            tile_place(t, id, tp, tq);
+            const uint64_t row0 = (uint64_t)tp * S::BM + rank * S::HALF + half * (S::HALF / 2);
+            const uint64_t column_block = (uint64_t)tq * (S::BN / 128) + half;
+            for (int k0 = 0; k0 < KB; k0 += S::CHUNK, ++chunk) {
+                const int c = chunk & 1, kb = k0 + in;
+                if (!(ok = warp_wait(&spent[c], ((chunk / 2) & 1) ^ 1))) break;
+                uint32_t *slot = exponents + (c * S::CHUNK + in) * (S::EXPONENTS / 4);
 #pragma unroll
-            for (int i = 0; i < S::COLUMNS / 2; ++i) pair[i] = 0;
-#pragma unroll 1
-            for (int kb = 0; kb < KB; ++kb, unit += S::UNITS) {
-                const int c = chunk & 1, in = kb % S::CHUNK, b = unit % S::BUFFERS;
-                if (in == 0) ok = ok && warp_wait(&scaled[c], (chunk / 2) & 1);
-                const float factor = row_scale[c][in][local] * column_scale[c][in][u];
-                ok = ok && warp_wait(&ready[b], (unit / S::BUFFERS) & 1);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int h = 0; h < S::COLUMNS; h += S::PIECE) {
-                    uint32_t v[S::PIECE];
-                    tmem_load(v, lanes + b * S::UNIT + h);
-                    tmem_wait(v);
-                    if (h + S::PIECE == S::COLUMNS) {  // the unit has been read
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(drained0 + 8 * b);
-                    }
-#pragma unroll
-                    for (int i = 0; i < S::PIECE; i += 2) fma_two(pair[(h + i) / 2], v[i], v[i + 1], factor, factor);
+                for (int r = lane / S::CHUNK; r < S::HALF / 2; r += 32 / S::CHUNK) {
+                    const int local = half * (S::HALF / 2) + r;
+                    slot[local % 32 * 4 + local / 32] =
+                        exponent_word(kb < KB && row0 + r < t.p_rows ? t.p_scales[(row0 + r) * KB + kb] : 1.0f);
                 }
-                if (in == S::CHUNK - 1 || kb == KB - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&spent[c]);
-                    ++chunk;
+                const uint32_t word =
+                    exponent_word(kb < KB && column_block * kBlock < t.q_rows ? t.q_scales[column_block * KB + kb] : 1.0f);
+#pragma unroll
+                for (int b = 0; b < S::CHUNK; ++b) {
+                    const uint32_t w = __shfl_sync(~0u, word, b);
+                    uint32_t *piece = exponents + (c * S::CHUNK + b) * (S::EXPONENTS / 4) + 128 * (1 + half);
+                    reinterpret_cast<uint4 *>(piece)[lane] = make_uint4(w, w, w, w);
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // tcgen05.cp reads them
+                __syncwarp();
+                if (lane == 0) mbar_release_cluster(scaled0 + 8 * c);
             }
-            if (!ok) break;
+        }
+        if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
+    } else {
+        const int quarter = warp % 4, local = quarter * 32 + lane;  // this thread's row of the CTA's half
+        const int from = (warp - 4) / 4 * S::COLUMNS;               // its first column
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + from;
+        const uint32_t drained0 = cluster_address(smem_addr(&drained), 0);
+        int tile = 0;
+        bool ok = true;
+        for (unsigned id = first; id < t.tiles; id += step, ++tile) {
+            if (!(ok = warp_wait(&ready, tile & 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t v[S::COLUMNS / 32][32];
+#pragma unroll
+            for (int i = 0; i < S::COLUMNS / 32; ++i) tmem_load(v[i], lanes + 32 * i);
+#pragma unroll
+            for (int i = 0; i < S::COLUMNS / 32; ++i) tmem_wait(v[i]);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(drained0);  // the next tile's products may begin
             unsigned tp, tq;
             tile_place(t, id, tp, tq);
             const uint64_t row = (uint64_t)tp * S::BM + rank * S::HALF + local;
             if (row < t.p_rows) {
 #pragma unroll
-                for (int h = 0; h < S::COLUMNS; h += 16) {
-                    float sum[16];
+                for (int i = 0; i < S::COLUMNS / 32; ++i) {
+                    float sum[32];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        asm("mov.b64 {%0, %1}, %2;" : "=f"(sum[2 * i]), "=f"(sum[2 * i + 1]) : "l"(pair[h / 2 + i]));
-                    store_row<T, 16>(p, row, (uint64_t)tq * S::BN + u * S::UNIT + from + h, sum);
+                    for (int e = 0; e < 32; ++e) sum[e] = __uint_as_float(v[i][e]);
+                    store_row<T, 32>(p, row, (uint64_t)tq * S::BN + from + 32 * i, sum);
                 }
             }
         }
@@ -670,7 +669,7 @@ __global__ void __launch_bounds__(S::THREADS)
         // Lane c holds the product of both operands' scales for the tile's column c, read one block ahead.
         auto scale_of = [&](int kb) -> float {
             return kb < kb1 && lane < S::BN && (uint64_t)q0 + lane < t.q_rows
-                       ? t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb] * t.p_scales[(uint64_t)tp * t.blocks + kb]
+                       ? checked_scale(t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb]) * checked_scale(t.p_scales[(uint64_t)tp * t.blocks + kb])
                        : 0.0f;
         };
         float sum[S::BN], next = scale_of(kb0);
@@ -776,7 +775,7 @@ template <typename T> static TileParams<T> tile_params(const ProductParams<T> &p
 
 template <typename T>
 static int launch_batch(const ProductParams<T> &p, const CUtensorMap &left, const CUtensorMap &right, cudaStream_t stream) {
-    if (const int rc = pcu_host::allow_shared<product_kernel<T>>(Batch::SMEM_BYTES, Batch::LAUNCHED)) return rc;
+    if (const int rc = pcu_host::allow_shared<product_kernel<T>>(Batch::SMEM_BYTES)) return rc;
     const TileParams<T> t = tile_params(p, false, Batch::BM, Batch::BN);
     const unsigned pairs = std::min(t.tiles, (unsigned)std::max(1, pcu_host::sm_count() / 2));
     product_kernel<T><<<2 * pairs, Batch::THREADS, Batch::SMEM_BYTES, stream>>>(left, right, t);
@@ -802,7 +801,7 @@ template <typename T> static int product_typed(const ProductParams<T> &p, cudaSt
             return few ? launch_rows<T, Rows<16>>(p, left, right, stream) : launch_rows<T, Rows<32>>(p, left, right, stream);
     } else if (p.inner) {
         if (code_map(&left, p.left, p.rows, p.inner, p.left_stride, Batch::HALF) &&
-            code_map(&right, p.right, p.columns, p.inner, p.right_stride, Batch::UNIT / 2))
+            code_map(&right, p.right, p.columns, p.inner, p.right_stride, Batch::BN / 2))
             return launch_batch<T>(p, left, right, stream);
     }
     const uint64_t tiles = (p.rows + 15) / 16 * ((p.columns + 15) / 16);

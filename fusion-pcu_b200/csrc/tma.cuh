@@ -72,6 +72,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
     return bounded_wait([&] { return mbar_try_wait(bar, parity); });
 }
 
+// For memory that another CTA of the cluster hands over with a release at cluster scope.
+__device__ __forceinline__ bool mbar_acquire_cluster(uint64_t *bar, uint32_t parity) {
+    const bool ok = bounded_wait([&] { return mbar_try_wait_cluster(bar, parity); });
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    return ok;
+}
+
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
     return bounded_wait([&] { return mbar_try_wait_cluster(bar, parity); });
 }

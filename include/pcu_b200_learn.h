@@ -140,7 +140,8 @@ int pcu_b200_block_quantize(int dtype, const void *input, uint64_t rows, uint64_
  * left: rows x inner codes with scales of 1 x 128 blocks (activations); right: columns x inner codes
  * with scales of 128 x 128 blocks (a weight matrix, its output features as rows).  out is F32, F16 or
  * BF16 (out_dtype) with rows of out_stride elements.  The sums are in binary32.  inner may be 0.
- * Any finite scales are taken, not only powers of two.
+ * Scales are powers of two from 2^-126 on, as pcu_b200_block_quantize writes them (the tensor cores
+ * apply them as exponents); any other scale gives NaN in its cells.
  * Codes with 16-byte aligned bases and strides run on the tensor cores; others give the same
  * results to rounding, slowly.
  * Events: the cell row * columns + column. */

@@ -81,8 +81,8 @@ def _operands(rows, inner, columns, seed, room=None):
         stride = (inner + 15) // 16 * 16 if room is None else inner + room
         base = torch.full((v.shape[0], stride), 0x7f, dtype=torch.uint8)  # NaN between the rows
         base[:, :inner] = codes.to(torch.float8_e4m3fn).view(torch.uint8)
-        # scales that are no powers of two, as other quantisers write them
-        scales = (scales * (0.5 + torch.rand(scales.shape, generator=gen, dtype=torch.float64))).float()
+        # any powers of two, not only the quantiser's
+        scales = (scales * 2.0 ** torch.randint(-3, 4, scales.shape, generator=gen)).float()
         return base.cuda()[:, :inner].view(torch.float8_e4m3fn), scales.cuda()
 
     return lay(x, 1) + lay(w, 128)
@@ -96,11 +96,11 @@ def _exact(a, sa, b, sb):
 
 
 def _tolerance(want, size, inner, dtype):
-    """Products of codes are exact in binary32.  A block's 128 products are added in any order (127 u of
-    their magnitudes; the tensor cores align a few at a time to 2^-24 of the largest or finer, which
-    127 u covers too), the scales' product rounds, and the blocks are added one by one."""
-    blocks = -(-inner // 128)
-    return size * (127 + 3 + blocks) * lu.u(torch.float32) + lu.u(dtype) * want.abs() * 1.01 + \
+    """Products of codes are exact in binary32, and so is a power of two times them.  The sums are in
+    binary32: a group of 32 products in any order (31 u of their magnitudes; the tensor cores align them to
+    2^-24 of the largest or finer, which that covers too), the groups one by one."""
+    groups = -(-inner // 32)
+    return size * (31 + 1 + groups) * lu.u(torch.float32) + lu.u(dtype) * want.abs() * 1.01 + \
         torch.finfo(dtype).smallest_normal
 
 
@@ -164,10 +164,35 @@ def test_faults(provider, rows):
     assert bool(torch.isnan(out[at]).all()) and int(torch.isnan(out).sum()) == 260
     a, sa, b, sb = _operands(rows, 500, 260, 2)
     status = provider.new_status()
-    sb = sb.clone()
-    sb[1] = 1e30
-    out = provider.block_matmul(a, sa * 1e3, b, sb * 1e5, dtype=torch.float16, status=status)
+    out = provider.block_matmul(a, sa * 2.0 ** 10, b, sb * 2.0 ** 16, dtype=torch.float16, status=status)
     assert provider.decode_status(status_word(status))[1] == 3
+
+
+@pytest.mark.parametrize("rows,room", [(1, None), (20, None), (300, None), (5, 3)])
+def test_a_scale_that_is_no_power_of_two_gives_nan(provider, rows, room):
+    for bad in (3.0, 0.0, -1.0, 2.0 ** -127, math.inf, math.nan, 1.0000001):
+        a, sa, b, sb = _operands(rows, 500, 260, 3, room)
+        sa[rows // 2, 3] = bad
+        status = provider.new_status()
+        out = provider.block_matmul(a, sa, b, sb, dtype=torch.float32, status=status)
+        assert bool(torch.isnan(out[rows // 2]).all()) and int(torch.isnan(out).sum()) == 260
+        assert provider.decode_status(status_word(status)) == (rows // 2 * 260, 5)
+        a, sa, b, sb = _operands(rows, 500, 260, 3, room)
+        sb[1, 2] = bad
+        status = provider.new_status()
+        out = provider.block_matmul(a, sa, b, sb, dtype=torch.float32, status=status)
+        assert bool(torch.isnan(out[:, 128:256]).all()) and int(torch.isnan(out).sum()) == 128 * rows
+        assert provider.decode_status(status_word(status)) == (128, 5)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_large_and_small_scales(provider, rows):
+    """Scales far from 1 whose products are not: exact powers of two."""
+    a, sa, b, sb = _operands(rows, 300, 200, 5)
+    want = provider.block_matmul(a, sa, b, sb, dtype=torch.float32)
+    for e in (100, -100):
+        got = provider.block_matmul(a, sa * 2.0 ** e, b, sb * 2.0 ** -e, dtype=torch.float32)
+        assert torch.equal(got, want)
 
 
 def test_empty(provider):
