@@ -158,25 +158,30 @@ template <typename T> __device__ __forceinline__ void store_cell(const ProductPa
     if (const unsigned kind = result_kind(Elem<T>::load(y))) record_fault(p.status, r * p.columns + c, kind);
 }
 
-// COLUMNS cells of one row from `column` on, in 16-byte pieces where the row allows it.
+// COLUMNS cells of one row from `column` on, in 32-byte pieces (whole sectors: a warp's lanes are in 32
+// rows) where the row allows it.
 template <typename T, int COLUMNS>
 __device__ __forceinline__ void store_row(const ProductParams<T> &p, uint64_t row, uint64_t column,
-                                          const float (&v)[COLUMNS]) {
-    constexpr int V = 16 / sizeof(T);
+                                          const uint32_t (&v)[COLUMNS]) {
+    constexpr int V = 32 / sizeof(T);
+    static_assert(COLUMNS % V == 0, "whole pieces");
     T *to = p.out + row * p.out_stride + column;
-    const bool whole = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+    const bool whole = (reinterpret_cast<uintptr_t>(to) & 31) == 0;
 #pragma unroll
     for (int i = 0; i < COLUMNS; i += V) {
         if (column + i >= p.columns) break;
-        alignas(16) T y[V];
+        alignas(32) T y[V];
         bool fine = true;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            y[j] = Elem<T>::round(v[i + j]);
-            fine &= isfinite(Elem<T>::load(y[j])) || column + i + j >= p.columns;
+            y[j] = Elem<T>::round(__uint_as_float(v[i + j]));
+            fine &= isfinite(Elem<T>::load(y[j]));
         }
         if (whole && column + i + V <= p.columns) {
-            *reinterpret_cast<uint4 *>(to + i) = *reinterpret_cast<const uint4 *>(y);
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(y);
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + i), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -332,19 +337,21 @@ __device__ __forceinline__ void tile_place(const TileParams<T> &t, unsigned id, 
 // 32 codes: a block's byte four times) and sum over all blocks in TMEM.  Scales of any kind had to be
 // applied in registers, a block's product at a time: that drained 256 KB of TMEM per pair and block, and
 // ran at 36 % of the tensor cores' rate (165 us for 8192 x 4096 x 4096) however the drain was spread.
+// With so few tiles that a quarter of the SMs would do, tiles of 256 x 64 (see product_typed).
 // Warps: 0 TMA loads, 1 tcgen05.cp of the exponents and tcgen05.mma (first CTA only), 2 and 3 exponents
 // into shared memory, 4 to 11 bring the sums to registers, 128 columns each, give TMEM back and store.
-struct Batch {
-    static constexpr int HALF = 128, BM = 2 * HALF, BN = 256;
+template <int BN_> struct Batch {
+    static constexpr int HALF = 128, BM = 2 * HALF, BN = BN_;
+    static constexpr int PIECES = (BN + 127) / 128;  // of 128 columns, or one of fewer
     static constexpr int EPILOGUE = 8, COLUMNS = BN / (EPILOGUE / 4), THREADS = (4 + EPILOGUE) * 32;
     static constexpr int P_BYTES = HALF * kBlock, Q_BYTES = BN / 2 * kBlock, STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int STAGES = 6;
     // exponents: 512 bytes per 128 rows and block, CHUNK blocks at a time, two chunks
-    static constexpr int CHUNK = 8, EXPONENTS = 512 * (1 + BN / 128);
+    static constexpr int CHUNK = 8, EXPONENTS = 512 * (1 + PIECES);
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * CHUNK * EXPONENTS + 1024;
     // TMEM columns: the sums, then the exponents of four blocks (4 columns per 128 rows)
     static constexpr int TMEM_COLUMNS = 512, SCALES_AT = BN, SCALES_STEP = 16, SCALES = 4;
-    static_assert(SCALES_AT + SCALES * SCALES_STEP <= TMEM_COLUMNS && 4 * (1 + BN / 128) <= SCALES_STEP, "TMEM");
+    static_assert(SCALES_AT + SCALES * SCALES_STEP <= TMEM_COLUMNS && 4 * (1 + PIECES) <= SCALES_STEP, "TMEM");
 };
 
 // A load by either CTA of a pair that signals the first CTA's barrier.
@@ -400,11 +407,10 @@ __device__ __forceinline__ uint32_t exponent_word(float scale) {
     return ((bits & 0x807fffffu) == 0 && e >= 1 && e <= 254 ? e : 0xffu) * 0x01010101u;
 }
 
-template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
+template <typename T, typename S>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(S::THREADS, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ TileParams<T> t) {
-    using S = Batch;
     const ProductParams<T> &p = t.out;
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ unsigned char smem_raw[];
@@ -479,7 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
                     const uint32_t from = exponents0 + (c * S::CHUNK + in) * S::EXPONENTS;
                     if (elect_one()) {
 #pragma unroll
-                        for (int i = 0; i < 1 + S::BN / 128; ++i) exponents_to_tmem(scales + 4 * i, from + 512 * i);
+                        for (int i = 0; i < 1 + S::PIECES; ++i) exponents_to_tmem(scales + 4 * i, from + 512 * i);
 #pragma unroll
                         for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further along the swizzled rows
                             mma_pair(tmem, pd + 2 * k, qd + 2 * k, shape, scales, scales + 4, kb > 0 || k > 0);
@@ -498,7 +504,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
         }
     } else if (warp < 4) {
         // Word (r % 32) * 4 + r / 32 of a piece is row r's exponent.  A warp takes half of this CTA's rows of P,
-        // 4 rows by 8 adjacent blocks a load, and one of the two pieces of Q, whose 128 rows share a scale.
+        // 4 rows by 8 adjacent blocks a load, and one piece of Q, whose rows share a scale.
         const int half = warp - 2, in = lane % S::CHUNK;
         const uint32_t scaled0 = cluster_address(smem_addr(&scaled[0]), 0);
         int chunk = 0;
@@ -507,7 +513,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
             unsigned tp, tq;
             tile_place(t, id, tp, tq);
             const uint64_t row0 = (uint64_t)tp * S::BM + rank * S::HALF + half * (S::HALF / 2);
-            const uint64_t column_block = (uint64_t)tq * (S::BN / 128) + half;
+            const uint64_t column_block = (uint64_t)tq * S::BN / 128 + half;
             for (int k0 = 0; k0 < KB; k0 += S::CHUNK, ++chunk) {
                 const int c = chunk & 1, kb = k0 + in;
                 if (!(ok = warp_wait(&spent[c], ((chunk / 2) & 1) ^ 1))) break;
@@ -521,7 +527,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
                 const uint32_t word =
                     exponent_word(kb < KB && column_block * kBlock < t.q_rows ? t.q_scales[column_block * KB + kb] : 1.0f);
 #pragma unroll
-                for (int b = 0; b < S::CHUNK; ++b) {
+                for (int b = 0; b < S::CHUNK && half < S::PIECES; ++b) {
                     const uint32_t w = __shfl_sync(~0u, word, b);
                     uint32_t *piece = exponents + (c * S::CHUNK + b) * (S::EXPONENTS / 4) + 128 * (1 + half);
                     reinterpret_cast<uint4 *>(piece)[lane] = make_uint4(w, w, w, w);
@@ -555,12 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Batch::THREADS, 1)
             const uint64_t row = (uint64_t)tp * S::BM + rank * S::HALF + local;
             if (row < t.p_rows) {
 #pragma unroll
-                for (int i = 0; i < S::COLUMNS / 32; ++i) {
-                    float sum[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) sum[e] = __uint_as_float(v[i][e]);
-                    store_row<T, 32>(p, row, (uint64_t)tq * S::BN + from + 32 * i, sum);
-                }
+                for (int i = 0; i < S::COLUMNS / 32; ++i) store_row<T, 32>(p, row, (uint64_t)tq * S::BN + from + 32 * i, v[i]);
             }
         }
         if (!ok && lane == 0) record_fault(p.status, 0, kWatchdog);
@@ -773,12 +774,12 @@ template <typename T> static TileParams<T> tile_params(const ProductParams<T> &p
     return t;
 }
 
-template <typename T>
+template <typename T, typename S>
 static int launch_batch(const ProductParams<T> &p, const CUtensorMap &left, const CUtensorMap &right, cudaStream_t stream) {
-    if (const int rc = pcu_host::allow_shared<product_kernel<T>>(Batch::SMEM_BYTES)) return rc;
-    const TileParams<T> t = tile_params(p, false, Batch::BM, Batch::BN);
+    if (const int rc = pcu_host::allow_shared<product_kernel<T, S>>(S::SMEM_BYTES)) return rc;
+    const TileParams<T> t = tile_params(p, false, S::BM, S::BN);
     const unsigned pairs = std::min(t.tiles, (unsigned)std::max(1, pcu_host::sm_count() / 2));
-    product_kernel<T><<<2 * pairs, Batch::THREADS, Batch::SMEM_BYTES, stream>>>(left, right, t);
+    product_kernel<T, S><<<2 * pairs, S::THREADS, S::SMEM_BYTES, stream>>>(left, right, t);
     return pcu_host::launch_status();
 }
 
@@ -800,9 +801,12 @@ template <typename T> static int product_typed(const ProductParams<T> &p, cudaSt
             code_map(&left, p.left, p.rows, p.inner, p.left_stride, few ? 16 : 32))
             return few ? launch_rows<T, Rows<16>>(p, left, right, stream) : launch_rows<T, Rows<32>>(p, left, right, stream);
     } else if (p.inner) {
-        if (code_map(&left, p.left, p.rows, p.inner, p.left_stride, Batch::HALF) &&
-            code_map(&right, p.right, p.columns, p.inner, p.right_stride, Batch::BN / 2))
-            return launch_batch<T>(p, left, right, stream);
+        // Tiles of 256 x 64 while all of them run at once: each takes some 0.6 of a 256 x 256 tile's time.
+        const uint64_t narrow = (p.rows + 255) / 256 * ((p.columns + 63) / 64);
+        const bool few = narrow <= (uint64_t)pcu_host::sm_count() / 2;
+        if (code_map(&left, p.left, p.rows, p.inner, p.left_stride, 128) &&
+            code_map(&right, p.right, p.columns, p.inner, p.right_stride, few ? 32 : 128))
+            return few ? launch_batch<T, Batch<64>>(p, left, right, stream) : launch_batch<T, Batch<256>>(p, left, right, stream);
     }
     const uint64_t tiles = (p.rows + 15) / 16 * ((p.columns + 15) / 16);
     product_plain_kernel<T><<<(unsigned)tiles, 256, 0, stream>>>(p);
