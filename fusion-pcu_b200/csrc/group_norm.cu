@@ -419,7 +419,7 @@ template <typename T, int V, int TENSORS> struct Slab {
         for (int t = 0; t < TENSORS; ++t)
             mine[t] = reinterpret_cast<T *>(smem + t * plan.slab_bytes) + (ty * across + tx) * V;
         scratch = reinterpret_cast<W *>(smem + TENSORS * plan.slab_bytes);
-        total = scratch + TENSORS * blockDim.x * V;
+        total = scratch + 2 * blockDim.x * V;
         joined = total + 2 * plan.block_groups;
     }
     __device__ __forceinline__ uint64_t channel() const { return c0 + (uint64_t)tx * V; }
@@ -485,6 +485,73 @@ template <typename T, int V, int TENSORS> struct Slab {
         }
         __syncthreads();
     }
+    // Rows that the cluster's r-th CTA holds.
+    __device__ __forceinline__ uint64_t rows_of(uint32_t r, const NormParams<T> &p) const {
+        const uint64_t from = (uint64_t)r * p.plan.slab_rows;
+        return from < p.positions ? min((uint64_t)p.plan.slab_rows, p.positions - from) : 0;
+    }
+    // Each thread's (mean, sum of squares about it) of its `count` rows of each channel, joined over the
+    // rows' threads, each group's channels and the cluster's CTAs to joined[g] (mean) and
+    // joined[block_groups + g] (variance); squares are always about the joint means.
+    __device__ __forceinline__ void moments(const W (&mean)[V], const W (&square)[V], const NormParams<T> &p) const {
+        const int wide = across * V;
+        const unsigned bg = p.plan.block_groups;
+        W *means = scratch, *squares = scratch + deep * wide;
+        if (active)
+#pragma unroll
+            for (int e = 0; e < V; ++e) means[ty * wide + tx * V + e] = mean[e], squares[ty * wide + tx * V + e] = square[e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < wide && rows; c += blockDim.x) {
+            // the first `longer` threads of a column have one row more than the others
+            const W few = (W)(rows / deep);
+            const int longer = rows % deep;
+            W all = 0, spread = 0;
+            for (int d = 0; d < deep; ++d) all += (d < longer ? few + W(1) : few) * means[d * wide + c];
+            all /= (W)rows;
+            for (int d = 0; d < deep; ++d) {
+                const W off = means[d * wide + c] - all, n = d < longer ? few + W(1) : few;
+                if (n > W(0)) spread += squares[d * wide + c] + n * off * off;
+            }
+            means[c] = all, squares[c] = spread;  // the first row's places: only this thread reads them
+        }
+        __syncthreads();
+        for (int g = threadIdx.x / 32; g < groups; g += blockDim.x / 32) {
+            W all = 0, spread = 0;
+            for (int d = threadIdx.x % 32; d < width && rows; d += 32) all += means[g * width + d];
+            for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
+            all /= (W)width;
+            for (int d = threadIdx.x % 32; d < width && rows; d += 32) {
+                const W off = means[g * width + d] - all;
+                spread += squares[g * width + d] + (W)rows * off * off;
+            }
+            for (int o = 16; o; o >>= 1) spread += __shfl_xor_sync(~0u, spread, o);
+            if (threadIdx.x % 32 == 0) total[g] = all, total[bg + g] = spread;
+        }
+        if (ranks > 1) cluster_sync();
+        else __syncthreads();
+        const W inverse = W(1) / (W)p.positions;
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+            W all = total[g], spread = total[bg + g];
+            if (ranks > 1) {
+                all = 0, spread = 0;
+                for (uint32_t r = 0; r < ranks; ++r) {
+                    W other;
+                    cluster_read(other, smem_addr(total + g), r);
+                    all += (W)rows_of(r, p) * other;
+                }
+                all *= inverse;
+                for (uint32_t r = 0; r < ranks; ++r) {
+                    W other, more;
+                    cluster_read(other, smem_addr(total + g), r);
+                    cluster_read(more, smem_addr(total + bg + g), r);
+                    other -= all;
+                    spread += more + (W)rows_of(r, p) * (W)width * other * other;
+                }
+            }
+            joined[g] = all, joined[bg + g] = spread * inverse / (W)width;
+        }
+        __syncthreads();
+    }
     // a quantity's joint sum for each channel of this thread's access
     __device__ __forceinline__ void sums_of(int slot, unsigned block_groups, W (&v)[V]) const {
         int g = tx * V / width, left = (g + 1) * width - tx * V;
@@ -502,54 +569,58 @@ template <typename T, int V> __global__ void __launch_bounds__(512, sizeof(WideO
     extern __shared__ __align__(16) unsigned char smem[];
     Slab<T, V, 1> at;
     at.place(p, smem);
-    at.bring(0, p.x);
     const uint64_t c = at.channel();
     const unsigned bg = p.plan.block_groups;
-    const W inverse = W(1) / ((W)p.positions * (W)p.width);
-    auto same = [](int, int, W v) { return v; };
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    W v[1][V] = {}, x[V], mean[V] = {}, r[V], w[V], b[V];
+    W mean[V] = {}, r[V] = {};
     const int step = at.step();
-    if (at.active) {
+    at.bring(0, p.x);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    // Sums about the thread's first row: with few rows a thread, even a far first element costs them no
+    // digits that count.
+    if (at.active && at.ty < at.rows) {
         const T *from = at.mine[0];
-        for (int i = at.ty; i < at.rows; i += at.deep, from += step) {
+        W first[V], x[V];
+        at.read(from, first);
+        int count = 1;
+        for (int i = at.ty + at.deep; i < at.rows; i += at.deep, ++count) {
+            from += step;
             at.read(from, x);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[0][e] += x[e];
+            for (int e = 0; e < V; ++e) {
+                const W d = x[e] - first[e];
+                mean[e] += d;
+                r[e] += d * d;
+            }
+        }
+        const W inverse = W(1) / (W)count;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const W shift = mean[e] * inverse;
+            r[e] -= mean[e] * shift;
+            mean[e] = first[e] + shift;
         }
     }
-    at.sum(v, 0, bg, same);
-    if (at.active) at.sums_of(0, bg, mean);
-#pragma unroll
-    for (int e = 0; e < V; ++e) mean[e] *= inverse, v[0][e] = W(0);
-    if (at.active) {
-        const T *from = at.mine[0];
-        for (int i = at.ty; i < at.rows; i += at.deep, from += step) {
-            at.read(from, x);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[0][e] += (x[e] - mean[e]) * (x[e] - mean[e]);
-        }
-    }
-    at.sum(v, 1, bg, same);
+    at.moments(mean, r, p);
     if (at.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // read; see the end
     if (at.rank == 0)
         for (int g = threadIdx.x; g < at.groups; g += blockDim.x) {
             W *to = p.stats_out + 2 * (at.n * p.groups + at.c0 / p.width + g);
-            to[0] = at.joined[g] * inverse;
-            to[1] = root(at.joined[bg + g] * inverse, p.eps);
+            to[0] = at.joined[g];
+            to[1] = root(at.joined[bg + g], p.eps);
         }
     if (at.active) {
+        W w[V], b[V], x[V];
         parameters<V>(p.weight, c, W(1), w), parameters<V>(p.bias, c, W(0), b);
-        at.sums_of(1, bg, r);
+        at.sums_of(0, bg, mean), at.sums_of(1, bg, r);
 #pragma unroll
-        for (int e = 0; e < V; ++e) r[e] = root(r[e] * inverse, p.eps);
+        for (int e = 0; e < V; ++e) w[e] *= root(r[e], p.eps);
         const T *from = at.mine[0];
         T *to = p.out.at(at.n, at.s0 + at.ty, c);
         const uint64_t stride = at.deep * p.out.row;
         for (int i = at.ty; i < at.rows; i += at.deep, from += step, to += stride) {
             at.read(from, x);
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = (x[e] - mean[e]) * r[e] * w[e] + b[e];
+            for (int e = 0; e < V; ++e) x[e] = (x[e] - mean[e]) * w[e] + b[e];
             activate<V>(p.activation, x);
             put<T, V>(to, x, p.status, [&] { return (at.n * p.positions + at.s0 + i) * p.channels + c; });
         }
@@ -929,8 +1000,11 @@ NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, ui
         return p;
     }
     // Slab form: blocks of whole groups whose rows are at least 128 bytes and whole accesses.  The smallest
-    // cluster whose slabs are at most 64 KB (three CTAs per SM overlap loading, sums and stores), or 200 KB in
-    // a cluster of 8; more CTAs, down to 16 KB each, when they do not fill the SMs twice.
+    // cluster whose CTAs hold at most 84 KB, so that two share an SM and overlap loading, sums and stores
+    // while their threads have some ten rows each to earn their set-up (48 KB: 158 against 131 us at 16 x
+    // 4095 x 1280 BF16 forward, 164 against 122 us at 32 x 1024 x 1280 backward), or 200 KB in a cluster of 8; more
+    // CTAs, down to 16 KB each, when they do not fill the SMs twice.
+    const uint64_t most = 84 * 1024;
     const uint64_t tensors = backward ? 2 : 1;
     const uint64_t step = (uint64_t)vector / std::gcd(width, (uint64_t)vector);
     auto try_slab = [&](uint64_t block) {
@@ -939,12 +1013,12 @@ NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, ui
         if (across > 512 || block * width % vector != 0) return false;
         const uint64_t row = block * width * bytes * tensors;
         uint64_t ranks = 1;
-        while (ranks < 8 && (positions + ranks - 1) / ranks * row > 65536) ranks *= 2;
+        while (ranks < 8 && (positions + ranks - 1) / ranks * row > most) ranks *= 2;
         const uint64_t blocks = (groups + block - 1) / block;
         while (ranks < 8 && batch * blocks * ranks < 2 * sms && (positions + ranks - 1) / ranks * row > 16384) ranks *= 2;
         const uint64_t rows = (positions + ranks - 1) / ranks;
-        const uint64_t threads = across > 256 || (!backward && batch * blocks * ranks <= 2 * sms) ? 512 : 256;
-        const uint64_t extra = tensors * threads * vector * wide + 4 * block * wide + 64;
+        const uint64_t threads = across > 256 ? 512 : 256;
+        const uint64_t extra = 2 * threads * vector * wide + 4 * block * wide + 64;
         if (rows > 0x7fffffffull || rows * row + extra + 64 > kSlabMost || batch * blocks * ranks > 0x7fffffffull) return false;
         p.form = NormPlan::kSlab;
         p.block_groups = (unsigned)block;
