@@ -419,7 +419,7 @@ template <typename T, int V, int TENSORS> struct Slab {
         for (int t = 0; t < TENSORS; ++t)
             mine[t] = reinterpret_cast<T *>(smem + t * plan.slab_bytes) + (ty * across + tx) * V;
         scratch = reinterpret_cast<W *>(smem + TENSORS * plan.slab_bytes);
-        total = scratch + 2 * blockDim.x * V;
+        total = scratch + 2 * blockDim.x * (V + 1);
         joined = total + 2 * plan.block_groups;
     }
     __device__ __forceinline__ uint64_t channel() const { return c0 + (uint64_t)tx * V; }
@@ -490,42 +490,78 @@ template <typename T, int V, int TENSORS> struct Slab {
         const uint64_t from = (uint64_t)r * p.plan.slab_rows;
         return from < p.positions ? min((uint64_t)p.plan.slab_rows, p.positions - from) : 0;
     }
-    // Each thread's (mean, sum of squares about it) of its `count` rows of each channel, joined over the
-    // rows' threads, each group's channels and the cluster's CTAs to joined[g] (mean) and
-    // joined[block_groups + g] (variance); squares are always about the joint means.
-    __device__ __forceinline__ void moments(const W (&mean)[V], const W (&square)[V], const NormParams<T> &p) const {
-        const int wide = across * V;
+    // Each thread's (mean, sum of squares about it) of its rows of each channel, joined over the rows'
+    // threads, each group's channels and the cluster's CTAs to joined[g] (mean) and joined[block_groups + g]
+    // (variance); squares are always about the joint means.  U: units per thread, its channels one by one, or
+    // (1) all of them together where they are in one group.
+    template <int U> __device__ __forceinline__ void moments(W (&mean)[V], W (&square)[V], const NormParams<T> &p) const {
+        constexpr int C = V / U;  // channels per unit
+        const int wide = across * U, long_group = width / C;
         const unsigned bg = p.plan.block_groups;
+        // the first `longer` threads of a column have one row more than the others
+        const W few = (W)(rows / deep);
+        const int longer = rows % deep;
         W *means = scratch, *squares = scratch + deep * wide;
+        if (C > 1) {  // every channel has the same number of rows
+            W all = 0, spread = 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) all += mean[e];
+            all *= W(1) / W(C);
+#pragma unroll
+            for (int e = 0; e < V; ++e) spread += square[e] + (ty < longer ? few + W(1) : few) * (mean[e] - all) * (mean[e] - all);
+            mean[0] = all, square[0] = spread;
+        }
         if (active)
 #pragma unroll
-            for (int e = 0; e < V; ++e) means[ty * wide + tx * V + e] = mean[e], squares[ty * wide + tx * V + e] = square[e];
+            for (int u = 0; u < U; ++u) means[ty * wide + tx * U + u] = mean[u], squares[ty * wide + tx * U + u] = square[u];
         __syncthreads();
-        for (int c = threadIdx.x; c < wide && rows; c += blockDim.x) {
-            // the first `longer` threads of a column have one row more than the others
-            const W few = (W)(rows / deep);
-            const int longer = rows % deep;
-            W all = 0, spread = 0;
-            for (int d = 0; d < deep; ++d) all += (d < longer ? few + W(1) : few) * means[d * wide + c];
-            all /= (W)rows;
-            for (int d = 0; d < deep; ++d) {
-                const W off = means[d * wide + c] - all, n = d < longer ? few + W(1) : few;
-                if (n > W(0)) spread += squares[d * wide + c] + n * off * off;
+        // With a unit per channel, first a thread per channel and part of the rows' threads.
+        int levels = deep, each = 1;
+        auto rows_in = [&](int level) {  // rows of a level's threads
+            const int from = min(deep, level * each), to = min(deep, from + each);
+            return (W)(to - from) * few + (W)(min(to, longer) - min(from, longer));
+        };
+        if (C == 1) {
+            levels = max(1, min(deep, (int)blockDim.x / wide)), each = (deep + levels - 1) / levels;
+            W *part_mean = scratch + 2 * deep * wide, *part_square = part_mean + levels * wide;
+            for (int i = threadIdx.x; i < levels * wide; i += blockDim.x) {
+                const int part = i / wide, c = i - part * wide, from = min(deep, part * each), to = min(deep, from + each);
+                const W n = rows_in(part);
+                W all = 0, spread = 0;
+#pragma unroll 4
+                for (int d = from; d < to; ++d) all += (d < longer ? few + W(1) : few) * means[d * wide + c];
+                if (n > W(0)) all /= n;
+#pragma unroll 4
+                for (int d = from; d < to; ++d) {
+                    const W off = means[d * wide + c] - all, m = d < longer ? few + W(1) : few;
+                    if (m > W(0)) spread += squares[d * wide + c] + m * off * off;
+                }
+                part_mean[i] = all, part_square[i] = spread;
             }
-            means[c] = all, squares[c] = spread;  // the first row's places: only this thread reads them
+            means = part_mean, squares = part_square;
+            __syncthreads();
         }
-        __syncthreads();
+        // Then a warp per group over its levels x units, 32 at a time.
+        const int lane = threadIdx.x % 32, down = 32 / long_group, right = 32 % long_group;
         for (int g = threadIdx.x / 32; g < groups; g += blockDim.x / 32) {
+            const W *gm = means + g * long_group, *gs = squares + g * long_group;
             W all = 0, spread = 0;
-            for (int d = threadIdx.x % 32; d < width && rows; d += 32) all += means[g * width + d];
+            for (int level = lane / long_group, i = lane % long_group; level < levels;) {
+                const W n = rows_in(level);
+                if (n > W(0)) all += n * gm[level * wide + i];
+                level += down, i += right;
+                if (i >= long_group) i -= long_group, ++level;
+            }
             for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
-            all /= (W)width;
-            for (int d = threadIdx.x % 32; d < width && rows; d += 32) {
-                const W off = means[g * width + d] - all;
-                spread += squares[g * width + d] + (W)rows * off * off;
+            if (rows) all /= (W)rows * (W)long_group;
+            for (int level = lane / long_group, i = lane % long_group; level < levels;) {
+                const W n = rows_in(level), off = gm[level * wide + i] - all;
+                if (n > W(0)) spread += gs[level * wide + i] + W(C) * n * off * off;
+                level += down, i += right;
+                if (i >= long_group) i -= long_group, ++level;
             }
             for (int o = 16; o; o >>= 1) spread += __shfl_xor_sync(~0u, spread, o);
-            if (threadIdx.x % 32 == 0) total[g] = all, total[bg + g] = spread;
+            if (lane == 0) total[g] = all, total[bg + g] = spread;
         }
         if (ranks > 1) cluster_sync();
         else __syncthreads();
@@ -600,7 +636,8 @@ template <typename T, int V> __global__ void __launch_bounds__(512, sizeof(WideO
             mean[e] = first[e] + shift;
         }
     }
-    at.moments(mean, r, p);
+    if (at.width % V == 0) at.template moments<1>(mean, r, p);
+    else at.template moments<V>(mean, r, p);
     if (at.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // read; see the end
     if (at.rank == 0)
         for (int g = threadIdx.x; g < at.groups; g += blockDim.x) {
@@ -1018,7 +1055,7 @@ NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, ui
         while (ranks < 8 && batch * blocks * ranks < 2 * sms && (positions + ranks - 1) / ranks * row > 16384) ranks *= 2;
         const uint64_t rows = (positions + ranks - 1) / ranks;
         const uint64_t threads = across > 256 ? 512 : 256;
-        const uint64_t extra = 2 * threads * vector * wide + 4 * block * wide + 64;
+        const uint64_t extra = 2 * threads * (vector + 1) * wide + 4 * block * wide + 64;
         if (rows > 0x7fffffffull || rows * row + extra + 64 > kSlabMost || batch * blocks * ranks > 0x7fffffffull) return false;
         p.form = NormPlan::kSlab;
         p.block_groups = (unsigned)block;
