@@ -26,6 +26,7 @@ template <typename T> struct DistillParams {
     int k;
     const W *weights;
     W temperature, to_log2;  // T and log2(e) / T
+    double t_inverse;
     W *loss;                 // null: gradient only
     W *stats_out;            // may be null
     const W *stats_in;       // gradient only
@@ -271,51 +272,47 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     const int chunks = (granules * 16 + kChunk - 1) / kChunk;
     T *g = p.gradient ? p.gradient + row * p.gradient_stride : nullptr;
     const W weight = p.weights ? p.weights[row] : W(1), c = p.to_log2;
-    const double t_inverse = 1.0 / (double)p.temperature;
+    const double t_inverse = p.t_inverse;
 
+    // First of all the slice is sent for (whole granules by bulk copies), and the first 256 of the teacher's
+    // entries, which are looked at while the slice is on its way.
+    int64_t index = -1;
+    W top_logit = 0;
+    if (tid < p.k) index = p.indices[row * p.k + tid], top_logit = p.top[row * p.k + tid];
     if (tid == 0) {
         for (int i = 0; i < chunks; ++i) mbar_init(&landed[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         repeated = 0;
     }
-    // the teacher's entries: exponents t / T, -infinity for absent ones
-    double a_max = -INFINITY;
-    int flags = 0;  // 1: an entry is present, 2: one is bad
-    for (int j = tid; j < p.k; j += kDistillThreads) {
-        const int64_t at = p.indices[row * p.k + j];
-        const double t = (double)p.top[row * p.k + j];
-        bool there = at >= 0 && t != -INFINITY;
-        if (there && (at >= vocab || !isfinite(t))) flags |= 2, there = false;
-        place[j] = there ? (int)at : -1;
-        prob[j] = there ? t * t_inverse : -INFINITY;
-        if (there) flags |= 1;
-        a_max = fmax(a_max, prob[j]);
-    }
     for (int j = tid; j < p.claims; j += kDistillThreads) claimed[j] = -1;
-    if (tid < V) {  // the elements of cut granules; whole ones come by bulk copies below
+    if (tid < V) {  // the elements of cut granules
         const W absent = -INFINITY;
         if (lead) slice[tid] = tid < lead || tid - lead >= count ? Elem<T>::round(absent) : z[v0 + tid - lead];
         const int at = whole1 * V + tid;
         if (whole1 < granules && (whole1 > 0 || !lead))
             slice[at] = at - lead < count ? z[v0 + at - lead] : Elem<T>::round(absent);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) a_max = fmax(a_max, __shfl_xor_sync(~0u, a_max, o));
-    flags = __reduce_or_sync(~0u, flags);
-    if (lane == 0) part_a[warp] = a_max, part_flags[warp] = flags;
     __syncthreads();
-    a_max = part_a[0], flags = part_flags[0];
+    auto fill = [&](T *to, W value) {  // the slice's part of a row
+        const T each = Elem<T>::round(value);
+        alignas(16) T many[V];
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) a_max = fmax(a_max, part_a[i]), flags |= part_flags[i];
-    if (weight == W(0) || !flags) {  // nothing to learn from
+        for (int e = 0; e < V; ++e) many[e] = each;
+        const int odd = (int)((16 - reinterpret_cast<uintptr_t>(to + v0) % 16) % 16 / sizeof(T));
+        const int head = min(count, odd), body = (count - head) / V;
+        for (int i = tid; i < body; i += kDistillThreads)
+            __stcs(reinterpret_cast<uint4 *>(to + v0 + head) + i, *reinterpret_cast<const uint4 *>(many));
+        if (tid < head) to[v0 + tid] = each;
+        if (tid < count - head - body * V) to[v0 + head + body * V + tid] = each;
+    };
+    auto nothing_to_learn = [&] {
         if (tid == 0 && rank == 0) {
             if (p.loss) p.loss[row] = W(0);
             if (p.stats_out) p.stats_out[2 * row] = W(0), p.stats_out[2 * row + 1] = W(1);
         }
-        if (g)
-            for (int v = v0 + tid; v < v1; v += kDistillThreads) g[v] = Elem<T>::round(W(0));
-        return;  // every CTA of the cluster
-    }
+        if (g) fill(g, W(0));
+    };
+    if (weight == W(0)) return nothing_to_learn();  // in every CTA of the cluster
     if (tid == 0)
         for (int i = 0; i < chunks; ++i) {
             const int a = max(whole0, i * (kChunk / 16)), b = min(whole1, (i + 1) * (kChunk / 16));
@@ -327,36 +324,61 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
             }
         }
 
-    // While the slice is on its way, the sums over the entries, with e_j = exp(a_j - a_max):
+    // the teacher's entries: exponents t / T, -infinity for absent ones.  (One copy of the code for all of
+    // them: what is not in the instruction cache comes slowly while the memory is busy.)
+    double a_max = -INFINITY;
+    int flags = 0;  // 1: an entry is present, 2: one is bad
+#pragma unroll 1
+    for (int j = tid; j < p.k; j += kDistillThreads) {
+        if (j >= kDistillThreads) index = p.indices[row * p.k + j], top_logit = p.top[row * p.k + j];
+        const double t = (double)top_logit;
+        bool there = index >= 0 && t != -INFINITY;
+        if (there && (index >= vocab || !isfinite(t))) flags |= 2, there = false;
+        if (there) flags |= 1;
+        place[j] = there ? (int)index : -1;
+        prob[j] = there ? t * t_inverse : -INFINITY;
+        a_max = fmax(a_max, prob[j]);
+    }
+    if (p.k > 32 * warp) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) a_max = fmax(a_max, __shfl_xor_sync(~0u, a_max, o));
+        flags = __reduce_or_sync(~0u, flags);
+    }
+    if (lane == 0) part_a[warp] = a_max, part_flags[warp] = flags;
+    __syncthreads();
+    a_max = part_a[0], flags = part_flags[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) a_max = fmax(a_max, part_a[i]), flags |= part_flags[i];
+    if (!flags) {  // in every CTA of the cluster
+        nothing_to_learn();
+        if (tid == 0)
+            for (int i = 0; i < chunks; ++i) mbar_wait(&landed[i], 0);  // nothing is left in flight
+        return;
+    }
+
+    // The sums over the entries, with e_j = exp(a_j - a_max):
     //   mass = sum e_j, lean = sum e_j (a_j - a_max), named = sum e_j z_j,
-    // from which loss / (w T^2) = (lean - (named - m mass) / T) / mass + ln s - ln mass.  The logits that
-    // the teacher names are read here from anywhere in the row, before any CTA overwrites it in place.
-    // A table notes whether an index appears twice (see the end).
+    // from which loss / (w T^2) = (lean - (named - m mass) / T) / mass + ln s - ln mass.  A table notes whether
+    // an index appears twice (see the end).
     double mass = 0, lean = 0, named = 0;
+#pragma unroll 1
     for (int j = tid; j < p.k; j += kDistillThreads) {
         const int at = place[j];
         if (at < 0) continue;
         const double a = prob[j] - a_max, e = exp(a);
         mass += e;
-        if (p.loss && e > 0) lean += e * a, named += e * (double)Elem<T>::load(z[at]);
+        if (e > 0) lean += e * a;
         prob[j] = e;
-        if (g)
-            for (unsigned at_table = (unsigned)at * 2654435761u;; ++at_table) {  // at most half of it is taken
-                const int was = atomicCAS(&claimed[at_table & (p.claims - 1)], -1, at);
-                if (was == -1) break;
-                if (was == at) {
-                    repeated = 1;
-                    break;
-                }
+        if (g) {
+            unsigned probe = (unsigned)at * 2654435761u;
+#pragma unroll 1
+            for (;; ++probe) {  // at most half of the table is taken
+                const int was = atomicCAS(&claimed[probe & (p.claims - 1)], -1, at);
+                if (was == at) repeated = 1;
+                if (was == -1 || was == at) break;
             }
+        }
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        mass += __shfl_xor_sync(~0u, mass, o);
-        lean += __shfl_xor_sync(~0u, lean, o);
-        named += __shfl_xor_sync(~0u, named, o);
-    }
-    if (lane == 0) part_sums[0][warp] = mass, part_sums[1][warp] = lean, part_sums[2][warp] = named;
 
     bool ok = true;
     W m, s, inverse;
@@ -413,37 +435,71 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         }
         if (lane == 0) part_m[warp] = m, part_s[warp] = s;
     }
-    __syncthreads();
-    mass = part_sums[0][0];
+    // The first CTA's loss takes the logits that the teacher names, those of other CTAs' slices before any
+    // CTA overwrites them in place.
+    if (p.loss && rank == 0)
+#pragma unroll 1
+        for (int j = tid; j < p.k; j += kDistillThreads) {
+            const int at = place[j];
+            if (at >= 0 && prob[j] > 0) named += prob[j] * (double)Elem<T>::load(at < v1 ? slice[lead + at - v0] : z[at]);
+        }
+    if (p.k > 32 * warp)
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) mass += part_sums[0][i];
+        for (int o = 16; o; o >>= 1) {
+            mass += __shfl_xor_sync(~0u, mass, o);
+            if (p.loss && rank == 0) lean += __shfl_xor_sync(~0u, lean, o), named += __shfl_xor_sync(~0u, named, o);
+        }
+    if (lane == 0) part_sums[0][warp] = mass, part_sums[1][warp] = lean, part_sums[2][warp] = named;
+
     if (!p.stats_in) {
-        m = part_m[0], s = part_s[0];
+        __syncthreads();
+        // One warp joins the warps' shares, and the cluster's: always the same tree, so the same bits in
+        // every CTA.
+        auto joined = [&](int shares) {
 #pragma unroll
-        for (int i = 1; i < WARPS; ++i) join(m, s, part_m[i], part_s[i], c);
+            for (int o = 1; o < 8; o *= 2)
+                if (o < shares) {
+                    const W m2 = __shfl_xor_sync(~0u, m, o), s2 = __shfl_xor_sync(~0u, s, o);
+                    // lower lanes' shares first on both sides
+                    W ma = lane & o ? m2 : m, sa = lane & o ? s2 : s;
+                    join(ma, sa, lane & o ? m : m2, lane & o ? s : s2, c);
+                    m = ma, s = sa;
+                }
+        };
+        static_assert(WARPS == 8, "as many warps as CTAs in the largest cluster");
+        if (warp == 0) {
+            m = part_m[lane % WARPS], s = part_s[lane % WARPS];
+            joined(WARPS);
+            if (lane == 0) share[0] = m, share[1] = s;
+        }
         if (ranks > 1) {
-            if (tid == 0) share[0] = m, share[1] = s;
             cluster_sync();
-            // in rank order in every CTA: the same bits everywhere
-            for (uint32_t r = 0; r < ranks; ++r) {
+            if (warp == 0) {
                 W m2, s2;
-                cluster_read(m2, smem_addr(&share[0]), r);
-                cluster_read(s2, smem_addr(&share[1]), r);
-                if (r == 0) m = m2, s = s2;
-                else join(m, s, m2, s2, c);
+                cluster_read(m2, smem_addr(&share[0]), lane % ranks);
+                cluster_read(s2, smem_addr(&share[1]), lane % ranks);
+                m = m2, s = s2;
+                joined((int)ranks);
+                if (lane == 0) part_m[0] = m, part_s[0] = s;
             }
             // read; this CTA waits for the others' readings when it ends
             asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         }
+        __syncthreads();
+        m = ranks > 1 ? part_m[0] : share[0], s = ranks > 1 ? part_s[0] : share[1];
     }
+    auto over_warps = [&](const double (&part)[WARPS]) {  // behind a barrier
+        double all = part[0];
+#pragma unroll
+        for (int i = 1; i < WARPS; ++i) all += part[i];
+        return all;
+    };
     const W up = p.upstream ? p.upstream[p.upstream_uniform ? 0 : row] : W(1);
     const bool invalid = (flags & 2) || !isfinite(m) || !isfinite(s) || !(s > W(0)) || !isfinite(weight) || (g && !isfinite(up));
     unsigned kind = invalid && tid == 0 ? (unsigned)PCU_B200_KIND_INVALID : 0u;
     if (rank == 0 && tid == 0) {
         if (p.loss) {
-            lean = part_sums[1][0], named = part_sums[2][0];
-#pragma unroll
-            for (int i = 1; i < WARPS; ++i) lean += part_sums[1][i], named += part_sums[2][i];
+            mass = over_warps(part_sums[0]), lean = over_warps(part_sums[1]), named = over_warps(part_sums[2]);
             const double t = (double)p.temperature;
             const W value = invalid ? W(NAN)
                                     : (W)((double)weight * t * t *
@@ -454,7 +510,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         if (p.stats_out) p.stats_out[2 * row] = m, p.stats_out[2 * row + 1] = s;
     }
     if (g && invalid) {
-        for (int v = v0 + tid; v < v1; v += kDistillThreads) g[v] = Elem<T>::round(W(NAN));
+        fill(g, W(NAN));
     } else if (g) {
         const W factor = up * weight * p.temperature;
         refer(run, m, c);
@@ -509,6 +565,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         else p.stats_in ? sweep(std::true_type{}, std::true_type{}) : sweep(std::true_type{}, std::false_type{});
         if (!isfinite(seen) && !kind) kind = PCU_B200_KIND_INVALID;
         __syncthreads();  // before the entries' elements are written again
+        mass = over_warps(part_sums[0]);
         for (int j = tid; j < p.k; j += kDistillThreads) {
             const int at = place[j];
             if (at < v0 || at >= v1) continue;
@@ -593,6 +650,7 @@ template <typename T> static int run_distill(const DistillCall &c, const ChainGu
     p.weights = (const W *)c.weights;
     p.temperature = (W)pcu_host::rate_f32(c.temperature_bits);
     p.to_log2 = (W)(1.4426950408889634074 / (double)p.temperature);
+    p.t_inverse = 1.0 / (double)p.temperature;
     p.loss = (W *)c.loss;
     p.stats_out = (W *)c.stats_out;
     p.stats_in = (const W *)c.stats_in;

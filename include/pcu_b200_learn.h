@@ -91,8 +91,8 @@ int pcu_b200_group_norm_backward(int dtype, int activation, const void *input, c
  *   - A negative index, or a teacher logit of -infinity, is an absent entry.  The same index may
  *     appear several times; each entry counts.
  *   - A student logit of -infinity is a masked vocabulary entry: q = 0 there.
- *   - A row with weight 0, or without a present entry, is not read: loss 0, statistics (0, 1),
- *     gradient 0, no fault.
+ *   - A row with weight 0, or without a present entry, has nothing to learn from, whatever its logits
+ *     are: loss 0, statistics (0, 1), gradient 0, no fault.
  * Events: the row.  InvalidFloatingOperand: a NaN or +infinity among the logits, no finite logit, a
  * present teacher entry that is NaN, +infinity or names an index >= vocab, or a weight or upstream
  * that is not finite; the row's loss and gradient are then NaN.  ArithmeticOverflow: the loss is
