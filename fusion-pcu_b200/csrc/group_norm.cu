@@ -22,10 +22,10 @@
 namespace pcu {
 
 constexpr int kNormThreads = 256;
-// Warp form: CTAs per SM that walk over the batch at once, by what a lane keeps in registers (elements of
-// the wide type, four bytes each counted).
-__host__ __device__ constexpr int warp_form_ctas(int elements, int wide_bytes) {
-    return elements * wide_bytes > 32 ? (elements * wide_bytes > 64 ? 1 : 2) : 3;
+// Warp form: CTAs per SM that walk over the batch at once, by the bytes of a lane's elements in the wide
+// type: forward a lane keeps them and two parameters each, backward also dy and two sums.
+__host__ __device__ constexpr int warp_form_ctas(int bytes, bool backward) {
+    return backward ? (bytes <= 32 ? 3 : bytes <= 64 ? 2 : 1) : (bytes <= 64 ? 3 : 1);
 }
 
 // A channels-last tensor: element (n, s, c) at n * batch + s * row + c.
@@ -95,22 +95,26 @@ template <int V, typename W> __device__ __forceinline__ void activate(int act, W
     }
 }
 
-// h and k = dy act'(h w + b) w.  ReLU's slope is a step, so a z within its own rounding error of 0 (h
-// and the product are each off by a few 2^-24) is decided in binary64; dz = dy act' goes to `dz`.
+// h and dz = dy act'(z), z = h w + b.  ReLU's slope is a step.  z is off by at most 2^-21 |h w| and its own
+// rounding, so its sign is right where |z| > 2^-19 |b|; the few others are decided in binary64.  A masked
+// upstream gradient gives 0, whatever it is.
 template <int V, typename W>
 __device__ __forceinline__ void bend(int act, const W (&x)[V], const W (&dy)[V], const W (&mean)[V], const W (&r)[V],
                                      const W (&w)[V], const W (&b)[V], W (&h)[V], W (&dz)[V]) {
 #pragma unroll
     for (int e = 0; e < V; ++e) h[e] = (x[e] - mean[e]) * r[e], dz[e] = dy[e];
     if (act == PCU_B200_ACTIVATION_RELU) {
+        bool near = false;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const W hw = h[e] * w[e], z = hw + b[e];
-            bool above = z > W(0);
-            if (sizeof(W) == 4 && fabs(z) <= (fabs(hw) + fabs(b[e])) * W(0x1p-20))
-                above = ((double)x[e] - (double)mean[e]) * (double)r[e] * (double)w[e] + (double)b[e] > 0.0;
-            dz[e] = above ? dz[e] : dz[e] * W(0);  // an infinite or NaN upstream shows
+            const W z = fma(h[e], w[e], b[e]);
+            if (sizeof(W) == 4) near |= fabs(z) <= fabs(b[e]) * W(0x1p-19);
+            dz[e] = z > W(0) ? dy[e] : W(0);
         }
+        if (near)
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                dz[e] = ((double)x[e] - (double)mean[e]) * (double)r[e] * (double)w[e] + (double)b[e] > 0.0 ? dy[e] : W(0);
     } else if (act == PCU_B200_ACTIVATION_SILU) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -188,7 +192,6 @@ template <typename T, int V, int K> struct WarpGroup {
     int sub;
     uint64_t slice, g;
     bool active, there[K];
-    uint64_t row[K], channel[K];
     W w[K][V], b[K][V];
 
     __device__ __forceinline__ bool place(const NormParams<T> &p) {
@@ -201,24 +204,32 @@ template <typename T, int V, int K> struct WarpGroup {
         slice = warp / sets;
         g = warp % sets * per + lane / plan.lanes;
         active = g < p.groups;
-        const unsigned across = (unsigned)(p.width / V);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const unsigned item = sub + k * plan.lanes;
-            there[k] = active && item < plan.items;
-            row[k] = there[k] ? item / across : 0;
-            channel[k] = there[k] ? g * p.width + item % across * V : 0;
-            parameters<V>(p.weight, channel[k], W(1), w[k]);
-            parameters<V>(p.bias, channel[k], W(0), b[k]);
+            there[k] = active && sub + k * plan.lanes < (int)plan.items;
+            unsigned row, channel;
+            item(p, k, row, channel);
+            parameters<V>(p.weight, channel, W(1), w[k]);
+            parameters<V>(p.bias, channel, W(0), b[k]);
         }
         return true;
     }
-    // where access k of sample n begins; absent ones point at the sample's first element
-    template <typename M> __device__ __forceinline__ auto first(const M &maps, int k, uint64_t n) const {
-        return maps.at(n, row[k], channel[k]);
+    // access k's place in a sample; (0, 0) where there is none
+    __device__ __forceinline__ void item(const NormParams<T> &p, int k, unsigned &row, unsigned &channel) const {
+        const unsigned item = sub + k * p.plan.lanes, across = (unsigned)(p.width / V);
+        row = there[k] ? item / across : 0;
+        channel = there[k] ? (unsigned)(g * p.width) + item % across * V : 0;
+    }
+    // its offset from the sample's first element (the plan sees to it that samples span less than 2^31)
+    template <typename M> __device__ __forceinline__ int offset(const NormParams<T> &p, const M &maps, int k) const {
+        unsigned row, channel;
+        item(p, k, row, channel);
+        return (int)(row * (unsigned)maps.row + channel);
     }
     __device__ __forceinline__ uint64_t event(const NormParams<T> &p, int k, uint64_t n) const {
-        return (n * p.positions + row[k]) * p.channels + channel[k];
+        unsigned row, channel;
+        item(p, k, row, channel);
+        return (n * p.positions + row) * p.channels + channel;
     }
 };
 
@@ -229,17 +240,18 @@ template <int U, typename W> __device__ __forceinline__ void lanes_sum(W (&v)[U]
 }
 
 template <typename T, int V, int K, int U>
-__global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K, sizeof(WideOf<T>))) norm_warp_kernel(const NormParams<T> p) {
+__global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K * sizeof(WideOf<T>), false)) norm_warp_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
     WarpGroup<T, V, K> at;
     if (!at.place(p)) return;
     const W inverse = W(1) / (W)(p.positions * p.width);
     const uint64_t stride = (uint64_t)p.plan.slices * U;
-    const T *from[K];
-    T *to[K];
+    const T *from = p.x.base + at.slice * U * p.x.batch;
+    T *to = p.out.base + at.slice * U * p.out.batch;
+    int in[K], out[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) from[k] = at.first(p.x, k, at.slice * U), to[k] = at.first(p.out, k, at.slice * U);
+    for (int k = 0; k < K; ++k) in[k] = at.offset(p, p.x, k), out[k] = at.offset(p, p.out, k);
     W *stats = p.stats_out + 2 * (at.slice * U * p.groups + at.g);
     for (uint64_t n = at.slice * U; n < p.batch; n += stride) {
         const int here = (int)min((uint64_t)U, p.batch - n);
@@ -248,7 +260,7 @@ __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (at.there[k] && u < here) Access<T, V>::load(from[k] + u * p.x.batch).open(x[u][k]);
+                if (at.there[k] && u < here) Access<T, V>::load(from + u * p.x.batch + in[k]).open(x[u][k]);
                 else
 #pragma unroll
                     for (int e = 0; e < V; ++e) x[u][k][e] = W(0);
@@ -284,31 +296,27 @@ __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K
 #pragma unroll
                 for (int e = 0; e < V; ++e) x[u][k][e] = x[u][k][e] * r * at.w[k][e] + at.b[k][e];
                 activate<V>(p.activation, x[u][k]);
-                put<T, V>(to[k] + u * p.out.batch, x[u][k], p.status, [&] { return at.event(p, k, n + u); });
+                put<T, V>(to + u * p.out.batch + out[k], x[u][k], p.status, [&] { return at.event(p, k, n + u); });
             }
         }
-#pragma unroll
-        for (int k = 0; k < K; ++k) from[k] += stride * p.x.batch, to[k] += stride * p.out.batch;
+        from += stride * p.x.batch, to += stride * p.out.batch;
         stats += 2 * stride * p.groups;
     }
 }
 
 template <typename T, int V, int K, int U>
-__global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K, sizeof(WideOf<T>))) norm_warp_backward_kernel(const NormParams<T> p) {
+__global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K * sizeof(WideOf<T>), true)) norm_warp_backward_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
     if (!chain_admits(p.guard)) return;
     WarpGroup<T, V, K> at;
     if (!at.place(p)) return;
     const W inverse = W(1) / (W)(p.positions * p.width);
     const uint64_t stride = (uint64_t)p.plan.slices * U;
-    const T *from[K], *up[K];
-    T *to[K];
+    const T *from = p.x.base + at.slice * U * p.x.batch, *up = p.dy.base + at.slice * U * p.dy.batch;
+    T *to = p.out.base + at.slice * U * p.out.batch;
+    int in[K], grad[K], out[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        from[k] = at.first(p.x, k, at.slice * U);
-        up[k] = at.first(p.dy, k, at.slice * U);
-        to[k] = at.first(p.out, k, at.slice * U);
-    }
+    for (int k = 0; k < K; ++k) in[k] = at.offset(p, p.x, k), grad[k] = at.offset(p, p.dy, k), out[k] = at.offset(p, p.out, k);
     const W *stats = p.stats + 2 * (at.slice * U * p.groups + (at.active ? at.g : 0));
     W dw[K][V] = {}, db[K][V] = {};
     for (uint64_t n = at.slice * U; n < p.batch; n += stride) {
@@ -319,8 +327,8 @@ __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (at.there[k] && u < here) {
-                    Access<T, V>::load(from[k] + u * p.x.batch).open(x[u][k]);
-                    Access<T, V>::load(up[k] + u * p.dy.batch).open(dy[u][k]);
+                    Access<T, V>::load(from + u * p.x.batch + in[k]).open(x[u][k]);
+                    Access<T, V>::load(up + u * p.dy.batch + grad[k]).open(dy[u][k]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < V; ++e) x[u][k][e] = dy[u][k][e] = W(0);
@@ -361,11 +369,10 @@ __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K
                 if (!at.there[k]) continue;
 #pragma unroll
                 for (int e = 0; e < V; ++e) x[u][k][e] = r[u] * (dy[u][k][e] - c1[u] - x[u][k][e] * c2[u]);
-                put<T, V>(to[k] + u * p.out.batch, x[u][k], p.status, [&] { return at.event(p, k, n + u); });
+                put<T, V>(to + u * p.out.batch + out[k], x[u][k], p.status, [&] { return at.event(p, k, n + u); });
             }
         }
-#pragma unroll
-        for (int k = 0; k < K; ++k) from[k] += stride * p.x.batch, up[k] += stride * p.dy.batch, to[k] += stride * p.out.batch;
+        from += stride * p.x.batch, up += stride * p.dy.batch, to += stride * p.out.batch;
         stats += 2 * stride * p.groups;
     }
     if (!p.partial) return;
@@ -1011,8 +1018,9 @@ bool shape_fits(uint64_t batch, uint64_t positions, uint64_t channels, uint64_t 
 
 constexpr size_t kSlabMost = 200 * 1024;  // shared memory of a CTA for a slab
 
-// `vector`: elements per access, 16 bytes' worth or 1.  No extent is 0.
-NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, uint64_t channels, uint64_t groups,
+// `vector`: elements per access, 16 bytes' worth or 1.  `near`: samples span less than 2^31 elements.  No
+// extent is 0.
+NormPlan plan_norm(int dtype, int vector, bool near, uint64_t batch, uint64_t positions, uint64_t channels, uint64_t groups,
                    bool backward) {
     NormPlan p{};
     const uint64_t width = channels / groups, bytes = pcu_host::element_bytes(dtype), wide = dtype == PCU_B200_F64 ? 8 : 4;
@@ -1021,14 +1029,18 @@ NormPlan plan_norm(int dtype, int vector, uint64_t batch, uint64_t positions, ui
     p.partial_split = 1;
     // Warp form: 16 elements of a lane are in registers (and as many of dy, and four parameters' worth), so
     // a group has at most 512 of them.
-    if (width % vector == 0 && positions <= 512 && positions * (width / vector) * vector <= 512) {
+    if (near && width % vector == 0 && positions <= 512 && positions * (width / vector) * vector <= 512) {
         p.form = NormPlan::kWarp;
         p.items = (unsigned)(positions * (width / vector));
+        // A lane takes two accesses (one backward), or 8 single elements (4), where the group has them: fewer
+        // lanes join their sums in fewer steps (8192 x 4096, groups of 128, F32: 51 us against 54 with four and 58 with
+        // one; backward one holds the registers of two loads in flight, two do not: 99 against 112 us).
+        const unsigned accesses = vector == 1 ? (backward ? 4 : 8) : (backward ? 1 : 2);
         p.lanes = 1;
-        while (p.lanes < 32 && (unsigned)p.lanes < p.items) p.lanes *= 2;
+        while (p.lanes < 32 && (unsigned)p.lanes * accesses < p.items) p.lanes *= 2;
         p.per_lane = (int)((p.items + p.lanes - 1) / p.lanes);
         const uint64_t per = 32 / p.lanes, sets = (groups + per - 1) / per;
-        const uint64_t ctas = p.per_lane > 4 ? 1 : warp_form_ctas(vector * p.per_lane, (int)wide);
+        const uint64_t ctas = p.per_lane > 4 ? 1 : warp_form_ctas((int)(vector * p.per_lane * wide), backward);
         // Each warp walks over a slice of the batch; as many warps as are resident at once.
         p.slices = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(batch, sms * ctas * (kNormThreads / 32) / sets));
         p.partial_rows = p.slices;
@@ -1092,10 +1104,13 @@ size_t workspace_size(int dtype, uint64_t batch, uint64_t positions, uint64_t ch
     const size_t bytes = pcu_host::element_bytes(dtype);
     if (!bytes || groups == 0 || channels % groups != 0 || !shape_fits(batch, positions, channels, groups)) return 0;
     if (batch == 0 || positions == 0 || channels == 0) return 0;
-    uint64_t need = plan_norm(dtype, 1, batch, positions, channels, groups, backward).workspace;
+    uint64_t need = 0;  // for either access width, samples near and far
     const int vector = (int)(16 / bytes);
-    if (channels % vector == 0)
-        need = std::max(need, plan_norm(dtype, vector, batch, positions, channels, groups, backward).workspace);
+    for (const bool near : {true, false}) {
+        need = std::max(need, plan_norm(dtype, 1, near, batch, positions, channels, groups, backward).workspace);
+        if (channels % vector == 0)
+            need = std::max(need, plan_norm(dtype, vector, near, batch, positions, channels, groups, backward).workspace);
+    }
     return need * (dtype == PCU_B200_F64 ? 8 : 4);
 }
 
@@ -1120,9 +1135,10 @@ template <typename T, int V> int run_norm(NormParams<T> p, bool backward, cudaSt
     int rc = PCU_B200_OK;
     const NormPlan &plan = p.plan;
     if (plan.form == NormPlan::kWarp) {
-        // accesses per lane: 1, or what 16 elements make
+        // accesses per lane: 1, 2, 4, or what 16 elements make
         if (plan.per_lane == 1) rc = run_warp<T, V, 1>(p, backward, stream);
-        else if (V * 4 <= 16 && plan.per_lane <= 4) rc = run_warp<T, V, std::min(4, 16 / V)>(p, backward, stream);
+        else if (plan.per_lane == 2) rc = run_warp<T, V, 2>(p, backward, stream);
+        else if (plan.per_lane <= 4) rc = run_warp<T, V, std::min(4, 16 / V)>(p, backward, stream);
         else rc = run_warp<T, V, 16 / V>(p, backward, stream);
         if (rc) return rc;
         p.guard = chain_follow(p.guard);
@@ -1185,7 +1201,9 @@ template <typename T> int typed_norm(const NormCall &c, const ChainGuard &guard)
         const bool wide = c.channels % V == 0 && whole(c.input, c.input_batch_stride, c.input_stride) &&
                           whole(c.out, c.out_batch_stride, c.out_stride) &&
                           (!c.backward || whole(c.upstream, c.upstream_batch_stride, c.upstream_stride));
-        p.plan = plan_norm(c.dtype, wide ? V : 1, c.batch, c.positions, c.channels, c.groups, c.backward);
+        auto spans = [&](uint64_t stride) { return (c.positions - 1) * stride + c.channels < (1ull << 31); };
+        const bool near = spans(c.input_stride) && spans(c.out_stride) && (!c.backward || spans(c.upstream_stride));
+        p.plan = plan_norm(c.dtype, wide ? V : 1, near, c.batch, c.positions, c.channels, c.groups, c.backward);
         p.partial = (W *)c.workspace;
         p.sums = p.partial + 2 * p.plan.partial_rows * p.channels;  // stream form
         // partial sums are for the stream form's groups, or for gradients that are wanted
