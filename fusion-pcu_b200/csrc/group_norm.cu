@@ -1048,11 +1048,11 @@ NormPlan plan_norm(int dtype, int vector, bool near, uint64_t batch, uint64_t po
         p.workspace = backward ? 2 * p.partial_rows * channels * positions : 0;
         return p;
     }
-    // Slab form: blocks of whole groups whose rows are at least 128 bytes and whole accesses.  The smallest
-    // cluster whose CTAs hold at most 84 KB, so that two share an SM and overlap loading, sums and stores
+    // Slab form: blocks of whole groups whose rows are at least 128 bytes and whole accesses, in the
+    // smallest cluster whose CTAs hold at most 84 KB, so that two share an SM and overlap loading, sums and stores
     // while their threads have some ten rows each to earn their set-up (48 KB: 158 against 131 us at 16 x
-    // 4095 x 1280 BF16 forward, 164 against 122 us at 32 x 1024 x 1280 backward), or 200 KB in a cluster of 8; more
-    // CTAs, down to 16 KB each, when they do not fill the SMs twice.
+    // 4095 x 1280 BF16 forward, 164 against 122 us at 32 x 1024 x 1280 backward), or 200 KB in a cluster of 8;
+    // more CTAs, down to 16 KB each, when they do not fill the SMs twice.
     const uint64_t most = 84 * 1024;
     const uint64_t tensors = backward ? 2 : 1;
     const uint64_t step = (uint64_t)vector / std::gcd(width, (uint64_t)vector);
@@ -1061,10 +1061,20 @@ NormPlan plan_norm(int dtype, int vector, bool near, uint64_t batch, uint64_t po
         const uint64_t across = block * width / vector;
         if (across > 512 || block * width % vector != 0) return false;
         const uint64_t row = block * width * bytes * tensors;
+        const uint64_t blocks = (groups + block - 1) / block, clusters = batch * blocks;
         uint64_t ranks = 1;
         while (ranks < 8 && (positions + ranks - 1) / ranks * row > most) ranks *= 2;
-        const uint64_t blocks = (groups + block - 1) / block;
-        while (ranks < 8 && batch * blocks * ranks < 2 * sms && (positions + ranks - 1) / ranks * row > 16384) ranks *= 2;
+        while (ranks < 8 && clusters * ranks < 2 * sms && (positions + ranks - 1) / ranks * row > 16384) ranks *= 2;
+        // The SMs come in 8 groups, and a cluster stays within one.  Where so many clusters take two turns, but
+        // somewhat smaller ones a single turn, those are taken (20 clusters at 5 x 4095 x 320: of 8 CTAs 18.6 us, of 6
+        // 16.7 us).
+        auto turns = [&](uint64_t r) { return (clusters + 8 * (sms / 8 / r) - 1) / (8 * (sms / 8 / r)); };
+        if (sms >= 64 && turns(ranks) == 2)
+            for (uint64_t r = ranks - 1; 2 * r > ranks; --r)
+                if (turns(r) == 1 && (positions + r - 1) / r * row <= 128 * 1024) {
+                    ranks = r;
+                    break;
+                }
         const uint64_t rows = (positions + ranks - 1) / ranks;
         const uint64_t threads = across > 256 ? 512 : 256;
         const uint64_t extra = 2 * threads * (vector + 1) * wide + 4 * block * wide + 64;
