@@ -830,6 +830,8 @@ int quantize(int dtype, const void *input, uint64_t rows, uint64_t columns, uint
     if (rows == 0 || columns == 0) return chain_decide_only(guard, s);
     if (!input || !codes || !scales || (rows > 1 && (input_stride < columns || codes_stride < columns)))
         return PCU_B200_ERROR_INVALID_ARGUMENT;
+    if (!pcu_host::aligned(input, pcu_host::element_bytes(dtype)) || !pcu_host::aligned(scales, 4) || !pcu_host::aligned(status, 8))
+        return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (rows >= kMostExtent || columns >= kMostExtent || input_stride > kMostStride || codes_stride > kMostStride ||
         (rows + block_rows - 1) / block_rows * ((columns + kBlock - 1) / kBlock) >= kMostExtent)
         return PCU_B200_ERROR_SIZE_OVERFLOW;
@@ -853,6 +855,9 @@ int product(int out_dtype, const void *left, const float *left_scales, const voi
     if (!out || (rows > 1 && out_stride < columns)) return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (inner && (!left || !left_scales || !right || !right_scales || (rows > 1 && left_stride < inner) ||
                   (columns > 1 && right_stride < inner)))
+        return PCU_B200_ERROR_INVALID_ARGUMENT;
+    if (!pcu_host::aligned(out, pcu_host::element_bytes(out_dtype)) || !pcu_host::aligned(left_scales, 4) ||
+        !pcu_host::aligned(right_scales, 4) || !pcu_host::aligned(status, 8))
         return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (rows >= kMostExtent || inner >= kMostExtent || columns >= kMostExtent || left_stride > kMostStride ||
         right_stride > kMostStride || out_stride > kMostStride ||

@@ -93,7 +93,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill
     a_max = block_max(a_max, scratch_d);
     bad = __syncthreads_or(bad);
     const bool skip = weight == W(0) || (a_max == -INFINITY && !bad);
-    if (skip) {  // nothing to learn from: the row is not read
+    if (skip) {  // nothing to learn from
         if (threadIdx.x == 0) {
             if (p.loss) p.loss[row] = W(0);
             if (p.stats_out) p.stats_out[2 * row] = W(0), p.stats_out[2 * row + 1] = W(1);
@@ -197,7 +197,7 @@ constexpr int kChunk = 16384;  // bytes per bulk copy, each with a barrier: 4 gr
 
 // A running maximum and sum of 2^(c (x - m)).  With hi = c m rounded, c x - hi is one multiply-add;
 // the sum so formed is 2^d times the wanted one, d = hi - c m (known exactly), and it is set right at the end.
-// A maximum of 2^64 and more, where c x may overflow, takes the difference first.
+// Where c m is 2^100 and more (or there is no maximum yet) the difference is taken first.
 template <typename W> struct Running {
     W m, s, hi;
     bool far;
@@ -205,8 +205,9 @@ template <typename W> struct Running {
 
 __device__ __forceinline__ void refer(Running<float> &r, float m, float c) {
     r.m = m;
-    r.far = !(fabsf(m) < 0x1p64f);
-    r.hi = r.far ? 0.0f : m * c;
+    r.hi = m * c;
+    r.far = !(fabsf(r.hi) < 0x1p100f);
+    if (r.far) r.hi = 0.0f;
 }
 __device__ __forceinline__ void refer(Running<double> &r, double m, double) { r.m = m, r.far = true, r.hi = 0; }
 
@@ -673,6 +674,12 @@ int distill(const DistillCall &c, const ChainGuard &guard) {
     if (c.wants_loss && !c.loss) return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (c.wants_gradient && (!c.gradient || c.gradient_stride < c.vocab)) return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (!c.wants_loss && !c.stats_in) return PCU_B200_ERROR_INVALID_ARGUMENT;
+    const size_t bytes = pcu_host::element_bytes(c.dtype), wide = c.dtype == PCU_B200_F64 ? 8 : 4;
+    for (const void *p : {c.logits, (const void *)c.gradient})
+        if (!pcu_host::aligned(p, bytes)) return PCU_B200_ERROR_INVALID_ARGUMENT;
+    for (const void *p : {c.top, c.weights, (const void *)c.loss, (const void *)c.stats_out, c.stats_in, c.upstream})
+        if (!pcu_host::aligned(p, wide)) return PCU_B200_ERROR_INVALID_ARGUMENT;
+    if (!pcu_host::aligned(c.indices, 8) || !pcu_host::aligned(c.status, 8)) return PCU_B200_ERROR_INVALID_ARGUMENT;
     // in place means the same rows: any other overlap would overwrite logits before they are read
     if (c.gradient == c.logits && c.wants_gradient && c.gradient_stride != c.stride) return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (c.rows > 0x7fffffffull || c.vocab > 0x7fffffffull || c.k > PCU_B200_DISTILL_TOP_MAX ||

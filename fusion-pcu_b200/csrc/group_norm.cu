@@ -182,6 +182,9 @@ template <int V, typename W> __device__ __forceinline__ void parameters(const W 
 __device__ __forceinline__ float root(float var, float eps) { return isfinite(var) ? rsqrtf(var + eps) : NAN; }
 __device__ __forceinline__ double root(double var, double eps) { return isfinite(var) ? 1.0 / sqrt(var + eps) : NAN; }
 
+// A sum of squares that rounding made negative is 0; NaN stays.
+template <typename W> __device__ __forceinline__ W not_negative(W v) { return v < W(0) ? W(0) : v; }
+
 // ---- warp form
 //
 // `lanes` lanes hold a group, K accesses each; 32 / lanes adjacent groups per warp.  A warp keeps its
@@ -639,7 +642,7 @@ template <typename T, int V> __global__ void __launch_bounds__(512, sizeof(WideO
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const W shift = mean[e] * inverse;
-            r[e] -= mean[e] * shift;
+            r[e] = not_negative(r[e] - mean[e] * shift);
             mean[e] = first[e] + shift;
         }
     }
@@ -785,7 +788,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
         const int to = threadIdx.x * V + e;
         const W shift = count ? sum[e] / (W)count : W(0);
         means[to] = count ? first[e] + shift : W(0);
-        squares[to] = count ? square[e] - sum[e] * shift : W(0);
+        squares[to] = count ? not_negative(square[e] - sum[e] * shift) : W(0);
     }
     __syncthreads();
     const uint64_t rows = at.s1 - at.s0;
@@ -1260,6 +1263,12 @@ int norm(const NormCall &c, const ChainGuard &guard) {
         (c.backward && (c.batch == 0 || c.positions == 0) && !c.dweight && !c.dbias))
         return chain_decide_only(guard, pcu_host::as_stream(c.stream));
     if (!c.backward && !c.stats_out) return PCU_B200_ERROR_INVALID_ARGUMENT;
+    const size_t bytes = pcu_host::element_bytes(c.dtype), wide = c.dtype == PCU_B200_F64 ? 8 : 4;
+    for (const void *p : {c.input, c.upstream, (const void *)c.out})
+        if (!pcu_host::aligned(p, bytes)) return PCU_B200_ERROR_INVALID_ARGUMENT;
+    for (const void *p : {c.weight, c.bias, c.stats_in, (const void *)c.stats_out, (const void *)c.dweight, (const void *)c.dbias})
+        if (!pcu_host::aligned(p, wide)) return PCU_B200_ERROR_INVALID_ARGUMENT;
+    if (!pcu_host::aligned(c.status, 8)) return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (c.batch && c.positions) {
         if (!good_maps(c.input, c.batch, c.positions, c.channels, c.input_batch_stride, c.input_stride) ||
             !good_maps(c.out, c.batch, c.positions, c.channels, c.out_batch_stride, c.out_stride))

@@ -17,7 +17,8 @@
  *   - There is no underflow policy: results underflow gradually, softmax terms below 2^-126 are 0.
  *   - Faults: a result that is not finite is recorded as InvalidFloatingOperand when it is NaN and
  *     as ArithmeticOverflow when it is an infinity; the events are given with each call.
- *   - Buffers must not overlap except where a call says so.
+ *   - Buffers must not overlap except where a call says so, and are aligned to their elements
+ *     (PCU_B200_ERROR_INVALID_ARGUMENT otherwise).
  */
 #ifndef PCU_B200_LEARN_H
 #define PCU_B200_LEARN_H
@@ -46,7 +47,7 @@ extern "C" {
  *   out = activation((x - mean) * r * weight[c] + bias[c]).
  * weight and bias are wide, `channels` elements, or NULL (1 and 0).  eps is a finite binary32
  * pattern, not negative.  stats receives (mean, r) for each (n, group), wide, 2 * batch * groups.
- * The activation's slope at z = 0 is 0 for ReLU.  channels must be a multiple of groups; batch and
+ * ReLU's slope at z = 0 is 0.  channels must be a multiple of groups; batch and
  * positions may be 0.  out has its own strides and may be input itself (same strides).
  * The variance is summed about the mean, never as a difference of two sums.
  * Events: the element's index (n * positions + s) * channels + c in out.  A group that holds a NaN
@@ -64,7 +65,8 @@ int pcu_b200_group_norm(int dtype, int activation, const void *input, const void
  * out by its own strides; it may be input or upstream itself, with the same strides), and the wide
  * weight_gradient and bias_gradient (channels each; NULL when not wanted).  stats is what the
  * forward call wrote.  With batch or positions 0 the parameters' gradients are zeros.
- * Whether z is above 0, for ReLU, is decided exactly for the given stats, weight and bias.
+ * Whether z is above 0, for ReLU, is decided in binary64 for the given stats, weight and bias; where it is
+ * not, upstream does not count, whatever it is.
  * Events: the element's index in gradient, then batch * positions * channels + c for
  * weight_gradient[c], then channels more + c for bias_gradient[c]. */
 size_t pcu_b200_group_norm_backward_workspace_size(int dtype, uint64_t batch, uint64_t positions, uint64_t channels,

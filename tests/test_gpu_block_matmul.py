@@ -139,6 +139,21 @@ def test_product_of_any_stride(provider, shape):
     assert bool((base[:, columns:] == 7.0).all())
 
 
+@pytest.mark.parametrize("rows", [2, 40])
+def test_offsets_beyond_32_bits(provider, rows):
+    """Rows of codes so far apart that the last one begins beyond 2^32 bytes."""
+    a, sa, b, sb = _operands(rows, 256, 70, 8)
+    want = provider.block_matmul(a, sa, b, sb, dtype=torch.float32)
+    stride = ((1 << 32) // (rows - 1) + 16) // 16 * 16
+    far = torch.empty(stride * (rows - 1) + 256, dtype=torch.uint8, device="cuda").as_strided((rows, 256), (stride, 1))
+    far.copy_(a.view(torch.uint8))
+    assert torch.equal(provider.block_matmul(far, sa, b, sb, dtype=torch.float32), want)
+    x = torch.randn((rows, 256), device="cuda")
+    codes, scales = provider.block_quantize(x)
+    out, _ = provider.block_quantize(x, codes=far)
+    assert torch.equal(out, codes.view(torch.uint8))
+
+
 @pytest.mark.parametrize("rows", [1, 9, 200])
 def test_cells_are_whole_sums(provider, rows):
     """Integers small enough for every sum to be exact in binary32: the product is exact, whatever the order."""

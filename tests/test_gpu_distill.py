@@ -164,6 +164,46 @@ def test_large_and_far_logits(provider):
     _check(provider, z - 20000.0, at.flip(1), top * 1000, 4.0, None, None, torch.float32)
 
 
+def test_small_and_large_temperatures(provider):
+    """A temperature whose reciprocal leaves hardly a term beside the largest, one that makes q uniform, and
+    one at which logits divided by it exceed binary32."""
+    z, at, top, gen = _data((6, 900, 5), torch.float32, 15)
+    for t in (1e-3, 1e6):
+        _check(provider, z, at, top, t, None, None, torch.float32)
+    t = 1e-37
+    z[:, 0] = z.amax(dim=1) + 1
+    at[:, 0], at[:, 1:] = 0, -1
+    loss, stats, gradient = provider.distill_loss_step(z, at, top, temperature=t)
+    # the teacher's only entry is the student's largest logit: nothing else has a share, both are certain
+    assert not loss.any() and not gradient.any() and bool((stats[:, 1] == 1).all())
+
+
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 600001), (torch.float64, 300000), (torch.bfloat16, 1000003)])
+def test_rows_longer_than_a_cluster_holds(provider, dtype, vocab):
+    z, at, top, gen = _data((3, vocab, 20), dtype, 16)
+    at[1, 4:] = at[1, 3]
+    w = torch.tensor([1.0, 0.5, 0.0], device="cuda").to(lu.WIDE[dtype])
+    loss, stats, gradient = _check(provider, z, at, top, 1.3, w, None, dtype)
+    a = z.clone()
+    provider.distill_loss_step(a, at, top, temperature=1.3, row_weights=w, gradient=a)
+    assert torch.equal(a, gradient)
+    z[0, vocab - 1] = math.nan
+    status = provider.new_status()
+    provider.distill_loss_step(z, at, top, temperature=1.3, row_weights=w, status=status)
+    assert provider.decode_status(status_word(status)) == (0, 5)
+
+
+def test_row_offsets_beyond_32_bits(provider):
+    """Two rows 2^31 elements apart."""
+    z, at, top, _ = _data((2, 500, 8), torch.float16, 17)
+    want = provider.distill_loss_step(z, at, top)
+    base = torch.empty((1 << 31) + 500, dtype=torch.float16, device="cuda")
+    far = base.as_strided((2, 500), (1 << 31, 1))
+    far.copy_(z)
+    got = provider.distill_loss_step(far, at, top, gradient=far)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape", [(3, 131072, 16), (400, 777, 16), (2, 40, 4)])
 def test_gradient_in_place(provider, shape, dtype):

@@ -205,6 +205,53 @@ def test_in_place(provider, shape, dtype):
         assert all(torch.equal(p, q) for p, q in zip(grads, again))
 
 
+def test_offsets_beyond_32_bits(provider):
+    """Positions, and samples, 2^31 elements apart: the rows' offsets need 64 bits in every form."""
+    x, dy, w, b = _data((2, 2, 64, 4), torch.bfloat16, 9)
+    want = provider.group_norm(x, 4, w, b, activation="silu")
+    grads = provider.group_norm_backward(x, dy, 4, want[1], w, b, activation="silu")
+    base = torch.empty((1 << 31) * 3 + 64, dtype=torch.bfloat16, device="cuda")
+    for strides in ((1 << 31, 64, 1), (64, 1 << 31, 1), (1 << 32, 1 << 31, 1)):
+        far = base.as_strided((2, 2, 64), strides)
+        far.copy_(x)
+        if strides[0] == 64:  # samples within the gaps of one another's rows are refused: rows may not interleave
+            with pytest.raises(provider.ProviderFailure):
+                provider.group_norm(far, 4, w, b, activation="silu")
+            continue
+        out, stats = provider.group_norm(far, 4, w, b, activation="silu")
+        e = lu.u(torch.float32) * 64
+        lu.within(stats, want[1].double(), e * (1 + want[1].double().abs()))
+        y, _, h = lu.norm_forward(x, 4, w, b, "silu")
+        lu.within(out, y, _forward_tolerance(x, 4, w, b, y, h, torch.bfloat16))
+        got = provider.group_norm_backward(far, dy, 4, want[1], w, b, activation="silu")
+        target = lu.norm_backward(x, dy, 4, want[1], w, b, "silu")
+        for g, t, tol in zip(got, target, _backward_tolerances(x, dy, 4, want[1], w, b, "silu", torch.bfloat16, target)):
+            lu.within(g, t, tol)
+
+
+def test_constant_groups(provider):
+    """No spread at all: the variance is 0, never less, and r is 1 / sqrt(eps)."""
+    for shape, g in (((3, 1, 64), 4), ((2, 500, 64), 4), ((1, 40000, 8), 1), ((2, 300, 30), 3)):
+        x = torch.full(shape, 1234.567, device="cuda")
+        out, stats = provider.group_norm(x, g, eps=0.25)
+        lu.within(stats[..., 1], torch.full_like(stats[..., 1], 2.0).double(), 8 * lu.u(torch.float32) + (1234.567 * lu.u(torch.float32) * 700) ** 2 * 8)
+        assert float(out.abs().max()) <= 2 * 1234.567 * lu.u(torch.float32) * 1400
+
+
+def test_masked_upstream_does_not_leak(provider):
+    """An infinite or NaN upstream where ReLU is off counts for nothing."""
+    for shape in ((4, 1, 64, 4), (2, 300, 64, 4), (1, 20000, 16, 2)):
+        x, dy, w, b = _data(shape, torch.float32, 12)
+        g = shape[3]
+        y, stats = provider.group_norm(x, g, w, b, activation="relu")
+        clean = torch.where(y > 0, dy, 0.0)
+        dirty = torch.where(y > 0, dy, torch.where(torch.rand_like(dy) < 0.5, math.nan, math.inf))
+        a = provider.group_norm_backward(x, clean, g, stats, w, b, activation="relu")
+        d = provider.group_norm_backward(x, dirty, g, stats, w, b, activation="relu")
+        # y is rounded, z decided in binary64: none lies between here, so the masks agree
+        assert all(torch.equal(p, q) for p, q in zip(a, d))
+
+
 def test_strided_output_leaves_the_gaps(provider):
     x, _, w, b = _data((3, 50, 24, 4), torch.float32, 1)
     base = torch.full((3, 51, 40), 7.0, device="cuda")

@@ -36,6 +36,9 @@ def _norm(lib, word, **change):
     (dict(xs=9, xb=26), INVALID),  # in place (out is x), but not element for element
     (dict(n=1 << 31), OVERFLOW), (dict(s=1 << 41), OVERFLOW), (dict(c=1 << 31, g=1), OVERFLOW),
     (dict(xs=1 << 57), OVERFLOW), (dict(n=1 << 20, s=1 << 39, xb=1 << 50), OVERFLOW),
+    (dict(x=VP(4098), out=VP(8192)), INVALID), (dict(out=VP(4097)), INVALID), (dict(w=VP(4097)), INVALID),
+    (dict(b=VP(4098)), INVALID), (dict(stats=VP(4098)), INVALID), (dict(dtype=2, x=VP(4097), out=VP(8192)), INVALID),
+    (dict(dtype=1, stats=VP(4100)), INVALID),
 ])
 def test_group_norm(lib, word, change, code):
     assert _norm(lib, word, **change) == code
@@ -59,7 +62,8 @@ def _norm_backward(lib, word, **change):
     (dict(dtype=4), INVALID), (dict(status=None), INVALID), (dict(x=None), INVALID), (dict(dy=None), INVALID),
     (dict(dx=None), INVALID), (dict(stats=None), INVALID), (dict(ys=7), INVALID), (dict(yb=20), INVALID),
     (dict(ys=1 << 57), OVERFLOW), (dict(ws=None), WORKSPACE), (dict(ws_bytes=3), WORKSPACE), (dict(ws=VP(4098)), WORKSPACE),
-    (dict(dx=P, dy=VP(8192), xs=9, xb=27), INVALID),
+    (dict(dx=P, dy=VP(8192), xs=9, xb=27), INVALID), (dict(dy=VP(4097)), INVALID), (dict(dw=VP(4097)), INVALID),
+    (dict(db=VP(4098)), INVALID),
 ])
 def test_group_norm_backward(lib, word, change, code):
     assert _norm_backward(lib, word, **change) == code
@@ -94,7 +98,8 @@ def _distill(lib, word, call, **change):
     (dict(stride=9), INVALID), (dict(at=None), INVALID), (dict(top=None), INVALID), (dict(t=0), INVALID),
     (dict(t=0xBF800000), INVALID), (dict(t=0x7F800000), INVALID), (dict(t=0x7FC00000), INVALID), (dict(t=1), INVALID),
     (dict(k=1025), OVERFLOW), (dict(rows=1 << 31), OVERFLOW), (dict(vocab=1 << 31, stride=1 << 31, gs=1 << 31), OVERFLOW),
-    (dict(stride=1 << 41), OVERFLOW),
+    (dict(stride=1 << 41), OVERFLOW), (dict(z=VP(4097)), INVALID), (dict(top=VP(4098)), INVALID),
+    (dict(at=VP(4100)), INVALID), (dict(w=VP(4097)), INVALID), (dict(stats=VP(4098)), INVALID),
 ])
 def test_distill(lib, word, call, change, code):
     assert _distill(lib, word, call, **change) == code
@@ -117,6 +122,7 @@ def test_distill_of_each_call(lib, word):
     (dict(dtype=1), INVALID), (dict(dtype=4), INVALID), (dict(high=2), INVALID), (dict(status=None), INVALID),
     (dict(x=None), INVALID), (dict(codes=None), INVALID), (dict(scales=None), INVALID), (dict(stride=9), INVALID),
     (dict(codes_stride=9), INVALID), (dict(rows=1 << 31), OVERFLOW), (dict(columns=1 << 31, stride=1 << 31, codes_stride=1 << 31), OVERFLOW),
+    (dict(x=VP(4097)), INVALID), (dict(scales=VP(4098)), INVALID),
     (dict(stride=1 << 41), OVERFLOW), (dict(rows=0, x=None, codes=None, scales=None), 0),
 ])
 def test_block_quantize(lib, word, change, code):
@@ -130,6 +136,7 @@ def test_block_quantize(lib, word, change, code):
     (dict(dtype=1), INVALID), (dict(dtype=4), INVALID), (dict(status=None), INVALID), (dict(a=None), INVALID),
     (dict(b=None), INVALID), (dict(sa=None), INVALID), (dict(sb=None), INVALID), (dict(out=None), INVALID),
     (dict(lda=9), INVALID), (dict(ldb=9), INVALID), (dict(ldo=9), INVALID), (dict(m=1 << 31), OVERFLOW),
+    (dict(out=VP(4098)), INVALID), (dict(sa=VP(4097)), INVALID), (dict(sb=VP(4098)), INVALID),
     (dict(k=1 << 31, lda=1 << 31, ldb=1 << 31), OVERFLOW), (dict(ldo=1 << 41), OVERFLOW),
     (dict(m=1 << 30, n=1 << 30, ldo=1 << 30), OVERFLOW), (dict(m=0, a=None, out=None), 0), (dict(n=0, b=None, out=None), 0),
 ])
