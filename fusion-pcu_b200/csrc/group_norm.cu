@@ -1238,13 +1238,13 @@ template <typename T> int typed_norm(const NormCall &c, const ChainGuard &guard)
     return rc;
 }
 
-// Rows of `channels` elements: a batch's rows lie within its stride, so no two rows overlap.
+// Rows of `channels` elements that do not overlap: a sample's rows lie within the batch stride, or, with
+// positions first, a position's rows within the row stride.
 bool good_maps(const void *base, uint64_t batch, uint64_t positions, uint64_t channels, uint64_t batch_stride,
                uint64_t stride) {
-    if (!base) return false;
-    if (positions > 1 && stride < channels) return false;
-    const uint64_t reach = (positions - 1) * stride + channels;
-    return batch <= 1 || batch_stride >= reach || (positions == 1 && batch_stride >= channels);
+    if (!base || (positions > 1 && stride < channels) || (batch > 1 && batch_stride < channels)) return false;
+    if (batch <= 1 || positions <= 1) return true;
+    return batch_stride >= (positions - 1) * stride + channels || stride >= (batch - 1) * batch_stride + channels;
 }
 
 int norm(const NormCall &c, const ChainGuard &guard) {
@@ -1255,6 +1255,9 @@ int norm(const NormCall &c, const ChainGuard &guard) {
     if (!std::isfinite(eps) || std::signbit(eps)) return PCU_B200_ERROR_INVALID_ARGUMENT;
     if (!shape_fits(c.batch, c.positions, c.channels, c.groups) || c.input_batch_stride > kMost || c.input_stride > kMost || c.out_batch_stride > kMost || c.out_stride > kMost ||
         (c.backward && (c.upstream_batch_stride > kMost || c.upstream_stride > kMost)) ||
+        !pcu_host::multiply_fits(c.input_batch_stride, c.batch, kMost) ||
+        !pcu_host::multiply_fits(c.out_batch_stride, c.batch, kMost) ||
+        (c.backward && !pcu_host::multiply_fits(c.upstream_batch_stride, c.batch, kMost)) ||
         !pcu_host::multiply_fits(c.input_stride, c.positions, kMost) ||
         !pcu_host::multiply_fits(c.out_stride, c.positions, kMost) ||
         (c.backward && !pcu_host::multiply_fits(c.upstream_stride, c.positions, kMost)))

@@ -214,10 +214,6 @@ def test_offsets_beyond_32_bits(provider):
     for strides in ((1 << 31, 64, 1), (64, 1 << 31, 1), (1 << 32, 1 << 31, 1)):
         far = base.as_strided((2, 2, 64), strides)
         far.copy_(x)
-        if strides[0] == 64:  # samples within the gaps of one another's rows are refused: rows may not interleave
-            with pytest.raises(provider.ProviderFailure):
-                provider.group_norm(far, 4, w, b, activation="silu")
-            continue
         out, stats = provider.group_norm(far, 4, w, b, activation="silu")
         e = lu.u(torch.float32) * 64
         lu.within(stats, want[1].double(), e * (1 + want[1].double().abs()))
@@ -227,6 +223,19 @@ def test_offsets_beyond_32_bits(provider):
         target = lu.norm_backward(x, dy, 4, want[1], w, b, "silu")
         for g, t, tol in zip(got, target, _backward_tolerances(x, dy, 4, want[1], w, b, "silu", torch.bfloat16, target)):
             lu.within(g, t, tol)
+
+
+@pytest.mark.parametrize("shape", [(6, 5, 64, 4), (3, 500, 48, 4), (2, 20000, 16, 2)])
+def test_positions_first(provider, shape):
+    """[positions, batch, channels] in memory, passed as [batch, positions, channels]: the same bits."""
+    x, dy, w, b = _data(shape, torch.float32, 13)
+    g = shape[3]
+    want, stats = provider.group_norm(x, g, w, b, activation="silu")
+    grads = provider.group_norm_backward(x, dy, g, stats, w, b, activation="silu")
+    xt, yt = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (x, dy))
+    out, stats2 = provider.group_norm(xt, g, w, b, activation="silu")
+    assert torch.equal(out, want) and torch.equal(stats, stats2)
+    assert all(torch.equal(p, q) for p, q in zip(grads, provider.group_norm_backward(xt, yt, g, stats, w, b, activation="silu")))
 
 
 def test_constant_groups(provider):

@@ -1,6 +1,9 @@
 """The learning operators together and beside the strict path: a distillation step of a network with a
 normalised layer, the guarded chain, and the Python layer's refusals."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -148,6 +151,65 @@ def test_guarded_chain_stops_at_a_learning_fault(provider):
     provider.group_norm(torch.zeros_like(x), 4, out=out, chain=c.stage(1))
     assert c.validate([128, 128]) == ("fault", 0, ((2 * 32) << 3) | 5)
     assert bool((out == 7).all())
+
+
+def test_first_calls_may_be_captured(provider):
+    """A process whose very first call of each operator is inside a graph capture."""
+    code = """
+import importlib, torch
+pcu = importlib.import_module("fusion-pcu_b200")
+torch.manual_seed(0)
+x = torch.randn((8, 900, 64), device="cuda"); z = torch.randn((3, 60000), device="cuda"); top, at = z.topk(8, dim=1)
+v = torch.randn((70, 512), device="cuda"); status = pcu.new_status()
+torch.cuda.synchronize()
+
+def calls():
+    y, stats = pcu.group_norm(x, 8, activation="gelu", status=status)
+    dx = pcu.group_norm_backward(x, x, 8, stats, activation="gelu", status=status)[0]
+    g = pcu.distill_loss_step(z, at, top, status=status)[2]
+    codes, scales = pcu.block_quantize(v, status=status)
+    w, ws = pcu.block_quantize(v, 128, status=status)
+    return y, dx, g, pcu.block_matmul(codes, scales, w, ws, status=status), pcu.block_matmul(codes[:4], scales[:4], w, ws, status=status)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(outs, calls())) and int(status[0]) == -1
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stdout + run.stderr
+
+
+def test_two_streams_at_once(provider):
+    """The operators keep no state between calls: the same calls on two streams at once, many times, give
+    the bits of one."""
+    gen = torch.Generator().manual_seed(4)
+    x = torch.randn((4, 2000, 64), generator=gen).cuda()
+    z = torch.randn((50, 70000), generator=gen).cuda()
+    top, at = z.topk(8, dim=1)
+    v = torch.randn((300, 512), generator=gen).cuda()
+    w, ws = provider.block_quantize(torch.randn((500, 512), generator=gen).cuda(), 128)
+
+    def calls(stream=None):
+        y, stats = provider.group_norm(x, 8, activation="silu", stream=stream)
+        dx = provider.group_norm_backward(x, x, 8, stats, activation="silu", stream=stream)[0]
+        g = provider.distill_loss_step(z, at, top, stream=stream)
+        codes, scales = provider.block_quantize(v, stream=stream)
+        return (y, dx) + g + (provider.block_matmul(codes, scales, w, ws, stream=stream),
+                              provider.block_matmul(codes[:8], scales[:8], w, ws, stream=stream))
+
+    want = calls()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[calls(s) for s in streams] for _ in range(5)]
+    torch.cuda.synchronize()
+    for both in got:
+        for outs in both:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
 def test_empty_stages_decide(provider):
