@@ -146,10 +146,18 @@ template <typename T> struct ProductParams {
     ChainGuard guard;
 };
 
-// A scale as the product takes it: a power of two from 2^-126 on, NaN for anything else.
-__device__ __forceinline__ float checked_scale(float scale) {
-    const unsigned bits = __float_as_uint(scale);
-    return (bits & 0x807fffffu) == 0 && bits >= 0x00800000u && bits < 0x7f800000u ? scale : NAN;
+// The factors of a block's product, scale x other scale = factor * rest: powers of two from 2^-126 on, so
+// exponents add, and what binary32 has no exponent for stays in `rest`, 1 otherwise.  (Multiplied, 2^64 by
+// 2^64 would be an infinity, and NaN with a product of 0.)  NaN for scales of any other kind.
+struct BlockFactor {
+    float factor, rest;
+};
+__device__ __forceinline__ BlockFactor block_factor(float scale, float other) {
+    auto good = [](unsigned bits) { return (bits & 0x807fffffu) == 0 && bits >= 0x00800000u && bits < 0x7f800000u; };
+    const unsigned a = __float_as_uint(scale), b = __float_as_uint(other);
+    if (!good(a) || !good(b)) return {NAN, 1.0f};
+    const int e = (int)(a >> 23) + (int)(b >> 23) - 127, near = min(max(e, 1), 254);
+    return {__uint_as_float((unsigned)near << 23), __uint_as_float((unsigned)(e - near + 127) << 23)};
 }
 
 template <typename T> __device__ __forceinline__ void store_cell(const ProductParams<T> &p, uint64_t r, uint64_t c, float v) {
@@ -215,8 +223,10 @@ template <typename T> __global__ void __launch_bounds__(256) product_plain_kerne
             for (int i = 0; i < 16; ++i) part = fmaf(sl[ty][i], sr[tx][i], part);
             __syncthreads();
         }
-        if (r < p.rows && c < p.columns)
-            acc += part * checked_scale(p.left_scales[r * blocks + kb]) * checked_scale(p.right_scales[c / kBlock * blocks + kb]);
+        if (r < p.rows && c < p.columns) {
+            const BlockFactor f = block_factor(p.left_scales[r * blocks + kb], p.right_scales[c / kBlock * blocks + kb]);
+            acc = fmaf(part * f.factor, f.rest, acc);
+        }
     }
     if (r < p.rows && c < p.columns) store_cell(p, r, c, acc);
 }
@@ -667,20 +677,21 @@ __global__ void __launch_bounds__(S::THREADS)
     } else {
         const int quarter = warp % 4, local = quarter * 32 + lane;  // this thread's row of the tile
         const uint64_t row = (uint64_t)p0 + local;
-        // Lane c holds the product of both operands' scales for the tile's column c, read one block ahead.
-        auto scale_of = [&](int kb) -> float {
+        // Lane c holds the factor of both operands' scales for the tile's column c, read one block ahead.
+        auto scale_of = [&](int kb) -> BlockFactor {
             return kb < kb1 && lane < S::BN && (uint64_t)q0 + lane < t.q_rows
-                       ? checked_scale(t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb]) * checked_scale(t.p_scales[(uint64_t)tp * t.blocks + kb])
-                       : 0.0f;
+                       ? block_factor(t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb], t.p_scales[(uint64_t)tp * t.blocks + kb])
+                       : BlockFactor{0.0f, 1.0f};
         };
-        float sum[S::BN], next = scale_of(kb0);
+        float sum[S::BN];
+        BlockFactor next = scale_of(kb0);
 #pragma unroll
         for (int i = 0; i < S::BN; ++i) sum[i] = 0;
         int it = 0;
         bool ok = true;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int b = it % S::BUFFERS;
-            const float factor = next;
+            const BlockFactor f = next;
             next = scale_of(kb + 1);
             if (!(ok = warp_wait(&ready[b], (it / S::BUFFERS) & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -690,8 +701,14 @@ __global__ void __launch_bounds__(S::THREADS)
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&drained[b]);
+            if (__any_sync(~0u, f.rest != 1.0f)) {
 #pragma unroll
-            for (int i = 0; i < S::BN; ++i) sum[i] = fmaf(__uint_as_float(v[i]), __shfl_sync(~0u, factor, i), sum[i]);
+                for (int i = 0; i < S::BN; ++i)
+                    sum[i] = fmaf(__uint_as_float(v[i]) * __shfl_sync(~0u, f.factor, i), __shfl_sync(~0u, f.rest, i), sum[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::BN; ++i) sum[i] = fmaf(__uint_as_float(v[i]), __shfl_sync(~0u, f.factor, i), sum[i]);
+            }
         }
         if (!ok) {
             if (lane == 0) record_fault(p.status, 0, kWatchdog);

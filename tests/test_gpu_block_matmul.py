@@ -210,6 +210,24 @@ def test_large_and_small_scales(provider, rows):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("rows,room", [(1, None), (20, None), (300, None), (5, 3)])
+@pytest.mark.parametrize("left,right,left_code,right_code", [(100, 100, 0.0, 1.0), (-70, -70, 448.0, 448.0),
+                                                             (70, 65, 2.0 ** -9, 2.0 ** -9), (-120, 127, 1.0, 448.0)])
+def test_scales_whose_product_has_no_exponent(provider, rows, room, left, right, left_code, right_code):
+    """2^left by 2^right is beyond binary32 (but for the last), the block's product is not: a power of two times
+    a sum of 128 equal products, exact."""
+    a, sa, b, sb = _operands(rows, 256, 140, 6, room)
+    a.view(torch.uint8)[:] = 0
+    a.view(torch.uint8)[:, :128] = torch.tensor(left_code).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    b.view(torch.uint8)[:] = torch.tensor(right_code).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    sa[:, 0], sb[:, 0], sa[:, 1], sb[:, 1] = 2.0 ** left, 2.0 ** right, 2.0 ** 100, 2.0 ** 100
+    status = provider.new_status()
+    out = provider.block_matmul(a, sa, b, sb, dtype=torch.float32, status=status)
+    want = math.ldexp(128 * left_code * right_code, left + right)
+    assert torch.equal(out.double(), torch.full_like(out, want, dtype=torch.float64))
+    assert status_word(status) == provider.STATUS_OK
+
+
 def test_empty(provider):
     f8 = torch.float8_e4m3fn
     z = torch.zeros((4, 0), dtype=torch.uint8, device="cuda").view(f8)
