@@ -87,7 +87,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill
             there = false;
         }
         place[j] = there ? (int)at : -1;
-        prob[j] = there ? t / (double)p.temperature : -INFINITY;
+        prob[j] = there ? t : -INFINITY;
         a_max = fmax(a_max, prob[j]);
     }
     a_max = block_max(a_max, scratch_d);
@@ -104,7 +104,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill
     }
     double mass = 0;
     for (int j = threadIdx.x; j < p.k; j += kDistillThreads)
-        if (place[j] >= 0) mass += exp(prob[j] - a_max);
+        if (place[j] >= 0) mass += exp((prob[j] - a_max) * p.t_inverse);
     mass = block_sum(mass, scratch_d);
     const double ln_mass = log(mass);
 
@@ -137,9 +137,9 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill
     for (int j = threadIdx.x; j < p.k; j += kDistillThreads) {
         if (place[j] < 0) continue;
         const double zj = (double)Elem<T>::load(z[place[j]]);
-        const double pj = exp(prob[j] - a_max) / mass;
+        const double a = (prob[j] - a_max) * p.t_inverse, pj = exp(a) / mass;
         if (pj > 0)
-            terms += pj * ((prob[j] - a_max - ln_mass) - ((zj - (double)m) / (double)p.temperature - log((double)s)));
+            terms += pj * ((a - ln_mass) - ((zj - (double)m) / (double)p.temperature - log((double)s)));
         chosen[j] = zj;
         prob[j] = pj;
     }
@@ -325,7 +325,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
             }
         }
 
-    // the teacher's entries: exponents t / T, -infinity for absent ones.  (One copy of the code for all of
+    // the teacher's entries: t, -infinity for absent ones (t / T could be an infinity where t - max t is not).  (One copy of the code for all of
     // them: what is not in the instruction cache comes slowly while the memory is busy.)
     double a_max = -INFINITY;
     int flags = 0;  // 1: an entry is present, 2: one is bad
@@ -337,7 +337,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         if (there && (index >= vocab || !isfinite(t))) flags |= 2, there = false;
         if (there) flags |= 1;
         place[j] = there ? (int)index : -1;
-        prob[j] = there ? t * t_inverse : -INFINITY;
+        prob[j] = there ? t : -INFINITY;
         a_max = fmax(a_max, prob[j]);
     }
     if (p.k > 32 * warp) {
@@ -357,8 +357,8 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         return;
     }
 
-    // The sums over the entries, with e_j = exp(a_j - a_max):
-    //   mass = sum e_j, lean = sum e_j (a_j - a_max), named = sum e_j z_j,
+    // The sums over the entries, with a_j = (t_j - max t) / T and e_j = exp(a_j):
+    //   mass = sum e_j, lean = sum e_j a_j, named = sum e_j z_j,
     // from which loss / (w T^2) = (lean - (named - m mass) / T) / mass + ln s - ln mass.  A table notes whether
     // an index appears twice (see the end).
     double mass = 0, lean = 0, named = 0;
@@ -366,7 +366,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     for (int j = tid; j < p.k; j += kDistillThreads) {
         const int at = place[j];
         if (at < 0) continue;
-        const double a = prob[j] - a_max, e = exp(a);
+        const double a = (prob[j] - a_max) * t_inverse, e = exp(a);
         mass += e;
         if (e > 0) lean += e * a;
         prob[j] = e;

@@ -178,6 +178,24 @@ def test_small_and_large_temperatures(provider):
     assert not loss.any() and not gradient.any() and bool((stats[:, 1] == 1).all())
 
 
+@pytest.mark.parametrize("vocab", [40, 300001])
+def test_teacher_beyond_the_range_of_its_exponents(provider, vocab):
+    """Teacher logits that a low temperature takes beyond binary64: only their differences count.  Two largest
+    ones, equal, and q uniform: the loss is T^2 (ln V - ln 2), the gradient T (1/V - 1/2) there and T/V elsewhere."""
+    t = float(torch.tensor(2.0 ** -120))
+    z = torch.zeros((1, vocab), dtype=torch.float64, device="cuda")
+    at = torch.tensor([[3, 17, 5, -1]], device="cuda")
+    top = torch.tensor([[1e290, 1e290, -1e290, 0.0]], dtype=torch.float64, device="cuda")
+    status = provider.new_status()
+    loss, _, gradient = provider.distill_loss_step(z, at, top, temperature=t, status=status)
+    want = torch.full_like(z, t / vocab)
+    want[0, 3] = want[0, 17] = t * (1 / vocab - 0.5)
+    eps = torch.finfo(torch.float64).eps
+    lu.within(loss, torch.full_like(loss, t * t * math.log(vocab / 2)), t * t * math.log(vocab) * 16 * eps)
+    lu.within(gradient, want, want.abs() * (16 + lu.chain(vocab)) * eps)
+    assert status_word(status) == provider.STATUS_OK
+
+
 @pytest.mark.parametrize("dtype,vocab", [(torch.float32, 600001), (torch.float64, 300000), (torch.bfloat16, 1000003)])
 def test_rows_longer_than_a_cluster_holds(provider, dtype, vocab):
     z, at, top, gen = _data((3, vocab, 20), dtype, 16)
