@@ -533,7 +533,10 @@ template <typename T, int V, int TENSORS> struct Slab {
         };
         if (C == 1) {
             levels = max(1, min(deep, (int)blockDim.x / wide)), each = (deep + levels - 1) / levels;
-            W *part_mean = scratch + 2 * deep * wide, *part_square = part_mean + levels * wide;
+            // Behind the threads' own shares, at most blockDim.x of each; a single part per channel takes the place
+            // of the channel's first share, which only its own thread reads.
+            W *part_mean = levels > 1 ? scratch + 2 * deep * wide : means;
+            W *part_square = levels > 1 ? part_mean + levels * wide : squares;
             for (int i = threadIdx.x; i < levels * wide; i += blockDim.x) {
                 const int part = i / wide, c = i - part * wide, from = min(deep, part * each), to = min(deep, from + each);
                 const W n = rows_in(part);

@@ -394,3 +394,11 @@ def test_parameter_gradients_alone_and_none(provider):
     want = provider.group_norm_backward(x, dy, 3, stats, ones, zeros)
     got = provider.group_norm_backward(x, dy, 3, stats, dweight=torch.empty_like(w), dbias=torch.empty_like(b))
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 90, 2664, 8), (1, 300, 1332, 4), (1, 200, 1022, 2), (3, 64, 4072, 8), (2, 50, 2280, 8)])
+def test_wide_blocks_of_odd_groups(provider, shape, dtype):
+    """Groups that end inside an access, in blocks of more channels than a CTA has threads."""
+    test_forward(provider, shape, dtype)
+    test_backward(provider, shape, dtype)
