@@ -101,6 +101,7 @@ constexpr int kQuantizeThreads = 256;
 
 template <typename T, int HIGH>
 __global__ void __launch_bounds__(kQuantizeThreads) quantize_kernel(const QuantizeParams<T> p) {
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     constexpr int kRows = kQuantizeThreads / 8, PASSES = HIGH == 1 ? 1 : HIGH / kRows;
     const unsigned across = (unsigned)((p.columns + kBlock - 1) / kBlock);
@@ -206,6 +207,7 @@ __device__ __forceinline__ void store_row(const ProductParams<T> &p, uint64_t ro
 
 // Any base and stride: 16 x 16 cells per CTA, one thread per cell.
 template <typename T> __global__ void __launch_bounds__(256) product_plain_kernel(const ProductParams<T> p) {
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     __shared__ float sl[16][17], sr[16][17];
     const uint64_t tiles = (p.columns + 15) / 16;
@@ -426,6 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(S::THREADS, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ TileParams<T> t) {
     const ProductParams<T> &p = t.out;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ unsigned char smem_raw[];
     unsigned char *const tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -609,6 +612,7 @@ __global__ void __launch_bounds__(S::THREADS)
     product_rows_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ TileParams<T> t) {
     const ProductParams<T> &p = t.out;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ unsigned char smem_raw[];
     unsigned char *const tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -767,10 +771,8 @@ static int quantize_typed(const void *input, uint64_t rows, uint64_t columns, ui
     const uint64_t blocks = (rows + high - 1) / high * ((columns + kBlock - 1) / kBlock);
     constexpr int kRows = kQuantizeThreads / 8;
     if (high == 1)
-        quantize_kernel<T, 1><<<(unsigned)((blocks + kRows - 1) / kRows), kQuantizeThreads, 0, stream>>>(p);
-    else
-        quantize_kernel<T, kBlock><<<(unsigned)blocks, kQuantizeThreads, 0, stream>>>(p);
-    return pcu_host::launch_status();
+        return pcu_host::launch_grid(quantize_kernel<T, 1>, (unsigned)((blocks + kRows - 1) / kRows), kQuantizeThreads, stream, p);
+    return pcu_host::launch_grid(quantize_kernel<T, kBlock>, (unsigned)blocks, kQuantizeThreads, stream, p);
 }
 
 // A map over rows x inner codes with boxes of one block of 128 by `high` rows.
@@ -804,8 +806,7 @@ static int launch_batch(const ProductParams<T> &p, const CUtensorMap &left, cons
     if (const int rc = pcu_host::allow_shared<product_kernel<T, S>>(S::SMEM_BYTES)) return rc;
     const TileParams<T> t = tile_params(p, false, S::BM, S::BN);
     const unsigned pairs = std::min(t.tiles, (unsigned)std::max(1, pcu_host::sm_count() / 2));
-    product_kernel<T, S><<<2 * pairs, S::THREADS, S::SMEM_BYTES, stream>>>(left, right, t);
-    return pcu_host::launch_status();
+    return pcu_host::launch_cluster(product_kernel<T, S>, 2 * pairs, S::THREADS, S::SMEM_BYTES, 0, stream, left, right, t);
 }
 
 template <typename T, typename S>
@@ -834,8 +835,7 @@ template <typename T> static int product_typed(const ProductParams<T> &p, cudaSt
             return few ? launch_batch<T, Batch<64>>(p, left, right, stream) : launch_batch<T, Batch<256>>(p, left, right, stream);
     }
     const uint64_t tiles = (p.rows + 15) / 16 * ((p.columns + 15) / 16);
-    product_plain_kernel<T><<<(unsigned)tiles, 256, 0, stream>>>(p);
-    return pcu_host::launch_status();
+    return pcu_host::launch_grid(product_plain_kernel<T>, (unsigned)tiles, 256, stream, p);
 }
 
 }  // namespace pcu

@@ -64,6 +64,7 @@ template <typename V> __device__ __forceinline__ V block_max(V v, V *scratch) {
 // Rows that no cluster holds: one CTA per row, which it reads twice.
 template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill_kernel(const DistillParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     __shared__ double scratch_d[kDistillThreads / 32];
     __shared__ W scratch_w[kDistillThreads / 32];
@@ -253,6 +254,7 @@ template <typename W> __device__ __forceinline__ void join(W &m, W &s, W m2, W s
 template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) distill_slice_kernel(const DistillParams<T> p) {
     using W = WideOf<T>;
     constexpr int V = 16 / sizeof(T), WARPS = kDistillThreads / 32;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t landed[kMostChunks];
@@ -616,8 +618,7 @@ static int launch_distill(DistillParams<T> p, uint64_t rows, cudaStream_t stream
     while (p.claims < 2 * p.k) p.claims *= 2;
     const uint64_t need = slice_bytes + (uint64_t)p.k * (sizeof(double) + sizeof(int)) + (uint64_t)p.claims * sizeof(int);
     if (slice_bytes > (uint64_t)kMostChunks * kChunk || need > 216 * 1024 || rows * ranks > 0x7fffffffull) {
-        distill_kernel<T><<<(unsigned)rows, kDistillThreads, 0, stream>>>(p);
-        return pcu_host::launch_status();
+        return pcu_host::launch_grid(distill_kernel<T>, (unsigned)rows, kDistillThreads, stream, p);
     }
     p.slice = (int)(slice_bytes / sizeof(T));
     p.slice_bytes = (uint32_t)slice_bytes;

@@ -253,6 +253,7 @@ template <int U, typename W> __device__ __forceinline__ void lanes_sum(W (&v)[U]
 template <typename T, int V, int K, int U>
 __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K * sizeof(WideOf<T>), false)) norm_warp_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     WarpGroup<T, V, K> at;
     if (!at.place(p)) return;
@@ -318,6 +319,7 @@ __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K
 template <typename T, int V, int K, int U>
 __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K * sizeof(WideOf<T>), true)) norm_warp_backward_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     WarpGroup<T, V, K> at;
     if (!at.place(p)) return;
@@ -622,6 +624,7 @@ template <typename T, int V, int TENSORS> struct Slab {
 
 template <typename T, int V> __global__ void __launch_bounds__(512, sizeof(WideOf<T>) == 8 ? 1 : 2) norm_slab_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ __align__(16) unsigned char smem[];
     Slab<T, V, 1> at;
@@ -690,6 +693,7 @@ template <typename T, int V> __global__ void __launch_bounds__(512, sizeof(WideO
 
 template <typename T, int V> __global__ void __launch_bounds__(512) norm_slab_backward_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;  // the same answer in every CTA of the grid
     extern __shared__ __align__(16) unsigned char smem[];
     Slab<T, V, 2> at;
@@ -777,6 +781,7 @@ template <typename T, int V> struct Stream {
 // (mean, sum of squares about it) of each channel over a chunk's rows: partial[n][chunk][channel][2].
 template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_stats_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     __shared__ W means[kNormThreads * V], squares[kNormThreads * V];
     const Stream<T, V> at(p);
@@ -833,6 +838,7 @@ template <typename W> __device__ __forceinline__ W norm_block_sum(W v, W *scratc
 // One CTA per (n, g): the group's statistics from its chunks'.  Also what a call without positions gets.
 template <typename T> __global__ void __launch_bounds__(kNormThreads) norm_join_stats_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     __shared__ W scratch[kNormThreads / 32];
     const uint64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups, parts = p.plan.chunks * p.width;
@@ -864,6 +870,7 @@ template <typename T> __global__ void __launch_bounds__(kNormThreads) norm_join_
 
 template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_apply_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     const Stream<T, V> at(p);
     if (!at.active) return;
@@ -886,6 +893,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
 // Sums of dz h and dz of each channel over a chunk's rows: partial[n][chunk][2][channel].
 template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_sums_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     __shared__ W scratch[kNormThreads * V];
     const Stream<T, V> at(p);
@@ -924,6 +932,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
 // One CTA per (n, g): c1 and c2 from its channels' sums.
 template <typename T> __global__ void __launch_bounds__(kNormThreads) norm_join_sums_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     __shared__ W scratch[kNormThreads / 32];
     const uint64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
@@ -943,6 +952,7 @@ template <typename T> __global__ void __launch_bounds__(kNormThreads) norm_join_
 
 template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) norm_stream_gradient_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     const Stream<T, V> at(p);
     if (!at.active) return;
@@ -967,6 +977,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
 // 32 channels by 32 threads each per CTA
 template <typename T> __global__ void __launch_bounds__(1024) norm_parameters_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
+    in_stream_order();
     if (!chain_admits(p.guard)) return;
     __shared__ W scratch[2][32][33];
     const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x % 32;
@@ -1140,8 +1151,7 @@ size_t workspace_size(int dtype, uint64_t batch, uint64_t positions, uint64_t ch
 
 #define PCU_LAUNCHED(call)               \
     do {                                 \
-        call;                            \
-        rc = pcu_host::launch_status();  \
+        rc = call;                       \
         if (rc) return rc;               \
         p.guard = chain_follow(p.guard); \
     } while (0)
@@ -1150,9 +1160,8 @@ template <typename T, int V, int K> int run_warp(NormParams<T> p, bool backward,
     constexpr int U = std::max(1, 16 / (V * K)), UB = std::max(1, 8 / (V * K));
     const uint64_t per = 32 / p.plan.lanes, warps = (p.groups + per - 1) / per * p.plan.slices;
     const unsigned blocks = (unsigned)((warps + kNormThreads / 32 - 1) / (kNormThreads / 32));
-    if (backward) norm_warp_backward_kernel<T, V, K, UB><<<blocks, kNormThreads, 0, stream>>>(p);
-    else norm_warp_kernel<T, V, K, U><<<blocks, kNormThreads, 0, stream>>>(p);
-    return pcu_host::launch_status();
+    if (backward) return pcu_host::launch_grid(norm_warp_backward_kernel<T, V, K, UB>, blocks, kNormThreads, stream, p);
+    return pcu_host::launch_grid(norm_warp_kernel<T, V, K, U>, blocks, kNormThreads, stream, p);
 }
 
 template <typename T, int V> int run_norm(NormParams<T> p, bool backward, cudaStream_t stream) {
@@ -1180,13 +1189,13 @@ template <typename T, int V> int run_norm(NormParams<T> p, bool backward, cudaSt
     } else {
         const unsigned grid = (unsigned)(p.batch * plan.tiles * plan.chunks), groups = (unsigned)(p.batch * p.groups);
         if (backward) {
-            PCU_LAUNCHED((norm_stream_sums_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
-            PCU_LAUNCHED((norm_join_sums_kernel<T><<<groups, kNormThreads, 0, stream>>>(p)));
-            PCU_LAUNCHED((norm_stream_gradient_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
+            PCU_LAUNCHED((pcu_host::launch_grid(norm_stream_sums_kernel<T, V>, grid, kNormThreads, stream, p)));
+            PCU_LAUNCHED((pcu_host::launch_grid(norm_join_sums_kernel<T>, groups, kNormThreads, stream, p)));
+            PCU_LAUNCHED((pcu_host::launch_grid(norm_stream_gradient_kernel<T, V>, grid, kNormThreads, stream, p)));
         } else {
-            PCU_LAUNCHED((norm_stream_stats_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
-            PCU_LAUNCHED((norm_join_stats_kernel<T><<<groups, kNormThreads, 0, stream>>>(p)));
-            PCU_LAUNCHED((norm_stream_apply_kernel<T, V><<<grid, kNormThreads, 0, stream>>>(p)));
+            PCU_LAUNCHED((pcu_host::launch_grid(norm_stream_stats_kernel<T, V>, grid, kNormThreads, stream, p)));
+            PCU_LAUNCHED((pcu_host::launch_grid(norm_join_stats_kernel<T>, groups, kNormThreads, stream, p)));
+            PCU_LAUNCHED((pcu_host::launch_grid(norm_stream_apply_kernel<T, V>, grid, kNormThreads, stream, p)));
         }
     }
     return PCU_B200_OK;
@@ -1239,12 +1248,10 @@ template <typename T> int typed_norm(const NormCall &c, const ChainGuard &guard)
         if (rc) return rc;
         p.guard = chain_follow(p.guard);
     } else if (!c.backward) {
-        norm_join_stats_kernel<T><<<(unsigned)(c.batch * c.groups), kNormThreads, 0, stream>>>(p);
-        return pcu_host::launch_status();
+        return pcu_host::launch_grid(norm_join_stats_kernel<T>, (unsigned)(c.batch * c.groups), kNormThreads, stream, p);
     }
     if (c.backward && (c.dweight || c.dbias)) {
-        norm_parameters_kernel<T><<<(unsigned)((c.channels + 31) / 32), 1024, 0, stream>>>(p);
-        rc = pcu_host::launch_status();
+        rc = pcu_host::launch_grid(norm_parameters_kernel<T>, (unsigned)((c.channels + 31) / 32), 1024, stream, p);
     }
     return rc;
 }

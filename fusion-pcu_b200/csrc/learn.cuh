@@ -109,6 +109,14 @@ template <typename T> __device__ __forceinline__ unsigned not_finite(uint4 raw) 
     return bad & sign;
 }
 
+// First in each kernel: waits for the grids before it in the stream (all of them, with what they wrote), and
+// lets the next one's CTAs be placed when all of this grid's are, so that a call's way in runs while the
+// call before it finishes.  Every thread passes here, whatever it does next.
+__device__ __forceinline__ void in_stream_order() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // 2^x.  binary32: the hardware's approximation (2 ulp), results below 2^-126 flushed to zero --
 // these are softmax terms, summed with one that is 1.  binary64: the library function.
 __device__ __forceinline__ float fast_exp2(float x) {

@@ -137,7 +137,8 @@ template <auto kernel> int allow_shared(int bytes, int registers = 0) {
     return PCU_B200_OK;
 }
 
-// A launch in clusters of `ranks` CTAs along x.
+// A launch of a kernel that begins with in_stream_order(), in clusters of `ranks` CTAs along x (0: as the
+// kernel says).
 template <typename... Params, typename... Args>
 int launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned block, size_t shared, unsigned ranks,
                    cudaStream_t stream, const Args &...args) {
@@ -146,17 +147,24 @@ int launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned block, siz
     config.blockDim = block;
     config.dynamicSmemBytes = shared;
     config.stream = stream;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = ranks;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = ranks;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = ranks ? 2 : 1;
     if (cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...); e != cudaSuccess) {
         (void)cudaGetLastError();
         return set_cuda_error(e);
     }
     return PCU_B200_OK;
+}
+
+template <typename... Params, typename... Args>
+int launch_grid(void (*kernel)(Params...), unsigned grid, unsigned block, cudaStream_t stream, const Args &...args) {
+    return launch_cluster(kernel, grid, block, 0, 0, stream, args...);
 }
 
 inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
