@@ -75,6 +75,8 @@ def _on_device(call):
     def wrapped(*args, **kwargs):
         torch = _torch()
         first = args[0] if args else kwargs[name]
+        if first.get_device() == torch._C._cuda_getDevice() and kwargs.get("stream") is None:  # -1: not on a GPU
+            return call(*args, **kwargs)
         if not first.is_cuda:
             raise ValueError(f"{name}: a CUDA tensor is wanted, got one on {first.device}")
         stream = kwargs.get("stream")
@@ -83,16 +85,15 @@ def _on_device(call):
                 raise ValueError(f"stream is on {stream.device}, {name} on {first.device}")
             with torch.cuda.stream(stream):
                 return call(*args, **kwargs)
-        if first.get_device() != torch._C._cuda_getDevice():
-            with torch.cuda.device(first.device):
-                return call(*args, **kwargs)
-        return call(*args, **kwargs)
+        with torch.cuda.device(first.device):
+            return call(*args, **kwargs)
     return wrapped
 
 
 def _want(name, t, like, shape=None, dtype=None):
     """`t` is a dense tensor of the given shape and type on the device of `like`."""
-    if t is None:
+    if t is None or (t.get_device() == like.get_device() and (dtype is None or t.dtype == dtype) and
+                     (shape is None or t.shape == shape) and t.is_contiguous()):
         return
     if not t.is_cuda or t.get_device() != like.get_device():
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
@@ -131,12 +132,13 @@ def _maps(name, t, like=None):
         raise ValueError(f"{name} is [batch, positions, channels] or [batch, channels], got {tuple(t.shape)}")
     if like is not None:
         _alike(name, t, like)
-    n, c = t.shape[0], t.shape[-1]
-    if t.dim() == 2:
-        s, batch_stride, stride = 1, t.stride(0), max(c, t.stride(0))
+    shape, strides = t.shape, t.stride()
+    n, c, batch_stride = shape[0], shape[-1], strides[0]
+    if len(shape) == 2:
+        s, stride = 1, max(c, batch_stride)
     else:
-        s, batch_stride, stride = t.shape[1], t.stride(0), t.stride(1)
-    if t.numel() and c > 1 and t.stride(-1) != 1:
+        s, stride = shape[1], strides[1]
+    if strides[-1] != 1 and c > 1 and n and s:
         raise ValueError(f"{name}: channels must be adjacent (channels last)")
     return n, s, c, batch_stride, stride
 
@@ -223,9 +225,10 @@ def _rows(name, t, like=None):
         raise ValueError(f"{name} is a matrix, got {tuple(t.shape)}")
     if like is not None:
         _alike(name, t, like)
-    if t.numel() and t.shape[1] > 1 and t.stride(1) != 1:
+    (rows, columns), (stride, step) = t.shape, t.stride()
+    if step != 1 and columns > 1 and rows:
         raise ValueError(f"{name}: columns must be adjacent")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return stride if rows > 1 else columns
 
 
 def _distill(logits, top_indices, top_logits, temperature, row_weights):
@@ -324,12 +327,16 @@ def distill_loss_step(logits, top_indices, top_logits, upstream=None, temperatur
 # ------------------------------------------------------------------ 8-bit block product
 
 def _codes(name, t, like=None):
-    torch = _torch()
-    if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+    if t.dtype not in _code_types():
         raise TypeError(f"{name} is {t.dtype}, float8_e4m3fn (or its bytes, uint8) is wanted")
-    if like is not None and (not t.is_cuda or t.get_device() != like.get_device()):
+    if like is not None and t.get_device() != like.get_device():
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
     return _rows(name, t)
+
+
+@functools.lru_cache(maxsize=None)
+def _code_types():
+    return frozenset((_torch().float8_e4m3fn, _torch().uint8))
 
 
 @_on_device
@@ -368,9 +375,8 @@ def block_matmul(left, left_scales, right, right_scales, out=None, dtype=None, s
     [rows, columns], of type `dtype` (bfloat16 by default, float16 or float32) when it is not given."""
     torch = _torch()
     left_stride, right_stride = _codes("left", left), _codes("right", right, left)
-    rows, inner = left.shape
-    columns = right.shape[0]
-    if right.shape[1] != inner:
+    (rows, inner), (columns, right_inner) = left.shape, right.shape
+    if right_inner != inner:
         raise ValueError(f"MatMulShape {tuple(left.shape)} {tuple(right.shape)}")
     blocks = -(-inner // 128)
     _want("left_scales", left_scales, left, (rows, blocks), torch.float32)
@@ -379,7 +385,7 @@ def block_matmul(left, left_scales, right, right_scales, out=None, dtype=None, s
         out = torch.empty((rows, columns), dtype=dtype or torch.bfloat16, device=left.device)
     elif dtype is not None and out.dtype != dtype:
         raise TypeError(f"out is {out.dtype}, {dtype} is wanted")
-    if out.dtype == torch.float64 or out.shape != (rows, columns) or not out.is_cuda or out.get_device() != left.get_device():
+    if out.dtype == torch.float64 or out.shape != (rows, columns) or out.get_device() != left.get_device():
         raise ValueError(f"out is a {rows} x {columns} float32/float16/bfloat16 matrix on {left.device}")
     code = _code(out)
     out_stride = _rows("out", out)
