@@ -689,37 +689,47 @@ __global__ void __launch_bounds__(S::THREADS)
     } else {
         const int quarter = warp % 4, local = quarter * 32 + lane;  // this thread's row of the tile
         const uint64_t row = (uint64_t)p0 + local;
-        // Lane c holds the factor of both operands' scales for the tile's column c, read one block ahead.
-        auto scale_of = [&](int kb) -> BlockFactor {
-            return kb < kb1 && lane < S::BN && (uint64_t)q0 + lane < t.q_rows
-                       ? block_factor(t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb], t.p_scales[(uint64_t)tp * t.blocks + kb])
-                       : BlockFactor{0.0f, 1.0f};
+        // Lane c holds both operands' scales for the tile's column c, AHEAD blocks ahead: a load that misses
+        // takes longer than a block.
+        constexpr int AHEAD = 4;
+        float sum[S::BN], p_scale[AHEAD], q_scale[AHEAD];
+        const bool there = lane < S::BN && (uint64_t)q0 + lane < t.q_rows;
+        auto fetch = [&](int kb, float &ps, float &qs) {
+            ps = qs = 1.0f;
+            if (kb < kb1 && there)
+                ps = __ldg(t.p_scales + (uint64_t)tp * t.blocks + kb), qs = __ldg(t.q_scales + ((uint64_t)q0 + lane) * t.blocks + kb);
         };
-        float sum[S::BN];
-        BlockFactor next = scale_of(kb0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fetch(kb0 + i, p_scale[i], q_scale[i]);
 #pragma unroll
         for (int i = 0; i < S::BN; ++i) sum[i] = 0;
         int it = 0;
         bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const int b = it % S::BUFFERS;
-            const BlockFactor f = next;
-            next = scale_of(kb + 1);
-            if (!(ok = warp_wait(&ready[b], (it / S::BUFFERS) & 1))) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t v[S::BN];
-            tmem_load(v, tmem + ((uint32_t)(quarter * 32) << 16) + b * S::BN);
-            tmem_wait(v);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&drained[b]);
-            if (__any_sync(~0u, f.rest != 1.0f)) {
+        static_assert(AHEAD == S::BUFFERS, "a block's place in the scales' ring is its buffer");
+        for (int kb = kb0; ok && kb < kb1;) {
 #pragma unroll
-                for (int i = 0; i < S::BN; ++i)
-                    sum[i] = fmaf(__uint_as_float(v[i]) * __shfl_sync(~0u, f.factor, i), __shfl_sync(~0u, f.rest, i), sum[i]);
-            } else {
+            for (int b = 0; b < S::BUFFERS; ++b) {
+                if (!ok || kb >= kb1) break;
+                const BlockFactor f = block_factor(q_scale[b], p_scale[b]);
+                fetch(kb + AHEAD, p_scale[b], q_scale[b]);
+                if (!(ok = warp_wait(&ready[b], (it / S::BUFFERS) & 1))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t v[S::BN];
+                tmem_load(v, tmem + ((uint32_t)(quarter * 32) << 16) + b * S::BN);
+                tmem_wait(v);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&drained[b]);
+                if (__any_sync(~0u, f.rest != 1.0f)) {
 #pragma unroll
-                for (int i = 0; i < S::BN; ++i) sum[i] = fmaf(__uint_as_float(v[i]), __shfl_sync(~0u, f.factor, i), sum[i]);
+                    for (int i = 0; i < S::BN; ++i)
+                        sum[i] = fmaf(__uint_as_float(v[i]) * __shfl_sync(~0u, f.factor, i), __shfl_sync(~0u, f.rest, i), sum[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < S::BN; ++i)
+                        sum[i] = fmaf(__uint_as_float(v[i]), __shfl_sync(~0u, f.factor, i), sum[i]);
+                }
+                ++kb, ++it;
             }
         }
         if (!ok) {
