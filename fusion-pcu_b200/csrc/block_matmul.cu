@@ -240,7 +240,7 @@ template <typename T> __global__ void __launch_bounds__(256) product_plain_kerne
 //   * batch form (product_kernel): P = left, Q = right.  A pair of CTAs works on 256 x 256 cells.
 //   * row form (product_rows_kernel), few rows: P = right, Q = left, 128 columns x BN rows, so that
 //     the weights, which are all the traffic there is, fill the instruction's 128 rows.  The blocks
-//     of one tile are split over a cluster's CTAs; the first CTA adds their sums, in rank order.  Each
+//     of one tile are split over a cluster's CTAs, which then add a share of the cells each, in rank order.  Each
 //     block's product goes to a TMEM buffer of its own and is added, scaled, to sums in registers.
 // All waits are bounded (mbar_wait); one that runs out records the watchdog kind, and the CTA still
 // waits for its own copies and products before it frees TMEM and returns.
@@ -738,7 +738,7 @@ __global__ void __launch_bounds__(S::THREADS)
 #pragma unroll
             for (int i = 0; i < S::BN; ++i)
                 if (row < t.p_rows && (uint64_t)q0 + i < t.q_rows) store_cell(p, (uint64_t)q0 + i, row, sum[i]);
-        } else {  // for the cluster's first CTA; every load and product of this CTA is done
+        } else {  // for the cluster; every load and product of this CTA is done
 #pragma unroll
             for (int i = 0; i < S::BN; ++i) reinterpret_cast<float *>(tiles)[i * S::BM + local] = sum[i];
         }
@@ -751,21 +751,19 @@ __global__ void __launch_bounds__(S::THREADS)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLUMNS) : "memory");
     if (ranks > 1) {
         cluster_sync();  // each CTA's sums are in its own shared memory
-        if (rank == 0) {
-            for (int i = threadIdx.x; i < S::BM * S::BN; i += S::THREADS) {
-                const uint64_t column = (uint64_t)p0 + i % S::BM, row = (uint64_t)q0 + i / S::BM;
-                if (column >= t.p_rows || row >= t.q_rows) continue;
-                float total = 0;
-                for (uint32_t r = 0; r < ranks; ++r) {
-                    float v;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                                 : "=f"(v)
-                                 : "r"(cluster_address(smem_addr(tiles) + 4 * i, r))
-                                 : "memory");
-                    total += v;
-                }
-                store_cell(p, row, column, total);
+        // Every CTA adds a share of the cells, in rank order; the reads of a cell's sums go out together.
+        for (int i = rank * S::THREADS + threadIdx.x; i < S::BM * S::BN; i += ranks * S::THREADS) {
+            const uint64_t column = (uint64_t)p0 + i % S::BM, row = (uint64_t)q0 + i / S::BM;
+            if (column >= t.p_rows || row >= t.q_rows) continue;
+            float part[8], total = 0;
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r) {
+                part[r] = 0;
+                if (r < ranks) cluster_read(part[r], smem_addr(tiles) + 4 * i, r);
             }
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r) total += part[r];
+            store_cell(p, row, column, total);
         }
         __syncwarp();
         cluster_sync();  // and stay until they have been read
