@@ -269,3 +269,49 @@ def test_python_refusals(provider):
     # arguments by name, the first one too
     assert torch.equal(provider.group_norm(x=x, groups=2)[0], provider.group_norm(x, 2)[0])
     assert status_word(provider.new_status()) == provider.STATUS_OK
+
+
+def _chained(provider, x, w, ws, logits, at, top, after=lambda: None):
+    """Calls that each need the one before, with buffers used again at once: an early start shows."""
+    codes = scales = norm = None
+    for _ in range(12):
+        codes, scales = provider.block_quantize(x, codes=codes, scales=scales)
+        after()
+        y = provider.block_matmul(codes, scales, w, ws, dtype=torch.float32)
+        after()
+        norm, stats = provider.group_norm(y, 4, activation="silu", out=norm)
+        after()
+        dx, _, _ = provider.group_norm_backward(y, norm, 4, stats, activation="silu", dx=y)
+        after()
+        _, row, gradient = provider.distill_loss_step(logits, at, top, upstream=dx[:, 0].contiguous(), gradient=logits)
+        after()
+        x = provider.group_norm(dx + gradient[:, :dx.shape[1]], 4, out=x)[0]
+        after()
+    return x, gradient
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_calls_keep_the_order_of_their_stream(provider, rows):
+    """The same bits whether each call has ended before the next is made, follows at once, or is replayed in a graph
+    with a fork and a join between them."""
+    gen = torch.Generator().manual_seed(rows)
+    x0 = torch.randn((rows, 512), generator=gen).cuda()
+    z0 = torch.randn((rows, 20000), generator=gen).cuda()
+    top, at = z0.topk(8, dim=1)
+    w, ws = provider.block_quantize(torch.randn((512, 512), generator=gen).cuda(), 128)
+    want = _chained(provider, x0.clone(), w, ws, z0.clone(), at, top, torch.cuda.synchronize)
+    got = _chained(provider, x0.clone(), w, ws, z0.clone(), at, top)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    x, z = x0.clone(), z0.clone()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        aside, _ = provider.group_norm(x0, 4, stream=side)
+        out = _chained(provider, x, w, ws, z, at, top)
+        torch.cuda.current_stream().wait_stream(side)
+        both = provider.group_norm(out[0] + aside, 4)[0]
+    for _ in range(3):
+        x.copy_(x0), z.copy_(z0)
+        graph.replay()
+    assert torch.equal(want[0], out[0]) and torch.equal(want[1], out[1])
+    assert torch.equal(both, provider.group_norm(want[0] + provider.group_norm(x0, 4)[0], 4)[0])
