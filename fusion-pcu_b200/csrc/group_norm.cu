@@ -984,13 +984,19 @@ template <typename T> __global__ void __launch_bounds__(1024) norm_parameters_ke
     const uint64_t split = p.plan.partial_split, rows = p.batch * p.positions ? p.plan.partial_rows : 0;
     W dw = 0, db = 0;
     if (c < p.channels) {
-        const W *from = p.partial + c / p.width * split * p.width + c % p.width;
-        const uint64_t whole = p.channels * split;
+        if (split == 1) {  // no divisions on the way to the loads
+            const W *at = p.partial + c + 2 * p.channels * (threadIdx.x / 32);
 #pragma unroll 4
-        for (uint64_t i = threadIdx.x / 32; i < rows * split; i += 32) {
-            const W *at = from + i / split * 2 * whole + i % split * p.width;
-            dw += at[0];
-            db += at[whole];
+            for (uint64_t i = threadIdx.x / 32; i < rows; i += 32, at += 64 * p.channels) dw += at[0], db += at[p.channels];
+        } else {
+            const W *from = p.partial + c / p.width * split * p.width + c % p.width;
+            const uint64_t whole = p.channels * split;
+#pragma unroll 4
+            for (uint64_t i = threadIdx.x / 32; i < rows * split; i += 32) {
+                const W *at = from + i / split * 2 * whole + i % split * p.width;
+                dw += at[0];
+                db += at[whole];
+            }
         }
     }
     scratch[0][threadIdx.x / 32][threadIdx.x % 32] = dw;
