@@ -12,10 +12,10 @@
 //   * stream form, for what fits neither: one pass for sums of row chunks, one that applies them.
 // Measured (graph replays, inputs beyond L2 or resident as a layer's are):
 //   warp form, 8192 x 4096, groups of 128, ReLU, F32: forward 51 us = 5.3 TB/s (0.80 of a copy's 6.55), backward
-//     84 us = 4.8 TB/s + 7 us for the parameters' gradients; bound by instruction issue (54 and 60 % of the
-//     slots taken, 22 warps an SM, the rest waits on fixed latencies), not by the memory;
-//   slab form, BF16, SiLU: forward 5 x 4095 x 320 16.6 us, one CTA an SM, a chain of load, sums, cluster, stores;
-//     backward 16 x 1024 x 640 34 us + 6 us, issue again: some 50 instructions an element, half of them the
+//     84 us = 4.8 TB/s + 6 us for the parameters' gradients; bound by instruction issue (54 and 60 % of the
+//     slots taken, 22 warps an SM, the rest waits on fixed latencies), not by the memory; BF16 39 and 84 us;
+//   slab form, BF16, SiLU: forward 5 x 4095 x 320 16.6 us (15.4 behind other calls), one CTA an SM, a chain of load, sums, cluster, stores;
+//     backward 16 x 1024 x 640 34 us + 5 us, issue again: some 50 instructions an element, half of them the
 //     SiLU slope, which is formed twice because dz does not fit beside x and dy;
 //   stream form: reads twice; 35 us against the slab form's 21 on a map that both take.
 // The variance is taken about the mean in every form (in the stream form within each thread about
