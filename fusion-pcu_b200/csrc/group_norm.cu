@@ -54,7 +54,7 @@ struct NormPlan {
     size_t slab_bytes, shared;  // of one tensor's slab; of the CTA
     unsigned tiles, tile, chunks;  // stream form: column tiles of `tile` accesses, row chunks
     uint64_t chunk_rows;
-    uint64_t partial_rows, partial_split;  // parameters' gradients: partial sums [rows][2][groups][split][width]
+    uint64_t partial_rows;                 // parameters' gradients: partial sums [rows][2][channels]
     uint64_t workspace;                    // elements of the wide type
 };
 
@@ -389,14 +389,40 @@ __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K
         stats += 2 * stride * p.groups;
     }
     if (!p.partial) return;
-    const uint64_t whole = p.groups * p.plan.items * V;
+    W *sums = p.partial + 2 * at.slice * p.channels;
+    if (p.positions == 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-        if (at.there[k]) {
-            W *sums = p.partial + 2 * at.slice * whole + (at.g * p.plan.items + at.sub + k * p.plan.lanes) * V;
+        for (int k = 0; k < K; ++k)
+            if (at.there[k]) {
+                W *mine = sums + at.g * p.width + (at.sub + k * p.plan.lanes) * V;
 #pragma unroll
-            for (int e = 0; e < V; ++e) sums[e] = dw[k][e], sums[whole + e] = db[k][e];
+                for (int e = 0; e < V; ++e) mine[e] = dw[k][e], mine[p.channels + e] = db[k][e];
+            }
+        return;
+    }
+    // The positions of each channel are summed here, through shared memory: the workspace, and the kernel that
+    // adds the slices, would have as many times the rows (138 x 61 x 82, 41 groups, F32: 115 us).
+    __shared__ W elements[kNormThreads / 32][32 * K * V];
+    W *mine = elements[threadIdx.x / 32];
+    const int lane = threadIdx.x % 32, width = (int)p.width, group = (int)p.plan.items * V;
+    const uint64_t g0 = at.g - lane / p.plan.lanes;
+    const int channels = (int)min((uint64_t)(32 / p.plan.lanes), p.groups - g0) * width;
+    auto give = [&](const W (&v)[K][V], W *to) {
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (at.there[k])
+#pragma unroll
+                for (int e = 0; e < V; ++e) mine[lane / p.plan.lanes * group + (at.sub + k * p.plan.lanes) * V + e] = v[k][e];
+        __syncwarp();
+        for (int i = lane; i < channels; i += 32) {
+            const int g = i / width;
+            W all = 0;
+            for (int at_ = g * group + i % width; at_ < (g + 1) * group; at_ += width) all += mine[at_];
+            to[g0 * width + i] = all;
         }
+    };
+    give(dw, sums), give(db, sums + p.channels);
 }
 
 // ---- columns: the thread mapping of the slab and stream forms
@@ -981,23 +1007,12 @@ template <typename T> __global__ void __launch_bounds__(1024) norm_parameters_ke
     if (!chain_admits(p.guard)) return;
     __shared__ W scratch[2][32][33];
     const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x % 32;
-    const uint64_t split = p.plan.partial_split, rows = p.batch * p.positions ? p.plan.partial_rows : 0;
+    const uint64_t rows = p.batch * p.positions ? p.plan.partial_rows : 0;
     W dw = 0, db = 0;
     if (c < p.channels) {
-        if (split == 1) {  // no divisions on the way to the loads
-            const W *at = p.partial + c + 2 * p.channels * (threadIdx.x / 32);
-#pragma unroll 4
-            for (uint64_t i = threadIdx.x / 32; i < rows; i += 32, at += 64 * p.channels) dw += at[0], db += at[p.channels];
-        } else {
-            const W *from = p.partial + c / p.width * split * p.width + c % p.width;
-            const uint64_t whole = p.channels * split;
-#pragma unroll 4
-            for (uint64_t i = threadIdx.x / 32; i < rows * split; i += 32) {
-                const W *at = from + i / split * 2 * whole + i % split * p.width;
-                dw += at[0];
-                db += at[whole];
-            }
-        }
+        const W *at = p.partial + c + 2 * p.channels * (threadIdx.x / 32);
+#pragma unroll 8
+        for (uint64_t i = threadIdx.x / 32; i < rows; i += 32, at += 64 * p.channels) dw += at[0], db += at[p.channels];
     }
     scratch[0][threadIdx.x / 32][threadIdx.x % 32] = dw;
     scratch[1][threadIdx.x / 32][threadIdx.x % 32] = db;
@@ -1057,7 +1072,6 @@ NormPlan plan_norm(int dtype, int vector, bool near, uint64_t batch, uint64_t po
     const uint64_t width = channels / groups, bytes = pcu_host::element_bytes(dtype), wide = dtype == PCU_B200_F64 ? 8 : 4;
     const uint64_t sms = (uint64_t)pcu_host::sm_count();
     p.vector = vector;
-    p.partial_split = 1;
     // Warp form: 16 elements of a lane are in registers (and as many of dy, and four parameters' worth), so
     // a group has at most 512 of them.
     if (near && width % vector == 0 && positions <= 512 && positions * (width / vector) * vector <= 512) {
@@ -1075,8 +1089,7 @@ NormPlan plan_norm(int dtype, int vector, bool near, uint64_t batch, uint64_t po
         // Each warp walks over a slice of the batch; as many warps as are resident at once.
         p.slices = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(batch, sms * ctas * (kNormThreads / 32) / sets));
         p.partial_rows = p.slices;
-        p.partial_split = positions;
-        p.workspace = backward ? 2 * p.partial_rows * channels * positions : 0;
+        p.workspace = backward ? 2 * p.partial_rows * channels : 0;
         return p;
     }
     // Slab form: blocks of whole groups whose rows are at least 128 bytes and whole accesses, in the
