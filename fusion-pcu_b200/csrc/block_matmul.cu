@@ -168,15 +168,14 @@ template <typename T> __device__ __forceinline__ void store_cell(const ProductPa
     if (const unsigned kind = result_kind(Elem<T>::load(y))) record_fault(p.status, r * p.columns + c, kind);
 }
 
-// COLUMNS cells of one row from `column` on, in 32-byte pieces (whole sectors: a warp's lanes are in 32
-// rows) where the row allows it.
+// COLUMNS cells of one row from `column` on, which lies on a 32-byte boundary, in pieces of that size (whole
+// sectors: a warp's lanes are in 32 rows).
 template <typename T, int COLUMNS>
 __device__ __forceinline__ void store_row(const ProductParams<T> &p, uint64_t row, uint64_t column,
                                           const uint32_t (&v)[COLUMNS]) {
     constexpr int V = 32 / sizeof(T);
     static_assert(COLUMNS % V == 0, "whole pieces");
     T *to = p.out + row * p.out_stride + column;
-    const bool whole = (reinterpret_cast<uintptr_t>(to) & 31) == 0;
 #pragma unroll
     for (int i = 0; i < COLUMNS; i += V) {
         if (column + i >= p.columns) break;
@@ -187,7 +186,7 @@ __device__ __forceinline__ void store_row(const ProductParams<T> &p, uint64_t ro
             y[j] = Elem<T>::round(__uint_as_float(v[i + j]));
             fine &= isfinite(Elem<T>::load(y[j]));
         }
-        if (whole && column + i + V <= p.columns) {
+        if (column + i + V <= p.columns) {
             const uint32_t *w = reinterpret_cast<const uint32_t *>(y);
             asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + i), "r"(w[0]), "r"(w[1]),
                          "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -202,6 +201,31 @@ __device__ __forceinline__ void store_row(const ProductParams<T> &p, uint64_t ro
             for (int j = 0; j < V; ++j)
                 if (const unsigned kind = result_kind(Elem<T>::load(y[j])); kind && column + i + j < p.columns)
                     record_fault(p.status, row * p.columns + column + i + j, kind);
+    }
+}
+
+// The same cells of a warp's 32 rows from `row` on (a lane's v: its row's), for a result whose rows lie anyhow: turned
+// in registers, so that adjacent lanes store adjacent columns (5536 x 764 x 11555, F16 out: 614 us without).
+template <typename T>
+__device__ __forceinline__ void store_turned(const ProductParams<T> &p, uint64_t row, uint64_t column, uint32_t (&v)[32]) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int s = 16; s; s >>= 1)
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (!(j & s)) {
+                const uint32_t got = __shfl_xor_sync(~0u, lane & s ? v[j] : v[j + s], s);
+                if (lane & s) v[j] = got;
+                else v[j + s] = got;
+            }
+    if (column + lane >= p.columns) return;
+    T *to = p.out + row * p.out_stride + column + lane;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        if (row + j >= p.rows) break;
+        const T y = Elem<T>::round(__uint_as_float(v[j]));
+        to[j * p.out_stride] = y;
+        if (const unsigned kind = result_kind(Elem<T>::load(y))) record_fault(p.status, (row + j) * p.columns + column + lane, kind);
     }
 }
 
@@ -560,6 +584,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(S::THREADS, 1)
         const int from = (warp - 4) / 4 * S::COLUMNS;               // its first column
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + from;
         const uint32_t drained0 = cluster_address(smem_addr(&drained), 0);
+        const bool pieces = ((reinterpret_cast<uintptr_t>(p.out) | p.out_stride * sizeof(T)) & 31) == 0;  // all rows alike
         int tile = 0;
         bool ok = true;
         for (unsigned id = first; id < t.tiles; id += step, ++tile) {
@@ -576,7 +601,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(S::THREADS, 1)
             unsigned tp, tq;
             tile_place(t, id, tp, tq);
             const uint64_t row = (uint64_t)tp * S::BM + rank * S::HALF + local;
-            if (row < t.p_rows) {
+            if (!pieces) {
+#pragma unroll
+                for (int i = 0; i < S::COLUMNS / 32; ++i)
+                    store_turned<T>(p, row - lane, (uint64_t)tq * S::BN + from + 32 * i, v[i]);
+            } else if (row < t.p_rows) {
 #pragma unroll
                 for (int i = 0; i < S::COLUMNS / 32; ++i) store_row<T, 32>(p, row, (uint64_t)tq * S::BN + from + 32 * i, v[i]);
             }
