@@ -10,6 +10,7 @@ worked on on their own device.  The reference has no counterpart of these operat
 """
 import functools
 import inspect
+import struct
 
 from . import _check, _rate_bits, _torch, library, new_status
 
@@ -20,8 +21,15 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 DISTILL_TOP_MAX = 1024
 
 # The kernels of small calls take a few microseconds, so the host's part is kept short: pointers go as
-# plain integers, devices are compared by index, what depends on numbers alone is remembered.
-_bits = functools.lru_cache(maxsize=None)(_rate_bits)
+# plain integers, devices are compared by index, workspace sizes are remembered by their arguments.
+_FLOAT, _WORD = struct.Struct("f"), struct.Struct("I")
+
+
+def _bits(value):
+    """The binary32 pattern of `value` as it is now.  Nothing is remembered: a 0-dimensional tensor is a number
+    whose value changes, 0.0 equals -0.0, and an annealed temperature is another number in each step.  A Python
+    float takes a short way (0.2 us against 1.8)."""
+    return _WORD.unpack(_FLOAT.pack(value))[0] if type(value) is float else _rate_bits(value)
 
 
 @functools.lru_cache(maxsize=None)
