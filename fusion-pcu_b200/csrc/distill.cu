@@ -203,8 +203,10 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill
 constexpr int kChunk = 16384;  // bytes per bulk copy, each with a barrier: 4 granules per thread
 
 // A running maximum and sum of 2^(c (x - m)).  With hi = c m rounded, c x - hi is one multiply-add;
-// the sum so formed is 2^d times the wanted one, d = hi - c m (known exactly), and it is set right at the end.
-// Where c m is 2^100 and more (or there is no maximum yet) the difference is taken first.
+// the sum so formed is 2^d times the wanted one, d = c m - hi (one multiply-add too), and it is set right at the end.
+// d is up to half of hi's last place: at most 1/2 below 2^24.  From there on, and where there is no maximum yet, the
+// difference is taken first, which costs one more instruction a term: 2^d grows until it leaves binary32, from hi =
+// 2^31 on (a mask of -1e10, or logits of 4 at a temperature of 1e-9).
 template <typename W> struct Running {
     W m, s, hi;
     bool far;
@@ -213,7 +215,7 @@ template <typename W> struct Running {
 __device__ __forceinline__ void refer(Running<float> &r, float m, float c) {
     r.m = m;
     r.hi = m * c;
-    r.far = !(fabsf(r.hi) < 0x1p100f);
+    r.far = !(fabsf(r.hi) < 0x1p24f);
     if (r.far) r.hi = 0.0f;
 }
 __device__ __forceinline__ void refer(Running<double> &r, double m, double) { r.m = m, r.far = true, r.hi = 0; }
@@ -232,7 +234,9 @@ template <typename W> __device__ __forceinline__ W term(const Running<W> &r, W x
 template <typename W> __device__ __forceinline__ void raise(Running<W> &r, W m, W c) {
     const Running<W> old = r;
     refer(r, m, c);
-    if (old.s != W(0)) r.s = old.s * (old.far || r.far ? fast_exp2((old.m - m) * c) : fast_exp2(old.hi - r.hi));
+    if (old.s != W(0))
+        r.s = old.far || r.far ? old.s / excess(old, c) * excess(r, c) * fast_exp2((old.m - m) * c)
+                               : old.s * fast_exp2(old.hi - r.hi);
 }
 
 __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
