@@ -37,6 +37,7 @@ template <typename T> struct DistillParams {
     int slice;            // elements of a row per CTA of its cluster (whole granules)
     uint32_t slice_bytes;
     int claims;           // places of the table of claimed indices: a power of two, at least 2 k
+    int chosen_at;        // where the logits that the teacher names lie, in doubles from the entries on
     unsigned long long *status;
     ChainGuard guard;
 };
@@ -263,7 +264,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t landed[kMostChunks];
     __shared__ W part_m[WARPS], part_s[WARPS], share[2];
-    __shared__ double part_a[WARPS], part_sums[3][WARPS];
+    __shared__ double part_a[WARPS], part_sums[2][WARPS];
     __shared__ int part_flags[WARPS], repeated;
     uint32_t ranks;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -282,6 +283,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     T *slice = reinterpret_cast<T *>(smem);  // element v at slice[lead + v - v0]
     double *prob = reinterpret_cast<double *>(smem + p.slice_bytes);
     int *place = reinterpret_cast<int *>(prob + p.k), *claimed = place + p.k;
+    T *chosen = reinterpret_cast<T *>(prob + p.chosen_at);  // with a loss; each thread reads what it wrote
     const int chunks = (granules * 16 + kChunk - 1) / kChunk;
     T *g = p.gradient ? p.gradient + row * p.gradient_stride : nullptr;
     const W weight = p.weights ? p.weights[row] : W(1), c = p.to_log2;
@@ -370,10 +372,10 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     }
 
     // The sums over the entries, with a_j = (t_j - max t) / T and e_j = exp(a_j):
-    //   mass = sum e_j, lean = sum e_j a_j, named = sum e_j z_j,
-    // from which loss / (w T^2) = (lean - (named - m mass) / T) / mass + ln s - ln mass.  A table notes whether
-    // an index appears twice (see the end).
-    double mass = 0, lean = 0, named = 0;
+    //   mass = sum e_j, lean = sum e_j (a_j - (z_j - m) / T),
+    // from which loss / (w T^2) = lean / mass + ln s - ln mass.  A table notes whether an index appears twice
+    // (see the end).
+    double mass = 0, lean = 0;
 #pragma unroll 1
     for (int j = tid; j < p.k; j += kDistillThreads) {
         const int at = place[j];
@@ -450,19 +452,17 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     }
     // The first CTA's loss takes the logits that the teacher names, those of other CTAs' slices before any
     // CTA overwrites them in place.
-    if (p.loss && rank == 0)
+    const bool losing = p.loss && rank == 0 && p.k > 32 * warp;
+    if (losing)
 #pragma unroll 1
         for (int j = tid; j < p.k; j += kDistillThreads) {
             const int at = place[j];
-            if (at >= 0 && prob[j] > 0) named += prob[j] * (double)Elem<T>::load(at < v1 ? slice[lead + at - v0] : z[at]);
+            if (at >= 0) chosen[j] = at < v1 ? slice[lead + at - v0] : z[at];
         }
     if (p.k > 32 * warp)
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            mass += __shfl_xor_sync(~0u, mass, o);
-            if (p.loss && rank == 0) lean += __shfl_xor_sync(~0u, lean, o), named += __shfl_xor_sync(~0u, named, o);
-        }
-    if (lane == 0) part_sums[0][warp] = mass, part_sums[1][warp] = lean, part_sums[2][warp] = named;
+        for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(~0u, mass, o);
+    if (lane == 0) part_sums[0][warp] = mass;
 
     if (!p.stats_in) {
         __syncthreads();
@@ -510,18 +510,17 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     const W up = p.upstream ? p.upstream[p.upstream_uniform ? 0 : row] : W(1);
     const bool invalid = (flags & 2) || !isfinite(m) || !isfinite(s) || !(s > W(0)) || !isfinite(weight) || (g && !isfinite(up));
     unsigned kind = invalid && tid == 0 ? (unsigned)PCU_B200_KIND_INVALID : 0u;
-    if (rank == 0 && tid == 0) {
-        if (p.loss) {
-            mass = over_warps(part_sums[0]), lean = over_warps(part_sums[1]), named = over_warps(part_sums[2]);
-            const double t = (double)p.temperature;
-            const W value = invalid ? W(NAN)
-                                    : (W)((double)weight * t * t *
-                                          ((lean - (named - (double)m * mass) * t_inverse) / mass + log((double)s) - log(mass)));
-            p.loss[row] = value;
-            if (!kind) kind = result_kind(value);
-        }
-        if (p.stats_out) p.stats_out[2 * row] = m, p.stats_out[2 * row + 1] = s;
+    if (rank == 0 && tid == 0 && p.stats_out) p.stats_out[2 * row] = m, p.stats_out[2 * row + 1] = s;
+    // Each z_j - m by itself: of logits that share a large offset the differences count, and sum e_j z_j - m mass
+    // would lose them (a row of -1e20 throughout had a loss of 1e4 for ln V - H(p)).
+    if (losing) {
+#pragma unroll 1
+        for (int j = tid; j < p.k; j += kDistillThreads)
+            if (place[j] >= 0 && prob[j] > 0) lean -= prob[j] * (((double)Elem<T>::load(chosen[j]) - (double)m) * t_inverse);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) lean += __shfl_xor_sync(~0u, lean, o);
     }
+    if (lane == 0) part_sums[1][warp] = lean;
     if (g && invalid) {
         fill(g, W(NAN));
     } else if (g) {
@@ -597,6 +596,16 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         }
         if (worst && !kind) kind = worst;
     }
+    if (p.loss && rank == 0) {
+        __syncthreads();
+        if (tid == 0) {
+            mass = over_warps(part_sums[0]), lean = over_warps(part_sums[1]);
+            const double t = (double)p.temperature;
+            const W value = invalid ? W(NAN) : (W)((double)weight * t * t * (lean / mass + log((double)s) - log(mass)));
+            p.loss[row] = value;
+            if (const unsigned lost = result_kind(value)) record_fault(p.status, row, lost);
+        }
+    }
     if (!ok) record_fault(p.status, 0, kWatchdog);
     if (kind) record_fault(p.status, row, kind);
     // nothing is left in flight towards this CTA's shared memory, and the cluster has read it
@@ -620,7 +629,8 @@ static int launch_distill(DistillParams<T> p, uint64_t rows, cudaStream_t stream
     const uint64_t slice_bytes = (bytes / 16 + ranks - 1) / ranks * 16;
     p.claims = 1;
     while (p.claims < 2 * p.k) p.claims *= 2;
-    const uint64_t need = slice_bytes + (uint64_t)p.k * (sizeof(double) + sizeof(int)) + (uint64_t)p.claims * sizeof(int);
+    p.chosen_at = p.k + (p.k + p.claims + 1) / 2;
+    const uint64_t need = slice_bytes + (uint64_t)p.chosen_at * sizeof(double) + (p.loss ? (uint64_t)p.k * sizeof(T) : 0);
     if (slice_bytes > (uint64_t)kMostChunks * kChunk || need > 216 * 1024 || rows * ranks > 0x7fffffffull) {
         return pcu_host::launch_grid(distill_kernel<T>, (unsigned)rows, kDistillThreads, stream, p);
     }
