@@ -193,6 +193,44 @@ __device__ __forceinline__ double root(double var, double eps) { return isfinite
 // A sum of squares that rounding made negative is 0; NaN stays.
 template <typename W> __device__ __forceinline__ W not_negative(W v) { return v < W(0) ? W(0) : v; }
 
+// The mean of each of `rows` rows' V channels, and the sum of squares about it, in one pass; 0 without rows.
+// next(x) brings the rows one by one.  Blocks of 16 rows are summed about the mean of the rows before them (the
+// first block about the first row): with d = x - mean, a block's sums s of d and q of d^2 and the rows n up to its
+// end, q - s^2 / n is what the block adds to the squares, both for it and for the mean's move by s / n.  A far first
+// row so costs the first block some digits and no more, where one sum about it over 7,000 rows left the squares
+// 2 % off.
+constexpr int kMomentRows = 16;
+template <int V, typename W, typename Next>
+__device__ __forceinline__ void row_moments(int rows, Next next, W (&mean)[V], W (&square)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) mean[e] = square[e] = W(0);
+    if (rows > 0) next(mean);
+    for (int done = 1; done < rows;) {
+        const int end = min(rows, (done / kMomentRows + 1) * kMomentRows);
+        W sum[V] = {}, squares[V] = {}, x[V];
+        // 16 elements on their way: more rows of 8 cost registers that other warps need (8 x 32768 x 320 BF16 188 us
+        // with two rows, 200 with four), single elements want more (300 x 2048 x 256 F32 in rows of 257 1367 us with
+        // 16 rows, 1567 with four)
+#pragma unroll 16 / V
+        for (; done < end; ++done) {
+            next(x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const W d = x[e] - mean[e];
+                sum[e] += d;
+                squares[e] += d * d;
+            }
+        }
+        const W inverse = W(1) / (W)done;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const W shift = sum[e] * inverse;
+            square[e] += not_negative(squares[e] - sum[e] * shift);
+            mean[e] += shift;
+        }
+    }
+}
+
 // ---- warp form
 //
 // `lanes` lanes hold a group, K accesses each; 32 / lanes adjacent groups per warp.  A warp keeps its
@@ -811,27 +849,16 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
     if (!chain_admits(p.guard)) return;
     __shared__ W means[kNormThreads * V], squares[kNormThreads * V];
     const Stream<T, V> at(p);
-    W first[V], sum[V] = {}, square[V] = {}, x[V];
-    int count = 0;
-    if (at.active)
-        for (uint64_t s = at.s0 + at.ty; s < at.s1; s += at.deep) {
-            Access<T, V>::load(p.x.at(at.n, s, at.c)).open(x);
+    W mean[V], square[V];
+    const T *from = p.x.at(at.n, at.s0 + at.ty, at.c);
+    const uint64_t stride = at.deep * p.x.row;
+    const int count = at.active && at.s0 + at.ty < at.s1 ? (int)((at.s1 - at.s0 - at.ty - 1) / at.deep + 1) : 0;
+    row_moments<V>(count, [&](W (&x)[V]) {
+        Access<T, V>::load(from).open(x);
+        from += stride;
+    }, mean, square);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (count == 0) first[e] = x[e];
-                const W d = x[e] - first[e];
-                sum[e] += d;
-                square[e] += d * d;
-            }
-            ++count;
-        }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int to = threadIdx.x * V + e;
-        const W shift = count ? sum[e] / (W)count : W(0);
-        means[to] = count ? first[e] + shift : W(0);
-        squares[to] = count ? not_negative(square[e] - sum[e] * shift) : W(0);
-    }
+    for (int e = 0; e < V; ++e) means[threadIdx.x * V + e] = mean[e], squares[threadIdx.x * V + e] = square[e];
     __syncthreads();
     const uint64_t rows = at.s1 - at.s0;
     for (int i = threadIdx.x; i < at.across * V; i += kNormThreads) {
