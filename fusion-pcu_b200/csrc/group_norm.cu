@@ -18,8 +18,9 @@
 //     backward 16 x 1024 x 640 34 us + 5 us, issue again: some 50 instructions an element, half of them the
 //     SiLU slope, which is formed twice because dz does not fit beside x and dy;
 //   stream form: reads twice; 35 us against the slab form's 21 on a map that both take.
-// The variance is taken about the mean in every form (in the stream form within each thread about
-// its first element, joined about the joint means).
+// The variance is taken about the mean in every form: the warp form has it before it sums the squares; a thread of
+// the slab and stream forms takes its rows' about the mean of those before (row_moments), and threads, channels,
+// CTAs and chunks are joined about their joint means.
 #include <algorithm>
 #include <numeric>
 
@@ -194,20 +195,22 @@ __device__ __forceinline__ double root(double var, double eps) { return isfinite
 template <typename W> __device__ __forceinline__ W not_negative(W v) { return v < W(0) ? W(0) : v; }
 
 // The mean of each of `rows` rows' V channels, and the sum of squares about it, in one pass; 0 without rows.
-// next(x) brings the rows one by one.  Blocks of 16 rows are summed about the mean of the rows before them (the
-// first block about the first row): with d = x - mean, a block's sums s of d and q of d^2 and the rows n up to its
-// end, q - s^2 / n is what the block adds to the squares, both for it and for the mean's move by s / n.  A far first
-// row so costs the first block some digits and no more, where one sum about it over 7,000 rows left the squares
-// 2 % off.
-constexpr int kMomentRows = 16;
-template <int V, typename W, typename Next>
+// next(x) brings the rows one by one.  A block of rows is summed about the mean of the rows before it (the first
+// about the first row): with d = x - mean, a block's sums s of d and q of d^2 and the rows n up to its end, q - s^2 / n
+// is what the block adds to the squares, both for it and for the mean's move by s / n.  A far first row so costs the
+// first block some digits and no more, where one sum about it over 7,000 rows left the squares 2 % off.
+// LONG, for thousands of rows: blocks of 16, each one's squares summed by themselves.  Else, for up to some hundred:
+// blocks that end at 32, 256, ... rows, on top of the squares before them (most threads have fewer than 32 rows;
+// blocks of 16 cost a forward pass of 16 x 4095 x 1280 BF16 1.5 %).
+template <int V, bool LONG, typename W, typename Next>
 __device__ __forceinline__ void row_moments(int rows, Next next, W (&mean)[V], W (&square)[V]) {
 #pragma unroll
     for (int e = 0; e < V; ++e) mean[e] = square[e] = W(0);
     if (rows > 0) next(mean);
     for (int done = 1; done < rows;) {
-        const int end = min(rows, (done / kMomentRows + 1) * kMomentRows);
-        W sum[V] = {}, squares[V] = {}, x[V];
+        const int end = min(rows, LONG ? (done / 16 + 1) * 16 : done < 32 ? 32 : 8 * done);
+        W sum[V] = {}, block[V] = {}, x[V];
+        W(&squares)[V] = LONG ? block : square;
         // 16 elements on their way: more rows of 8 cost registers that other warps need (8 x 32768 x 320 BF16 188 us
         // with two rows, 200 with four), single elements want more (300 x 2048 x 256 F32 in rows of 257 1367 us with
         // 16 rows, 1567 with four)
@@ -225,7 +228,8 @@ __device__ __forceinline__ void row_moments(int rows, Next next, W (&mean)[V], W
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const W shift = sum[e] * inverse;
-            square[e] += not_negative(squares[e] - sum[e] * shift);
+            const W about = not_negative(squares[e] - sum[e] * shift);
+            square[e] = LONG ? square[e] + about : about;
             mean[e] += shift;
         }
     }
@@ -695,35 +699,15 @@ template <typename T, int V> __global__ void __launch_bounds__(512, sizeof(WideO
     at.place(p, smem);
     const uint64_t c = at.channel();
     const unsigned bg = p.plan.block_groups;
-    W mean[V] = {}, r[V] = {};
+    W mean[V], r[V];
     const int step = at.step();
     at.bring(0, p.x);
     asm volatile("cp.async.wait_all;" ::: "memory");
-    // Sums about the thread's first row: with few rows a thread, even a far first element costs them no
-    // digits that count.
-    if (at.active && at.ty < at.rows) {
-        const T *from = at.mine[0];
-        W first[V], x[V];
-        at.read(from, first);
-        int count = 1;
-        for (int i = at.ty + at.deep; i < at.rows; i += at.deep, ++count) {
-            from += step;
-            at.read(from, x);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const W d = x[e] - first[e];
-                mean[e] += d;
-                r[e] += d * d;
-            }
-        }
-        const W inverse = W(1) / (W)count;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const W shift = mean[e] * inverse;
-            r[e] = not_negative(r[e] - mean[e] * shift);
-            mean[e] = first[e] + shift;
-        }
-    }
+    const T *row = at.mine[0];
+    row_moments<V, false>(at.active && at.ty < at.rows ? (at.rows - at.ty - 1) / at.deep + 1 : 0, [&](W (&x)[V]) {
+        at.read(row, x);
+        row += step;
+    }, mean, r);
     if (at.width % V == 0) at.template moments<1>(mean, r, p);
     else at.template moments<V>(mean, r, p);
     if (at.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // read; see the end
@@ -853,7 +837,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
     const T *from = p.x.at(at.n, at.s0 + at.ty, at.c);
     const uint64_t stride = at.deep * p.x.row;
     const int count = at.active && at.s0 + at.ty < at.s1 ? (int)((at.s1 - at.s0 - at.ty - 1) / at.deep + 1) : 0;
-    row_moments<V>(count, [&](W (&x)[V]) {
+    row_moments<V, true>(count, [&](W (&x)[V]) {
         Access<T, V>::load(from).open(x);
         from += stride;
     }, mean, square);

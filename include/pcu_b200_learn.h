@@ -49,7 +49,8 @@ extern "C" {
  * pattern, not negative.  stats receives (mean, r) for each (n, group), wide, 2 * batch * groups.
  * ReLU's slope at z = 0 is 0.  channels must be a multiple of groups; batch and
  * positions may be 0.  out has its own strides and may be input itself (same strides).
- * The variance is summed about the mean, never as a difference of two sums.
+ * The variance is not the mean of x^2 less the square of the mean: its squares are taken about the mean, or,
+ * where rows are read once, about the mean of the rows before, a block of rows at a time.
  * Events: the element's index (n * positions + s) * channels + c in out.  A group that holds a NaN
  * or an infinity gives NaN throughout.
  * Device workspace: pcu_b200_group_norm_workspace_size bytes (may be 0). */
