@@ -14,7 +14,9 @@
  *   - F16 and BF16 tensors are taken beside F32 and F64.  The arithmetic on F16, BF16 and F32 is in
  *     binary32 ("wide" below: F32 for these three, F64 for F64) and rounds once, to nearest even,
  *     where a result is stored.
- *   - There is no underflow policy: results underflow gradually, softmax terms below 2^-126 are 0.
+ *   - There is no underflow policy: results underflow gradually.  Factors that are 0 below 2^-126: softmax
+ *     terms, SiLU's 1 / (1 + exp(-z)) and the normal density in GELU's slope, so that SiLU and its slope
+ *     are 0 from z = -87.3 on, where they are -1.1e-36.  (In F64 that quotient is 0 below 2^-1024.)
  *   - Faults: a result that is not finite is recorded as InvalidFloatingOperand when it is NaN and
  *     as ArithmeticOverflow when it is an infinity; the events are given with each call.
  *   - Buffers must not overlap except where a call says so, and are aligned to their elements
