@@ -32,7 +32,7 @@ template <typename T> __device__ __forceinline__ void load_codes_input(const T *
         constexpr int V = 16 / sizeof(T);
 #pragma unroll
         for (int i = 0; i < 16; i += V) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(from + i));
+            const uint4 raw = *reinterpret_cast<const uint4 *>(from + i);
             const T *t = reinterpret_cast<const T *>(&raw);
 #pragma unroll
             for (int j = 0; j < V; ++j) v[i + j] = Elem<T>::load(t[j]);
@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(S::THREADS)
         auto fetch = [&](int kb, float &ps, float &qs) {
             ps = qs = 1.0f;
             if (kb < kb1 && there)
-                ps = __ldg(t.p_scales + (uint64_t)tp * t.blocks + kb), qs = __ldg(t.q_scales + ((uint64_t)q0 + lane) * t.blocks + kb);
+                ps = t.p_scales[(uint64_t)tp * t.blocks + kb], qs = t.q_scales[((uint64_t)q0 + lane) * t.blocks + kb];
         };
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) fetch(kb0 + i, p_scale[i], q_scale[i]);

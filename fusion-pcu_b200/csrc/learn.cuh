@@ -111,7 +111,9 @@ template <typename T> __device__ __forceinline__ unsigned not_finite(uint4 raw) 
 
 // First in each kernel: waits for the grids before it in the stream (all of them, with what they wrote), and
 // lets the next one's CTAs be placed when all of this grid's are, so that a call's way in runs while the
-// call before it finishes.  Every thread passes here, whatever it does next.
+// call before it finishes.  Every thread passes here, whatever it does next.  What calls read is loaded with
+// coherent loads (no __ldg): a kernel is there before its predecessor has written, so its inputs are not constant
+// for as long as it runs, which non-coherent loads want.
 __device__ __forceinline__ void in_stream_order() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
