@@ -37,7 +37,6 @@ template <typename T> struct DistillParams {
     int slice;            // elements of a row per CTA of its cluster (whole granules)
     uint32_t slice_bytes;
     int claims;           // places of the table of claimed indices: a power of two, at least 2 k
-    int chosen_at;        // where the logits that the teacher names lie, in doubles from the entries on
     unsigned long long *status;
     ChainGuard guard;
 };
@@ -282,8 +281,7 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     const int whole0 = lead ? 1 : 0, whole1 = (lead + count) / V;  // granules [whole0, whole1) are not cut
     T *slice = reinterpret_cast<T *>(smem);  // element v at slice[lead + v - v0]
     double *prob = reinterpret_cast<double *>(smem + p.slice_bytes);
-    int *place = reinterpret_cast<int *>(prob + p.k), *claimed = place + p.k;
-    T *chosen = reinterpret_cast<T *>(prob + p.chosen_at);  // with a loss; each thread reads what it wrote
+    int *place = reinterpret_cast<int *>(prob + p.k), *claimed = place + (p.k + 1) / 2 * 2;
     const int chunks = (granules * 16 + kChunk - 1) / kChunk;
     T *g = p.gradient ? p.gradient + row * p.gradient_stride : nullptr;
     const W weight = p.weights ? p.weights[row] : W(1), c = p.to_log2;
@@ -451,14 +449,14 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
         if (lane == 0) part_m[warp] = m, part_s[warp] = s;
     }
     // The first CTA's loss takes the logits that the teacher names, those of other CTAs' slices before any
-    // CTA overwrites them in place.
+    // CTA overwrites them in place: a thread's first one is kept in a register, further ones in the table's place.
     const bool losing = p.loss && rank == 0 && p.k > 32 * warp;
-    if (losing)
-#pragma unroll 1
-        for (int j = tid; j < p.k; j += kDistillThreads) {
-            const int at = place[j];
-            if (at >= 0) chosen[j] = at < v1 ? slice[lead + at - v0] : z[at];
-        }
+    auto named = [&](int j) {
+        const int at = place[j];
+        return at < 0 ? Elem<T>::round(W(0)) : at < v1 ? slice[lead + at - v0] : z[at];
+    };
+    T first_named = Elem<T>::round(W(0)), *further_named = reinterpret_cast<T *>(claimed) - kDistillThreads;
+    if (losing && tid < p.k) first_named = named(tid);
     if (p.k > 32 * warp)
 #pragma unroll
         for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(~0u, mass, o);
@@ -466,6 +464,9 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
 
     if (!p.stats_in) {
         __syncthreads();
+        if (losing)
+#pragma unroll 1
+            for (int j = tid + kDistillThreads; j < p.k; j += kDistillThreads) further_named[j] = named(j);
         // One warp joins the warps' shares, and the cluster's: always the same tree, so the same bits in
         // every CTA.
         auto joined = [&](int shares) {
@@ -515,8 +516,10 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads, 3) dist
     // would lose them (a row of -1e20 throughout had a loss of 1e4 for ln V - H(p)).
     if (losing) {
 #pragma unroll 1
-        for (int j = tid; j < p.k; j += kDistillThreads)
-            if (place[j] >= 0 && prob[j] > 0) lean -= prob[j] * (((double)Elem<T>::load(chosen[j]) - (double)m) * t_inverse);
+        for (int j = tid; j < p.k; j += kDistillThreads) {
+            const double zj = (double)Elem<T>::load(j == tid ? first_named : further_named[j]);
+            if (place[j] >= 0 && prob[j] > 0) lean -= prob[j] * ((zj - (double)m) * t_inverse);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) lean += __shfl_xor_sync(~0u, lean, o);
     }
@@ -629,8 +632,7 @@ static int launch_distill(DistillParams<T> p, uint64_t rows, cudaStream_t stream
     const uint64_t slice_bytes = (bytes / 16 + ranks - 1) / ranks * 16;
     p.claims = 1;
     while (p.claims < 2 * p.k) p.claims *= 2;
-    p.chosen_at = p.k + (p.k + p.claims + 1) / 2;
-    const uint64_t need = slice_bytes + (uint64_t)p.chosen_at * sizeof(double) + (p.loss ? (uint64_t)p.k * sizeof(T) : 0);
+    const uint64_t need = slice_bytes + (uint64_t)p.k * sizeof(double) + (uint64_t)((p.k + 1) / 2 * 2 + p.claims) * sizeof(int);
     if (slice_bytes > (uint64_t)kMostChunks * kChunk || need > 216 * 1024 || rows * ranks > 0x7fffffffull) {
         return pcu_host::launch_grid(distill_kernel<T>, (unsigned)rows, kDistillThreads, stream, p);
     }

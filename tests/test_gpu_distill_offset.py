@@ -48,3 +48,17 @@ def test_named_entries_that_are_masked(provider, named, dtype):
     near = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -50
     limit = near + (72 + lu.chain(5000) + 8) * e + 64 * 2.0 ** -50 + 4 * e * want[0][[0, 2]].abs()
     lu.within(loss[[0, 2]], want[0][[0, 2]], limit)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("k", [255, 257, 1023, 1024])
+@pytest.mark.parametrize("vocab", [1500, 131071])
+def test_loss_of_many_entries_with_the_gradient_in_place(provider, vocab, k, dtype):
+    """Named logits lie in other blocks' slices, which the gradient overwrites: the same bits as apart."""
+    z, at, top, gen = _data((6, vocab, k), dtype, 34)
+    want = provider.distill_loss_step(z, at, top, temperature=1.5)
+    _check(provider, z, at, top, 1.5, dtype)
+    for _ in range(5):
+        a = z.clone()
+        got = provider.distill_loss_step(a, at, top, temperature=1.5, gradient=a)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
