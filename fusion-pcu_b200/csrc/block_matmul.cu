@@ -93,7 +93,7 @@ template <typename T> struct QuantizeParams {
     ChainGuard guard;
 };
 
-// Bound by memory: 16384 x 4096 F32 with blocks of 128 rows 55 us = 6.1 TB/s, 0.93 of a copy; 8192 x 4096 BF16 with
+// Bound by memory: 16384 x 4096 F32 with blocks of 128 rows 53 us = 6.3 TB/s, 0.96 of a copy; 8192 x 4096 BF16 with
 // blocks of one row 20 us = 5.0 TB/s.  Eight threads take a row's 128 elements of a block, 16 each, and keep them in registers between
 // the maximum and the codes, so the input is read once.  HIGH 1: a block is such a row, 32 blocks per
 // CTA.  HIGH 128: a CTA takes a block, 4 rows per thread.
@@ -261,7 +261,8 @@ template <typename T> __global__ void __launch_bounds__(256) product_plain_kerne
 // ------------------------------------------------------------------ tensor core product
 //
 // D = P . Q^T over blocks of 128 of the inner dimension.
-//   * batch form (product_kernel): P = left, Q = right.  A pair of CTAs works on 256 x 256 cells.
+//   * batch form (product_kernel): P = left, Q = right.  A pair of CTAs works on 256 x 256 cells, whose sums over
+//     all blocks, scaled by the tensor cores, stay in TMEM.
 //   * row form (product_rows_kernel), few rows: P = right, Q = left, 128 columns x BN rows, so that
 //     the weights, which are all the traffic there is, fill the instruction's 128 rows.  The blocks
 //     of one tile are split over a cluster's CTAs, which then add a share of the cells each, in rank order.  Each
@@ -623,7 +624,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(S::THREADS, 1)
 
 // ---- row form
 //
-// 1 x 4096 x 16384 with its quantiser: 18.8 us for 64 MB of codes, 10.3 of them at a copy's rate; 32 rows 24.7.  Two CTAs
+// 1 x 4096 x 16384 with its quantiser: 18.8 us for 64 MB of codes (17.2 behind other passes), 10.3 of them at a copy's rate;
+// 32 rows 24.7 (21.3).  Two CTAs
 // an SM with 5 blocks of 18 KB in flight each.  What is left is the way in and out (two launches, TMEM, the first
 // loads, the cluster's sums): six stages, or three CTAs an SM with four, leave one row at 18.7 to 19.0 us.
 template <int BN_> struct Rows {

@@ -185,11 +185,11 @@ template <typename T> __global__ void __launch_bounds__(kDistillThreads) distill
 
 // ---- rows in shared memory
 //
-// Measured: a step over 4096 x 131072 BF16 524 us, 4.1 TB/s of the 6.55 that a copy reaches; 777 x 50003 F32 74 us;
-// backward alone, 2048 x 32768 BF16, 57 us = 4.8 TB/s; a loss of 4 rows of 131072 8.3 us, mostly the launch.
+// Measured: a step over 4096 x 131072 BF16 512 us, 4.2 TB/s of the 6.55 that a copy reaches; 777 x 50003 F32 72 us;
+// backward alone, 2048 x 32768 BF16, 54 us = 5.0 TB/s; a loss of 4 rows of 131072 6.8 us, mostly the launch.
 // What bounds it is each CTA's chain: of some 24,000 cycles 10,000 are spent until the slice has landed and is
-// summed, 5,000 on joining (warps, cluster, the teacher's exponentials), 6,500 on the gradient, and three CTAs
-// per SM, all that shared memory holds, cover each other's gaps only in part; 51 % of the issue slots are taken.
+// summed, up to 5,000 on joining (warps, cluster, the teacher's exponentials; the loss's own sums follow the gradient),
+// 6,500 on the gradient, and three CTAs per SM, all that shared memory holds, cover each other's gaps only in part.
 //
 // A cluster of 1, 2, 4 or 8 CTAs takes a row, each a slice of the vocabulary that stays in its shared
 // memory: bulk copies bring it in once, the running maximum and sum are taken as it lands, the CTAs

@@ -11,11 +11,11 @@
 //   * slab form: a block of whole groups of one n sits in the shared memory of a cluster of CTAs;
 //   * stream form, for what fits neither: one pass for sums of row chunks, one that applies them.
 // Measured (graph replays, inputs beyond L2 or resident as a layer's are):
-//   warp form, 8192 x 4096, groups of 128, ReLU, F32: forward 51 us = 5.3 TB/s (0.80 of a copy's 6.55), backward
-//     84 us = 4.8 TB/s + 6 us for the parameters' gradients; bound by instruction issue (54 and 60 % of the
-//     slots taken, 22 warps an SM, the rest waits on fixed latencies), not by the memory; BF16 39 and 84 us;
-//   slab form, BF16, SiLU: forward 5 x 4095 x 320 16.6 us (15.4 behind other calls), one CTA an SM, a chain of load, sums, cluster, stores;
-//     backward 16 x 1024 x 640 34 us + 5 us, issue again: some 50 instructions an element, half of them the
+//   warp form, 8192 x 4096, groups of 128, ReLU, F32: forward 49 us = 5.5 TB/s (0.84 of a copy's 6.55), backward
+//     87 us = 4.6 TB/s with the parameters' gradients; 54 and 60 % of the issue slots are taken by 22 warps an SM,
+//     which the registers leave: too few to cover each other's latencies; BF16 39 and 84 us;
+//   slab form, BF16, SiLU: forward 5 x 4095 x 320 15.7 us, one CTA an SM, a chain of load, sums, cluster, stores;
+//     backward 16 x 1024 x 640 36 us, 52 % of the slots by 22 % of the warps: some 50 instructions an element, half of them the
 //     SiLU slope, which is formed twice because dz does not fit beside x and dy;
 //   stream form: reads twice; 35 us against the slab form's 21 on a map that both take.
 // The variance is taken about the mean in every form: the warp form has it before it sums the squares; a thread of
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kNormThreads, K > 4 ? 1 : warp_form_ctas(V * K
         return;
     }
     // The positions of each channel are summed here, through shared memory: the workspace, and the kernel that
-    // adds the slices, would have as many times the rows (138 x 61 x 82, 41 groups, F32: 115 us).
+    // adds the slices, would have as many times the rows (138 x 61 x 82, 41 groups, F32: 96 us for 21).
     __shared__ W elements[kNormThreads / 32][32 * K * V];
     W *mine = elements[threadIdx.x / 32];
     const int lane = threadIdx.x % 32, width = (int)p.width, group = (int)p.plan.items * V;
@@ -1010,7 +1010,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kNormThreads) nor
     }
 }
 
-// ---- the parameters' gradients from partial sums [rows][2][groups][split][width], in a fixed order:
+// ---- the parameters' gradients from partial sums [rows][2][channels], in a fixed order:
 // 32 channels by 32 threads each per CTA
 template <typename T> __global__ void __launch_bounds__(1024) norm_parameters_kernel(const NormParams<T> p) {
     using W = WideOf<T>;
