@@ -624,10 +624,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(S::THREADS, 1)
 
 // ---- row form
 //
-// 1 x 4096 x 16384 with its quantiser: 18.8 us for 64 MB of codes (17.2 behind other passes), 10.3 of them at a copy's rate;
-// 32 rows 24.7 (21.3).  Two CTAs
-// an SM with 5 blocks of 18 KB in flight each.  What is left is the way in and out (two launches, TMEM, the first
-// loads, the cluster's sums): six stages, or three CTAs an SM with four, leave one row at 18.7 to 19.0 us.
+// 1 x 4096 x 16384 with its quantiser: 18.8 us for 64 MB of codes (17.2 behind other passes), 10.3 of them at a copy's
+// rate; 32 rows 24.7 (21.3).  Two CTAs an SM with 5 blocks of 18 KB in flight each.  What is left is the way in and out
+// (two launches, TMEM, the first loads, the cluster's sums): six stages, or three CTAs an SM with four, leave one row
+// at 18.7 to 19.0 us.
 template <int BN_> struct Rows {
     static constexpr int BM = 128, BN = BN_, BUFFERS = 4, EPILOGUE = 4, THREADS = (2 + EPILOGUE) * 32;
     static constexpr int TMEM_COLUMNS = BUFFERS * BN;
